@@ -342,6 +342,29 @@ int pgm_lomb_scargle_fast_f64(const double* t, const double* y, const double* dy
                               double f0, double df, int64_t nf, int fit_mean, int oversampling,
                               double* scratch, double* power, void* stream);
 
+/*
+ * Norm of a set of gradients and its clipping (no counterpart in the reference: what a user of pgmuvi/trainers.py:177-182 would
+ * put between `loss.backward()` and `optimizer.step()`):
+ *     n = (sum |g|^p)^(1/p) over all entries of all tensors,   c = min(1, max_norm / (n + 1e-6)),   out = c g,
+ * for each of `batch` members by itself (batch 1: one model; otherwise every tensor has a leading axis of `batch` members).
+ * The tensors are described by HOST arrays of `count` entries:
+ *   in_host / out_host  device addresses (out_host NULL: the norm only; out_host[t] == in_host[t]: in place);
+ *   numel_host          entries per member;       type_host   0 fp64, 1 fp32, 2 bf16, 3 fp16 (mixed sets are fine);
+ *   member_host         [count][2] distance between members of in / out, in entries (may be NULL for batch 1);
+ *   layout_host         NULL, or [count][12]: four sizes, four strides of in, four of out (entries, outermost first) of a tensor
+ *                       whose entries per member are not one contiguous run; first size 0 = they are.
+ * p: 1, 2 or 0 (largest magnitude).  max_norm >= 0 (infinity: nothing is clipped).  norm: [batch] fp64 (norm_f64 != 0) or fp32,
+ * device.  scratch: pgm_grad_scratch_doubles(batch, count) doubles of device memory owned by the caller, used by this call only.
+ * Sums are fp64; fp64 tensors' squares are held in three ranges, so that the norm neither overflows nor vanishes where the
+ * result does not.  A NaN norm makes every output NaN, an infinite one zero (NaN where the gradient is infinite).  Memory that
+ * is written must not be shared with another tensor of the call (-12; interleaved columns of one buffer are fine).
+ * Nothing is kept between calls; the call may be captured.  -98: out of host memory.
+ */
+int64_t pgm_grad_scratch_doubles(int batch, int count);
+int pgm_grad_clip(int batch, int count, const uint64_t* in_host, const uint64_t* out_host, const int64_t* numel_host,
+                  const unsigned char* type_host, const int64_t* member_host, const int64_t* layout_host, int p,
+                  double max_norm, void* norm, int norm_f64, double* scratch, int64_t scratch_doubles, void* stream);
+
 /* fp64 MFMA issue-rate probe (TFLOP/s of back-to-back v_mfma_f64_16x16x4_f64 on
  * every CU); used once by bench.py to report the measured peak beside the
  * datasheet figure.  Synchronises. */

@@ -70,6 +70,9 @@ SYMBOLS = {
     "pgm_lomb_scargle_fast_scratch_doubles": (c_int64, [c_int64, c_int64, c_int]),
     "pgm_lomb_scargle_fast_f64": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_double, c_double, c_int64, c_int, c_int,
                                           c_void_p, c_void_p, c_void_p]),
+    "pgm_grad_scratch_doubles": (c_int64, [c_int, c_int]),
+    "pgm_grad_clip": (c_int, [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_double, c_void_p, c_int,
+                              c_void_p, c_int64, c_void_p]),
 }
 
 

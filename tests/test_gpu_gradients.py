@@ -1,0 +1,268 @@
+"""GPU tests of gradient norms and clipping against sums in exact arithmetic (``math.fsum``) on the CPU.
+
+Tolerances, from the arithmetic: the norm's sum of n squares is formed in fp64 by chains of at most CHAIN(n) additions (a
+thread's share of at least 2048 x 256 threads or of one workgroup, then trees), each off by half a step, the square by another:
+relative error of the sum <= (CHAIN + 2) 2^-53, of its root half of that plus a rounding.  A clipped entry carries the factor's
+error (norm, sum, division: 3 roundings) and one rounding to its own type, half a step relative to the value
+(fp64 2^-53, fp32 2^-24, bf16 2^-8, fp16 2^-11 or 2^-25 absolute below its normal range).
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from pgmuvi_amd import gradients as G
+
+HALF_STEP = {torch.float64: 2.0 ** -53, torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float64: 2.0 ** -1075, torch.float32: 2.0 ** -150, torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("-m gpu tests need the MI355X")
+    return torch.device("cuda:0")
+
+
+def _norm_tol(n, out_dtype):
+    chain = 64 + n / 1024
+    return (chain + 4) * 2.0 ** -53 + (2.0 ** -24 if out_dtype is torch.float32 else 0.0)
+
+
+def _exact(arrays, p):
+    """Norm of float64 arrays (exact sum; squares scaled so that none overflows)."""
+    if p == math.inf:
+        return max(float(np.abs(a).max()) for a in arrays if a.size)
+    if p == 1:
+        return math.fsum(float(v) for a in arrays for v in np.abs(a).reshape(-1))
+    top = max((float(np.abs(a).max()) for a in arrays if a.size), default=0.0)
+    if top == 0.0:
+        return 0.0
+    return top * math.sqrt(math.fsum((float(v) / top) ** 2 for a in arrays for v in a.reshape(-1)))
+
+
+def _cpu(t):
+    return t.detach().double().cpu().numpy()
+
+
+def _check_clip(grads, outs, before, norm, max_norm, p=2):
+    want = _exact(before, p)
+    n = sum(b.size for b in before)
+    tol = _norm_tol(n, norm.dtype)
+    assert abs(float(norm) - want) <= tol * want
+    c = min(1.0, max_norm / (want + 1e-6))
+    for o, b in zip(outs, before):
+        err = np.abs(_cpu(o) - c * b)
+        bound = (_norm_tol(n, torch.float64) + 4 * 2.0 ** -53 + HALF_STEP[o.dtype] * (1 + 2.0 ** -12)) * np.abs(c * b) + TINY[o.dtype]
+        assert (err <= bound).all(), float((err - bound).max())
+
+
+def _make(shapes, dtype, seed, scale=1.0, dev="cuda"):
+    gen = torch.Generator().manual_seed(seed)
+    return [(torch.randn(s, generator=gen, dtype=torch.float64) * scale).to(dtype).to(dev) for s in shapes]
+
+
+SETS = {
+    "one": [(1,)], "scalar": [()], "fit": [(), (4,), (4, 1, 1), (4, 1, 1), (1,)], "odd": [(1,), (3, 5), (0,), (255,), (257,), (1023,), (7, 11, 13)],
+    "wg": [(8191,), (1,)], "past_one_wg": [(8193,), (1,), (2047,)], "two_launches": [(n % 7 + 1,) for n in range(130)],
+    "large": [(100003,), (1,), (65536,), (33,)],
+}
+
+
+@pytest.mark.parametrize("p", [1, 2, math.inf])
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("name", list(SETS))
+def test_norm_and_clip(dev, name, dtype, p):
+    grads = _make(SETS[name], dtype, 11, dev=dev)
+    before = [_cpu(g) for g in grads]
+    want = _exact(before, p)
+    norm = G.total_norm(grads, p)
+    assert norm.dtype is (torch.float64 if dtype is torch.float64 else torch.float32) and norm.shape == ()
+    assert abs(float(norm) - want) <= _norm_tol(sum(b.size for b in before), norm.dtype) * want
+    for max_norm in (0.5 * want, 2.0 * want):                    # (clipped; left alone)
+        outs = [torch.full_like(g, 7.0) for g in grads]
+        got = G.clip_grads_(grads, max_norm, p, out=outs)
+        assert float(got) == float(norm)
+        _check_clip(grads, outs, before, got, max_norm, p)
+        assert all((_cpu(g) == b).all() for g, b in zip(grads, before))      # (out of place: the gradients stay)
+    got = G.clip_grads_(grads, 0.5 * want, p)
+    _check_clip(grads, grads, before, got, 0.5 * want, p)
+
+
+def test_mixed_types_share_one_norm(dev):
+    grads = [_make([(1000 + i,)], t, 3 + i, dev=dev)[0] for i, t in enumerate(HALF_STEP)]
+    before = [_cpu(g) for g in grads]
+    norm = G.clip_grads_(grads, 1.5)
+    assert norm.dtype is torch.float64
+    _check_clip(grads, grads, before, norm, 1.5)
+
+
+@pytest.mark.parametrize("scale", [1e-320, 1e-300, 1e-160, 1e-140, 1e140, 1e160, 1e305])
+def test_norms_over_the_whole_range_of_fp64(dev, scale):
+    for n in (17, 100_000):
+        g = _make([(n,)], torch.float64, 5, dev=dev)[0]
+        g = (g * 2.0 ** -4) * scale if scale > 1 else g * scale
+        g[n // 2:] *= 1e-3
+        want = _exact([_cpu(g)], 2)
+        got = float(G.total_norm([g]))
+        assert abs(got - want) <= _norm_tol(n, torch.float64) * want + 2.0 ** -1074
+    mixed = torch.tensor([1e200, 1e-200, 3.0, 1e200], dtype=torch.float64, device=dev)
+    assert abs(float(G.total_norm([mixed])) / (math.sqrt(2.0) * 1e200) - 1) < 4 * 2.0 ** -53
+
+
+@pytest.mark.parametrize("p", [1, 2, math.inf])
+@pytest.mark.parametrize("n", [9, 50_000])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_nonfinite_gradients(dev, value, n, p):
+    grads = _make([(n,), (3,)], torch.float64, 2, dev=dev)
+    grads[0][n // 3] = value
+    ref = [g.clone() for g in grads]
+    norm = G.total_norm(grads, p)
+    assert math.isnan(float(norm)) if math.isnan(value) else float(norm) == math.inf
+    with pytest.raises(RuntimeError, match="not finite"):
+        G.clip_grads_(grads, 1.0, p, error_if_nonfinite=True)
+    assert all(torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) for a, b in zip(grads, ref))     # (untouched)
+    G.clip_grads_(grads, 1.0, p)
+    flat = torch.cat([g.reshape(-1) for g in grads])
+    if math.isnan(value):
+        assert bool(torch.isnan(flat).all())
+    else:
+        assert bool(torch.isnan(flat[n // 3])) and int((flat != 0).sum()) == 1         # (0 times infinity; every other entry zero)
+
+
+def test_zero_and_limits(dev):
+    z = [torch.zeros(5, dtype=torch.float64, device=dev), torch.zeros(0, dtype=torch.float64, device=dev)]
+    assert float(G.clip_grads_(z, 1.0)) == 0.0 and int((z[0] != 0).sum()) == 0
+    assert float(G.total_norm([z[1]])) == 0.0
+    g = _make([(40,)], torch.float64, 1, dev=dev)
+    keep = g[0].clone()
+    G.clip_grads_(g, math.inf)
+    assert torch.equal(g[0], keep)
+    G.clip_grads_(g, 0.0)
+    assert int((g[0] != 0).sum()) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("batch, n", [(1, 5), (2, 40_000), (7, 1), (3, 9000), (40, 2049), (513, 300), (600, 3001)])
+def test_members(dev, batch, n, dtype):
+    grads = _make([(batch, 4), (batch, 4, 1), (batch,), (batch, n)], dtype, 23, dev=dev)
+    for g in grads:
+        g.mul_(torch.logspace(0, -3, batch, device=dev).to(dtype).reshape((batch,) + (1,) * (g.dim() - 1)))
+    grads[3][batch - 1] = 0
+    before = [_cpu(g) for g in grads]
+    norm = G.total_norm(grads, members=True)
+    assert norm.shape == (batch,)
+    max_norm = 0.3
+    got = G.clip_grads_(grads, max_norm, members=True)
+    assert torch.equal(got, norm)
+    for b in sorted({0, batch // 2, batch - 1}):
+        rows = [np.asarray(a[b]) for a in before]
+        _check_clip(None, [g[b] for g in grads], rows, got[b], max_norm)
+
+
+def test_a_member_does_not_depend_on_its_company(dev):
+    grads = _make([(700, 4), (700, 2000)], torch.float64, 9, dev=dev)
+    alone = [g[5:6].clone() for g in grads]
+    all_norms = G.total_norm(grads, members=True)
+    assert abs(float(G.total_norm(alone, members=True)) / float(all_norms[5]) - 1) <= 2 * _norm_tol(2004, torch.float64)
+    nan_mate = [g.clone() for g in grads]
+    nan_mate[1][6] = math.nan
+    n2 = G.clip_grads_(nan_mate, 1.0, members=True)
+    G.clip_grads_(grads, 1.0, members=True)
+    keep = [i for i in range(700) if i != 6]
+    assert torch.equal(n2[keep], all_norms[keep]) and bool(torch.isnan(n2[6]))
+    assert all(torch.equal(a[keep], b[keep]) for a, b in zip(nan_mate, grads))
+
+
+def test_strides_and_views(dev):
+    buf = _make([(50, 13)], torch.float64, 4, dev=dev)[0]
+    ref = buf.clone()
+    cols = [buf[:, :4], buf[:, 4:5], buf[:, 6:]]                 # column 5 belongs to nobody
+    norm = G.clip_grads_(cols, 0.2, members=True)
+    want = torch.cat([ref[:, :5], ref[:, 6:]], 1).norm(dim=1)
+    assert float((norm / want - 1).abs().max()) < 32 * 2.0 ** -53
+    c = torch.clamp(0.2 / (want + 1e-6), max=1.0)[:, None]
+    assert float((buf - torch.where(torch.arange(13, device=dev) == 5, ref, ref * c)).abs().max()) <= 64 * 2.0 ** -53 * float(ref.abs().max())
+    assert torch.equal(buf[:, 5], ref[:, 5])
+    for t in (torch.randn(300, 70, device=dev, dtype=torch.float64).t(), torch.randn(9, 40, 30, device=dev)[::2, :, 1:28:3], torch.randn(8001, device=dev)[1:].bfloat16()[1:],
+              torch.randn(4, 3, 5, 6, device=dev).permute(3, 1, 0, 2)):
+        b = _cpu(t)
+        outs = [torch.zeros(t.shape, dtype=t.dtype, device=dev)]
+        norm = G.clip_grads_([t], 0.5, out=outs)
+        _check_clip(None, outs, [b], norm, 0.5)
+        G.clip_grads_([t], 0.5)
+        assert torch.equal(t, outs[0])
+    e = torch.randn(5, device=dev).expand(7, 5)
+    assert abs(float(G.total_norm([e])) / float(e.double().norm()) - 1) < 2.0 ** -23
+    with pytest.raises(ValueError, match="share memory"):
+        G.clip_grads_([e], 1.0)
+    g = torch.randn(5, device=dev)
+    with pytest.raises(ValueError, match="share memory"):
+        G.clip_grads_([g, g], 1.0)
+    assert abs(float(G.total_norm([g, g])) / (math.sqrt(2) * float(g.double().norm())) - 1) < 2.0 ** -23
+
+
+def test_parameters_and_torch_agree(dev):
+    ps = [torch.nn.Parameter(p) for p in _make([(4,), (4, 1), (200, 30)], torch.float64, 6, dev=dev)] + [torch.nn.Parameter(torch.zeros(2, device=dev))]
+    for i, p in enumerate(ps[:3]):
+        p.grad = torch.sin(p.detach() * 40 + i)
+    ref = [p.grad.clone() for p in ps[:3]]
+    n = G.clip_grad_norm_(ps, 0.7)
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps[:3]]
+    for q, r in zip(qs, ref):
+        q.grad = r
+    m = torch.nn.utils.clip_grad_norm_(qs, 0.7)
+    assert abs(float(n) / float(m) - 1) < 1e-13 and ps[3].grad is None
+    assert all(float((p.grad - q.grad).abs().max()) < 1e-14 for p, q in zip(ps, qs))
+
+
+@pytest.mark.parametrize("n", [20, 300_000])
+def test_streams_and_a_replayed_graph(dev, n):
+    g = _make([(n,), (5,)], torch.float64, 8, dev=dev)
+    want = [x.clone() for x in g]
+    want_norm = G.clip_grads_(want, 0.5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    mine = [x.clone() for x in g]
+    with torch.cuda.stream(side):
+        norm = G.clip_grads_(mine, 0.5)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(norm, want_norm) and all(torch.equal(a, b) for a, b in zip(mine, want))
+    static, out = [x.clone() for x in g], [torch.empty_like(x) for x in g]
+    with torch.cuda.stream(side):
+        G.clip_grads_(static, 0.5, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    norms = []
+    for graph in graphs:                                         # two graphs of the same call: neither leans on the other's scratch memory
+        with torch.cuda.graph(graph):
+            norms.append(G.clip_grads_(static, 0.5, out=out))
+    for k in range(4):
+        for s, x in zip(static, g):
+            s.copy_(x * (k + 1))
+        for o in out:
+            o.zero_()
+        graphs[k % 2].replay()
+        eager = [torch.empty_like(x) for x in g]
+        e = G.clip_grads_([x * (k + 1) for x in g], 0.5, out=eager)
+        torch.cuda.synchronize()
+        assert torch.equal(norms[k % 2], e) and all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+def test_repeated_calls_give_the_same_bits(dev):
+    grads = _make([(1_000_003,), (17,), (40_000,)], torch.float64, 12, dev=dev)
+    first = G.total_norm(grads)
+    for _ in range(3):
+        assert torch.equal(G.total_norm(grads), first)
+
+
+def test_more_than_32_bits_of_offset(dev):
+    rows = torch.zeros(2, (1 << 31) + 5, dtype=torch.bfloat16, device=dev)
+    rows[0, -1], rows[1, 0], rows[1, -2] = 3.0, 4.0, 12.0
+    norm = G.total_norm([rows], members=True)
+    assert norm.tolist() == [3.0, float(torch.tensor(math.sqrt(160.0)).float())]
+    G.clip_grads_([rows], 6.5 - 1e-6, members=False)             # (norm 13: factor one half, to 1e-7)
+    assert rows[0, -1] == 1.5 and rows[1, 0] == 2.0 and rows[1, -2] == 6.0 and float(rows[1, 5:-2].abs().max()) == 0.0
