@@ -365,6 +365,26 @@ int pgm_grad_clip(int batch, int count, const uint64_t* in_host, const uint64_t*
                   const unsigned char* type_host, const int64_t* member_host, const int64_t* layout_host, int p,
                   double max_norm, void* norm, int norm_f64, double* scratch, int64_t scratch_doubles, void* stream);
 
+/*
+ * Draws from rows of log-weights with tempering and truncation, from given random numbers: starts of a multi-modal fit or of the
+ * sampler's chains from the frequency posterior of a periodogram (pgmuvi/lightcurve.py:5516-5541 takes the highest peaks only).
+ * Row b (type 0 fp64, 1 fp32, 2 bf16, 3 fp16; entries col_stride apart, rows row_stride apart, in entries): with the best value m,
+ *   z_i = (l_i - m) / temperature, w_i = exp z_i (-inf and NaN weigh nothing); in the order (value descending, index ascending)
+ *   A = the first top_k (0: all), P = the shortest beginning of A with at least top_p of A's weight (1: all of A), kept = the
+ *   entries of P with w_i >= min_p; Z = the kept weight.  u[b][s] in [0, 1) draws the first kept i, by index, whose running sum
+ *   exceeds u Z:  index[b][s] = i,  logp[b][s] = z_i - log Z (logp may be NULL).  Temperature 0: the best entry (the first of equals).
+ * lengths[rows] (device, may be NULL): entries of each row; what lies behind is not read.  A row without a weight: index -1, logp -inf.
+ * temperature_row / top_k_row / top_p_row / min_p_row: NULL, or [rows] device values used instead of the scalars -- there a
+ * temperature <= 0 or NaN means 0, a top_k <= 0 all, a top_p >= 1 or NaN all and <= 0 the best entry, a min_p <= 0 or NaN none.
+ * u outside [0, 1) draws the first or the last kept entry.  1 <= cols < 2^24.  Sums are fp64 in a fixed order; nothing is kept between calls; the call may
+ * be captured.
+ */
+int pgm_draw_indices(const void* logits, int type, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride,
+                     const int64_t* lengths, const double* u, int64_t draws,
+                     double temperature, const double* temperature_row, int64_t top_k, const int64_t* top_k_row,
+                     double top_p, const double* top_p_row, double min_p, const double* min_p_row,
+                     int64_t* index, double* logp, void* stream);
+
 /* fp64 MFMA issue-rate probe (TFLOP/s of back-to-back v_mfma_f64_16x16x4_f64 on
  * every CU); used once by bench.py to report the measured peak beside the
  * datasheet figure.  Synchronises. */

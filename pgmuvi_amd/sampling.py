@@ -1,0 +1,96 @@
+"""Draws from log-weights on the MI355X (``pgm_draw_indices``): temperature, top-k, top-p and min-p truncation, from random
+numbers the caller gives.
+
+The reference seeds a fit from the highest peaks of a periodogram (``pgmuvi/lightcurve.py:5516-5541``), so every start is the
+same one.  A periodogram is also a posterior over the frequency (:func:`pgmuvi_amd.lombscargle.draw_frequencies`), and starts
+drawn from it differ in proportion to what the data say: top-p keeps the highest-density set, min-p a likelihood ratio,
+top-k the best grid points, and a temperature above one spreads the starts of several chains
+(:func:`pgmuvi_amd.mcmc.run_mcmc`, ``initial_values="periodogram"``).
+
+There is no CPU path: tensors on the GPU or an error.  Nothing synchronises the host.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _hip
+
+_TYPE = {torch.float64: 0, torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}
+
+
+def _setting(value, off, lo, hi, name, rows, dev, dtype):
+    """(scalar, device pointer or None, tensor kept alive) of a truncation argument: a number for all rows, or one per row."""
+    if torch.is_tensor(value) and value.dim() > 0:
+        if tuple(value.shape) != (rows,):
+            raise ValueError(f"draw_indices: {name} must be a number or one per row ({rows}), got {tuple(value.shape)}")
+        _hip.require_gpu(value, "draw_indices")
+        if dtype is torch.int64 and value.dtype.is_floating_point:
+            raise TypeError(f"draw_indices: {name} takes whole numbers")
+        t = value.detach().to(device=dev, dtype=dtype).contiguous()
+        return off, t.data_ptr(), t
+    if value is None:
+        return off, None, None
+    number = int(value) if dtype is torch.int64 else float(value)
+    if not lo <= number <= hi or (dtype is torch.int64 and number != value):
+        raise ValueError(f"draw_indices: {name} must be in [{lo}, {hi}], got {value}")
+    return number, None, None
+
+
+def draw_indices(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=None, top_p=None, min_p=None, lengths=None,
+                 return_logprob: bool = False):
+    """Indices drawn from rows of unnormalised log-probabilities.
+
+    ``logits`` (B, V) or (V,), float64 / float32 / bfloat16 / float16, any strides; ``u`` uniform numbers in [0, 1), (B, S) or
+    (B,) -- (S,) or () for one row -- each of which draws one index.  With ``w = exp((l - max l) / temperature)`` and the order
+    (value descending, index ascending): ``top_k`` keeps the first k entries, ``top_p`` the shortest beginning of those that
+    holds at least that share of their weight, ``min_p`` the entries of that with a weight of at least ``min_p`` times the
+    best one's.  The index is the first kept one, in index order, whose running weight exceeds ``u`` times the kept weight.
+    ``temperature`` 0 takes the best entry.  Each of the four is a number (``None``: off) or a (B,) tensor.  ``lengths`` (B,):
+    entries of each row; the rest is not read.  Entries of -inf or NaN are never drawn.
+
+    Returns int64 indices of the shape of ``u`` (-1 where a row has nothing to draw), with ``return_logprob`` also the
+    float64 log-probabilities of the draws under the truncated distribution (-inf there)."""
+    if not torch.is_tensor(logits) or logits.dtype not in _TYPE or logits.layout is not torch.strided:
+        raise TypeError("draw_indices: logits must be a dense float64, float32, bfloat16 or float16 tensor")
+    if not torch.is_tensor(u) or u.dtype not in _TYPE:
+        raise TypeError("draw_indices: u must be a floating-point tensor of random numbers")
+    _hip.require_gpu(logits, "draw_indices")
+    dev = logits.device
+    if u.device != dev:
+        raise ValueError(f"draw_indices: u is on {u.device}, the logits on {dev}")
+    single = logits.dim() == 1
+    if logits.dim() not in (1, 2):
+        raise ValueError(f"draw_indices: logits must be (B, V) or (V,), got {tuple(logits.shape)}")
+    l = logits.detach().unsqueeze(0) if single else logits.detach()
+    B, V = l.shape
+    if u.dim() > 2 - single or (not single and (u.dim() == 0 or u.shape[0] != B)):
+        raise ValueError(f"draw_indices: u must be {'(S,) or ()' if single else f'({B}, S) or ({B},)'}, got {tuple(u.shape)}")
+    ud = u.detach().to(torch.float64).contiguous()
+    S = ud.numel() // B if B else 0
+    settings = [_setting(temperature, 1.0, 0.0, 1e300, "temperature", B, dev, torch.float64),
+                _setting(top_k, 0, 1, (1 << 62), "top_k", B, dev, torch.int64),
+                _setting(top_p, 1.0, 0.0, 1.0, "top_p", B, dev, torch.float64),
+                _setting(min_p, 0.0, 0.0, 1.0, "min_p", B, dev, torch.float64)]
+    ln = None
+    if lengths is not None:
+        if not torch.is_tensor(lengths):
+            lengths = torch.as_tensor(lengths)
+        if tuple(lengths.shape) != (B,) or lengths.dtype.is_floating_point:
+            raise ValueError(f"draw_indices: lengths must be {B} whole numbers")
+        ln = lengths.to(device=dev, dtype=torch.int64).contiguous()
+    index = torch.empty(u.shape, dtype=torch.int64, device=dev)
+    logp = torch.empty(u.shape, dtype=torch.float64, device=dev) if return_logprob else None
+    if V == 0:                                                   # rows without entries
+        index.fill_(-1)
+        if return_logprob:
+            logp.fill_(float("-inf"))
+    elif B and S:
+        if V >= 1 << 24:
+            raise ValueError(f"draw_indices: rows of at most {(1 << 24) - 1} entries, got {V}")
+        (t, tp, _t), (k, kp, _k), (p, pp, _p), (m, mp, _m) = settings
+        with torch.cuda.device(dev):
+            rc = _hip.load().pgm_draw_indices(l.data_ptr(), _TYPE[l.dtype], B, V, l.stride(0), l.stride(1), None if ln is None else ln.data_ptr(),
+                                              ud.data_ptr(), S, t, tp, k, kp, p, pp, m, mp, index.data_ptr(),
+                                              None if logp is None else logp.data_ptr(), _hip.current_stream_ptr(dev))
+        _hip._check(rc, "pgm_draw_indices")
+    return (index, logp) if return_logprob else index

@@ -1,0 +1,228 @@
+"""GPU tests of the draws against numpy in float64.
+
+The indices are compared exactly: the inputs are fixed, and a draw or a cut would have to lie within the ~1e-13 relative
+difference of two orders of summation to come out differently.  The log-probabilities are z - log Z: z carries two roundings
+(difference, quotient) and Z the sum of up to V weights, each with an error of at most 2 steps of the exponential and one of its
+argument's: |error| <= 2 |z| 2^-53 + (4 + V / 64) 2^-53 + 2 |log Z| 2^-53.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+import os, sys
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import _draw_oracle as oracle
+from pgmuvi_amd.sampling import draw_indices
+
+TYPES = [torch.float64, torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("-m gpu tests need the MI355X")
+    return torch.device("cuda:0")
+
+
+def _rows(B, V, dtype, seed, peaks=2):
+    """Log odds like a periodogram's: exponential noise and a few peaks."""
+    rng = np.random.default_rng(seed)
+    l = rng.exponential(size=(B, V))
+    for b in range(B):
+        for _ in range(peaks):
+            l[b, rng.integers(0, V)] += rng.uniform(0, 12)
+    return torch.as_tensor(l).to(dtype)
+
+
+def _check(logits, u, got, lengths=None, **settings):
+    idx, logp = got
+    l = logits.double().cpu().numpy()
+    idx, logp, u = idx.cpu().numpy(), logp.cpu().numpy(), u.double().cpu().numpy()
+    assert idx.dtype == np.int64 and logp.dtype == np.float64 and idx.shape == u.shape
+    if u.ndim == 1:
+        idx, logp, u = idx[:, None], logp[:, None], u[:, None]
+    for b in range(l.shape[0]):
+        row = {k: (v[b] if isinstance(v, (list, np.ndarray)) else v) for k, v in settings.items()}
+        n = l.shape[1] if lengths is None else max(0, min(l.shape[1], lengths[b]))
+        want, wlp = oracle.draw_row(l[b, :n], u[b], **row)
+        if idx[b].tolist() != want.tolist() and 0.0 < row.get("top_p", 1.0) < 1.0:
+            # A cut exactly on the border.  Weights k/5 (test_ties_go_to_the_lower_index) can put a running sum at top_p Z in real
+            # arithmetic; whether the computed sum reaches the computed product is then a matter of roundings.  Each weight is off by
+            # at most 4 half steps (exponential and argument), a sum of V of them by V half steps more, the product by one: cuts of
+            # top_p (1 +- e) with e = (V + 5) 2^-53 enclose every correctly rounded one.
+            e = (n + 5) * 2.0 ** -53
+            near = [oracle.draw_row(l[b, :n], u[b], **dict(row, top_p=row["top_p"] * f)) for f in (1 - e, 1 + e)]
+            want, wlp = next((r for r in near if idx[b].tolist() == r[0].tolist()), (want, wlp))
+        assert idx[b].tolist() == want.tolist(), (b, row)
+        live = want >= 0
+        z = l[b, idx[b][live]] - np.nanmax(l[b, :n]) if live.any() else np.zeros(0)
+        t = row.get("temperature", 1.0)
+        t = t if t > 0 else 1.0                                  # (0, negative, NaN: the best entry, z = 0)
+        with np.errstate(invalid="ignore"):
+            tol = 2.0 ** -53 * (4 * np.abs(np.nan_to_num(z) / t) + 4 + l.shape[1] / 64 + 2 * np.abs(wlp[live]) + 8)
+        assert (np.abs(logp[b][live] - wlp[live]) <= tol).all()
+        assert (logp[b][~live] == -math.inf).all()
+
+
+SETTINGS = [dict(), dict(temperature=0.3), dict(temperature=4.0), dict(top_k=1), dict(top_k=7), dict(top_k=10 ** 9), dict(top_p=0.9), dict(top_p=0.05), dict(top_p=0.0),
+            dict(top_p=1.0), dict(min_p=0.1), dict(min_p=1.0), dict(top_k=40, top_p=0.8, min_p=0.02, temperature=1.7), dict(temperature=0.0), dict(top_p=0.999, min_p=1e-9)]
+
+
+@pytest.mark.parametrize("settings", SETTINGS, ids=lambda s: "-".join(f"{k}{v}" for k, v in s.items()) or "plain")
+@pytest.mark.parametrize("dtype", TYPES)
+def test_draws(dev, dtype, settings):
+    for B, V, S in ((1, 1, 3), (3, 2, 5), (2, 63, 9), (2, 65, 1), (5, 1113, 8), (2, 9001, 33)):
+        l = _rows(B, V, dtype, 100 * V + B)
+        u = torch.as_tensor(np.random.default_rng(V).random((B, S)))
+        _check(l, u, draw_indices(l.to(dev), u.to(dev), return_logprob=True, **settings), **settings)
+
+
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=300), dict(top_p=0.6), dict(top_k=5000, top_p=0.97), dict(min_p=0.3)], ids=str)
+@pytest.mark.parametrize("dtype, V", [(torch.float64, 51200), (torch.float64, 204800), (torch.float32, 70001), (torch.bfloat16, 140001), (torch.float64, 1_300_001)])
+def test_long_rows(dev, dtype, V, settings):
+    l = _rows(1, V, dtype, V)
+    u = torch.as_tensor(np.random.default_rng(V).random((1, 40)))
+    _check(l, u, draw_indices(l.to(dev), u.to(dev), return_logprob=True, **settings), **settings)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [40, 3000, 30_000])
+def test_ties_go_to_the_lower_index(dev, dtype, V):
+    rng = np.random.default_rng(V)
+    for levels in (1, 2, 5):
+        l = torch.as_tensor(np.log(rng.integers(1, levels + 1, size=(3, V)).astype(float)) if levels > 1 else np.full((3, V), -7.5)).to(dtype)
+        u = torch.as_tensor(rng.random((3, 20)))
+        for settings in (dict(top_k=V // 3), dict(top_k=V - 1), dict(top_p=0.5), dict(top_p=0.37, temperature=0.8), dict(top_k=V // 2 + 1, top_p=0.25), dict(temperature=0.0)):
+            _check(l, u, draw_indices(l.to(dev), u.to(dev), return_logprob=True, **settings), **settings)
+    uniform = torch.zeros(1, V, dtype=dtype, device=dev)
+    u = (torch.arange(V, dtype=torch.float64, device=dev)[None] + 0.5) / V
+    assert torch.equal(draw_indices(uniform, u)[0], torch.arange(V, device=dev))
+    half = draw_indices(uniform, u, top_p=0.5)[0]
+    assert int(half.max()) == (V + 1) // 2 - 1 and int(half.min()) == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_masked_and_nonfinite_entries(dev, dtype):
+    low = torch.finfo(dtype).min
+    V = 700
+    base = _rows(7, V, dtype, 5)
+    base[0, :] = -math.inf                                       # nothing to draw
+    base[1, :] = math.nan
+    base[2, ::2] = -math.inf
+    base[2, 1::4] = math.nan
+    base[3, 5:] = low                                            # masked with the type's lowest value
+    base[4, :] = low                                             # ... all of them: equal weights
+    base[5, 3], base[5, 90] = math.inf, math.inf                 # two certain ones
+    base[6, 1:] = -math.inf                                      # a single entry
+    u = torch.as_tensor(np.random.default_rng(1).random((7, 12)))
+    for settings in (dict(), dict(top_k=4), dict(top_p=0.7), dict(min_p=0.2), dict(temperature=0.0), dict(top_k=699, top_p=0.99), dict(temperature=1e6)):
+        got = draw_indices(base.to(dev), u.to(dev), return_logprob=True, **settings)
+        assert (got[0][:2] == -1).all() and (got[1][:2] == -math.inf).all()
+        sub = [2, 3, 4, 6]
+        _check(base[sub], u[sub], (got[0][sub], got[1][sub]), **settings)
+        assert set(got[0][5].tolist()) <= {3, 90}
+        keep = 1 if settings.get("temperature") == 0.0 else 2
+        assert float((got[1][5] + math.log(keep)).abs().max()) < 1e-15
+    signed = torch.tensor([[-0.0, 0.0, -0.0, 0.0]], dtype=dtype, device=dev)       # equal values
+    assert draw_indices(signed, torch.tensor([[0.1, 0.9]], device=dev), top_k=2).tolist() == [[0, 1]]
+
+
+def test_random_numbers_at_their_limits(dev):
+    l = torch.tensor([[-2000.0, 0.0, 1.0, -2000.0, 0.5, -2000.0]], dtype=torch.float64, device=dev)
+    u = torch.tensor([[0.0, 1.0 - 2.0 ** -53, 1.0, 5.0, -1.0, math.nan, -0.0]], dtype=torch.float64, device=dev)
+    assert draw_indices(l, u).tolist() == [[1, 4, 4, 4, 1, 4, 1]]                # (entries without weight are never drawn)
+    u32 = torch.tensor([[0.0, 0.25, 1.0 - 2.0 ** -24]], device=dev)
+    assert draw_indices(l, u32).tolist() == [[1, 2, 4]]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_lengths_settings_per_row_and_strides(dev, dtype):
+    B, V, S = 9, 1500, 6
+    l = _rows(B, V, dtype, 77)
+    u = torch.as_tensor(np.random.default_rng(2).random((B, S)))
+    lengths = [0, 1, 2, 64, 700, 1499, 1500, 5000, -3]
+    poisoned = l.clone()
+    for b, n in enumerate(lengths):
+        poisoned[b, max(0, n):] = math.inf                       # (never read)
+    per = dict(temperature=np.array([1.0, 0.5, 0.0, -1.0, 2.0, 1.0, 3.0, math.nan, 1.0]), top_k=np.array([0, 3, 5, 0, -2, 40, 1000, 3, 1]),
+               top_p=np.array([1.0, 0.5, 0.9, 0.0, 0.8, 2.0, math.nan, 0.3, 0.5]), min_p=np.array([0.0, 0.1, 0.0, 0.0, -1.0, 0.05, 0.0, 7.0, math.nan]))
+    on = {k: torch.as_tensor(v).to(dev) for k, v in per.items()}
+    got = draw_indices(poisoned.to(dev), u.to(dev), lengths=torch.as_tensor(lengths), return_logprob=True, **on)
+    _check(l, u, got, lengths=lengths, **per)
+    assert got[0][0].tolist() == [-1] * S and got[0][8].tolist() == [-1] * S
+    wide = torch.zeros(B, 2 * V + 7, dtype=dtype, device=dev)
+    views = [wide[:, 3:V + 3], wide[:, 1:2 * V:2], torch.zeros(V, B, dtype=dtype, device=dev).t()]
+    plain = draw_indices(l.to(dev), u.to(dev), top_k=50, top_p=0.9)
+    for v in views:
+        v.copy_(l)
+        assert torch.equal(draw_indices(v, u.to(dev), top_k=50, top_p=0.9), plain)
+    one = draw_indices(l[4].to(dev), u[4].to(dev), top_k=50, top_p=0.9)
+    assert torch.equal(one, plain[4]) and one.shape == (S,)
+    assert torch.equal(draw_indices(l.to(dev), u[:, 2].to(dev), top_k=50, top_p=0.9), plain[:, 2])
+    assert draw_indices(l[4].to(dev), u[4, 1].to(dev), top_k=50, top_p=0.9).item() == int(plain[4, 1])
+    assert torch.equal(draw_indices(l[4].to(dev).expand(3, V), u[4:5].to(dev).expand(3, S), top_k=50, top_p=0.9), plain[4:5].expand(3, S))
+
+
+def test_empty_shapes_and_refusals(dev):
+    l = torch.zeros(4, 10, device=dev)
+    assert draw_indices(l, torch.zeros(4, 0, device=dev)).shape == (4, 0)
+    assert draw_indices(l[:0], torch.zeros(0, 3, device=dev)).shape == (0, 3)
+    i, p = draw_indices(l[:, :0], torch.zeros(4, 2, device=dev), return_logprob=True)
+    assert (i == -1).all() and (p == -math.inf).all()
+    for args, kw in (((l, torch.zeros(3, 2, device=dev)), {}), ((l, torch.zeros((), device=dev)), {}), ((l[0], torch.zeros(2, 2, device=dev)), {}),
+                     ((l[None], torch.zeros(4, 2, device=dev)), {}), ((l, torch.zeros(4, 2)), {}), ((l, torch.zeros(4, 2, device=dev)), dict(top_p=1.5)),
+                     ((l, torch.zeros(4, 2, device=dev)), dict(lengths=torch.zeros(3, dtype=torch.int64))), ((l, torch.zeros(4, 2, device=dev)), dict(top_k=0)),
+                     ((l, torch.zeros(4, 2, device=dev)), dict(temperature=torch.ones(3, device=dev)))):
+        with pytest.raises((ValueError, RuntimeError)):
+            draw_indices(*args, **kw)
+
+
+def test_a_row_does_not_depend_on_its_company_or_on_the_call(dev):
+    l, u = _rows(300, 2000, torch.float64, 3).to(dev), torch.rand(300, 4, dtype=torch.float64, device=dev)
+    all_rows = draw_indices(l, u, top_p=0.8, return_logprob=True)
+    for _ in range(2):
+        again = draw_indices(l, u, top_p=0.8, return_logprob=True)
+        assert torch.equal(again[0], all_rows[0]) and torch.equal(again[1], all_rows[1])
+    some = draw_indices(l[17:19], u[17:19], top_p=0.8, return_logprob=True)
+    assert torch.equal(some[0], all_rows[0][17:19]) and torch.equal(some[1], all_rows[1][17:19])
+
+
+def test_streams_and_a_replayed_graph(dev):
+    l, u = _rows(20, 3001, torch.float32, 8).to(dev), torch.rand(20, 5, dtype=torch.float64, device=dev)
+    want = draw_indices(l, u, top_k=30, top_p=0.9, return_logprob=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = draw_indices(l, u, top_k=30, top_p=0.9, return_logprob=True)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = draw_indices(l, u, top_k=30, top_p=0.9, return_logprob=True)
+    for k in range(3):
+        u.copy_(torch.rand(20, 5, dtype=torch.float64, device=dev))
+        l.copy_(_rows(20, 3001, torch.float32, 50 + k))
+        graph.replay()
+        eager = draw_indices(l, u, top_k=30, top_p=0.9, return_logprob=True)
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1])
+
+
+def test_frequencies_of_draws_follow_the_weights(dev):
+    w = np.array([0.05, 0.3, 0.15, 0.4, 0.1])
+    u = (torch.arange(1000, dtype=torch.float64, device=dev)[None] + 0.5) / 1000
+    idx = draw_indices(torch.as_tensor(np.log(w))[None].to(dev), u)[0]
+    assert torch.bincount(idx, minlength=5).tolist() == [50, 300, 150, 400, 100]
+
+
+def test_more_than_32_bits_of_offset(dev):
+    V = 4_000_000
+    rows = torch.zeros(1100, V, dtype=torch.bfloat16, device=dev)
+    rows[1099, V - 2] = 30.0
+    u = torch.full((1100, 1), 0.75, dtype=torch.float64, device=dev)
+    idx = draw_indices(rows, u, min_p=0.5)
+    assert int(idx[1099]) == V - 2 and int(idx[0]) == 3 * V // 4
