@@ -376,14 +376,16 @@ int pgm_grad_clip(int batch, int count, const uint64_t* in_host, const uint64_t*
  * lengths[rows] (device, may be NULL): entries of each row; what lies behind is not read.  A row without a weight: index -1, logp -inf.
  * temperature_row / top_k_row / top_p_row / min_p_row: NULL, or [rows] device values used instead of the scalars -- there a
  * temperature <= 0 or NaN means 0, a top_k <= 0 all, a top_p >= 1 or NaN all and <= 0 the best entry, a min_p <= 0 or NaN none.
- * u outside [0, 1) draws the first or the last kept entry.  1 <= cols < 2^24.  Sums are fp64 in a fixed order; nothing is kept between calls; the call may
- * be captured.
+ * u outside [0, 1) draws the first or the last kept entry.  1 <= cols < 2^24.  scratch: pgm_draw_scratch_doubles doubles of device
+ * memory owned by the caller, used by this call only (NULL where that is 0).  Sums are fp64 in a fixed order; nothing is kept
+ * between calls; the call may be captured.
  */
+int64_t pgm_draw_scratch_doubles(int type, int64_t rows, int64_t cols, int64_t draws);
 int pgm_draw_indices(const void* logits, int type, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride,
                      const int64_t* lengths, const double* u, int64_t draws,
                      double temperature, const double* temperature_row, int64_t top_k, const int64_t* top_k_row,
                      double top_p, const double* top_p_row, double min_p, const double* min_p_row,
-                     int64_t* index, double* logp, void* stream);
+                     int64_t* index, double* logp, double* scratch, int64_t scratch_doubles, void* stream);
 
 /* fp64 MFMA issue-rate probe (TFLOP/s of back-to-back v_mfma_f64_16x16x4_f64 on
  * every CU); used once by bench.py to report the measured peak beside the

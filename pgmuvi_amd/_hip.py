@@ -74,7 +74,8 @@ SYMBOLS = {
     "pgm_grad_clip": (c_int, [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_double, c_void_p, c_int,
                               c_void_p, c_int64, c_void_p]),
     "pgm_draw_indices": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_double, c_void_p,
-                                 c_int64, c_void_p, c_double, c_void_p, c_double, c_void_p, c_void_p, c_void_p, c_void_p]),
+                                 c_int64, c_void_p, c_double, c_void_p, c_double, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "pgm_draw_scratch_doubles": (c_int64, [c_int, c_int64, c_int64, c_int64]),
 }
 
 

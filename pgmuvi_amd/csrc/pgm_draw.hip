@@ -15,12 +15,14 @@
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 #include <stdint.h>
+#include <algorithm>
 #include "../../include/pgmuvi_hip.h"
 
 namespace {
 
 typedef unsigned long long u64;
-constexpr int NT = 1024, NW = NT / 64, BINS = 2048, MAX_CELLS = 4096;
+constexpr int LOAD = 16, BATCH = 4;                             // bytes of a lane's load; loads of a wavefront in flight
+constexpr int MAX_CELLS = 2048;                                 // of a row (wider cells beyond: `units` loads per lane each)
 constexpr int64_t MAX_COLS = 1 << 24;                             // (2^24 weights of at most one, in steps of 2^-40, fit 64 bits)
 constexpr int64_t EVERY = INT64_MAX;
 
@@ -61,20 +63,29 @@ template <int F16BIT> struct Half {                              // bf16 (0) and
 
 struct Param { double v; const double* p; };                    // one number for every row, or one per row
 struct ParamI { int64_t v; const int64_t* p; };
+constexpr int STATE = 2;                                        // per row in memory: the cut's key and index
 struct DrawArgs {
   const void* logits; int64_t row_stride, col_stride, cols;
   const int64_t* lengths;                                       // entries of each row, or null: cols
   const double* u; int64_t draws;
   Param temperature, top_p, min_p; ParamI top_k;
   int64_t* index; double* logp;
+  int units, max_cells;                                         // loads per lane and cell, cells of a full row
+  u64* keys; double* sums; u64* lows; u64* state;               // rows whose passes are launches of their own: [row][max_cells], [row][groups], [row][STATE]
 };
 
 template <class K> struct Cut { K key; int64_t idx; };          // kept: key above, or equal and index not above
 template <class K> __device__ __forceinline__ bool before(const Cut<K>& c, K key, int64_t i) { return key > c.key || (key == c.key && i <= c.idx); }
 
+// ---- wavefront reductions -------------------------------------------------------------------------------------------------
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
+  return v;
+}
+template <class V> __device__ __forceinline__ V wave_max(V v) {
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) { const V o = __shfl_xor(v, s); v = o > v ? o : v; }
   return v;
 }
 template <class V> __device__ __forceinline__ V wave_scan(V v) {
@@ -83,101 +94,248 @@ template <class V> __device__ __forceinline__ V wave_scan(V v) {
   for (int s = 1; s < 64; s <<= 1) { const V o = __shfl_up(v, s); if (lane >= s) v += o; }
   return v;
 }
-
-struct Bins { uint32_t count[BINS]; u64 hi[BINS], lo[BINS]; };
-struct Shared {
-  union { Bins bins; double cells[MAX_CELLS]; };
-  u64 red[NW][3];
-  u64 found[6];
-  double sums[NW];
-};
-
 __device__ __forceinline__ double mass_of(u64 hi, u64 lo) { return (double)hi * 0x1p-40 + (double)lo * 0x1p-80; }
 
+// ---- one row ----------------------------------------------------------------------------------------------------------------
 template <class F> struct Row {
-  typedef typename F::key K;
-  const typename F::raw* x; int64_t stride, n;
+  typedef typename F::raw raw; typedef typename F::key K;
+  static constexpr int VEC = LOAD / (int)sizeof(raw), UNIT = 64 * VEC;       // entries of one load of a lane, of a wavefront
+  const raw* x; int64_t stride, n;
+  int units, cells;
   double best, t;
+  __device__ __forceinline__ int64_t width() const { return (int64_t)units * UNIT; }
   __device__ __forceinline__ K key(int64_t i) const { return F::to_key(x[i * stride]); }
   __device__ __forceinline__ double z(K k) const { const double l = F::of_key(k); return l == best ? 0.0 : (l - best) / t; }
-  __device__ __forceinline__ double weight(K k) const { return exp(z(k)); }
+  // this lane's entries of unit j: VEC neighbours from at(j) on; key 0 (no value has it) behind the end
+  __device__ __forceinline__ int64_t at(int64_t j) const { return j * UNIT + (threadIdx.x & 63) * VEC; }
+  __device__ __forceinline__ void load(int64_t j, K (&k)[VEC]) const {
+    const int64_t i = at(j);
+    if (stride == 1 && (j + 1) * UNIT <= n) {
+      raw r[VEC];
+      __builtin_memcpy(r, x + i, LOAD);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) k[e] = F::to_key(r[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) k[e] = i + e < n ? F::to_key(x[(i + e) * stride]) : (K)0;
+    }
+  }
+};
+template <class F> __device__ __forceinline__ typename F::key neg_key() {                     // the key of -inf (and NaN)
+  if constexpr (sizeof(typename F::raw) == 2) return F::to_key((typename F::raw)0xffffu);
+  else return F::to_key((typename F::raw)(-__builtin_inf()));
+}
+// a key above that of -inf and not above any whose value is at least v
+template <class F> __device__ __forceinline__ typename F::key key_below(double v) {
+  typedef typename F::key K;
+  const K neg = neg_key<F>();
+  K k;
+  if constexpr (sizeof(typename F::raw) == 8) k = F::to_key(v);
+  else if constexpr (sizeof(typename F::raw) == 4) k = F::to_key((float)v);
+  else {                                                        // (halves: by bisection of their ordered patterns, up to +inf)
+    K a = neg, b = 0xffffu - neg;
+    while (a + 1 < b) { const K m = (a + b) >> 1; if (F::of_key(m) >= v) b = m; else a = m; }
+    k = b;
+  }
+  return k <= neg + 1 ? neg + 1 : k - 1;
+}
+
+// Two builds of a row's code: 16 wavefronts for long rows, 4 for short ones and for the launches that share a row among workgroups
+struct Long { static constexpr int NT = 1024, BITS = 11, CELLS = MAX_CELLS, LIST = 1024; };
+struct Short { static constexpr int NT = 256, BITS = 9, CELLS = 64, LIST = 256; };
+
+template <class C> struct Shared {
+  static constexpr int BINS = 1 << C::BITS, NW = C::NT / 64;
+  union {
+    struct { uint32_t count[BINS]; u64 hi[BINS], lo[BINS]; } bins;
+    double cells[C::CELLS];                                     // weights of the cells, then their running sums
+  };
+  u64 best[C::CELLS];                                           // highest key of every cell, 0: nothing above -inf
+  u64 list_key[C::LIST]; uint32_t list_idx[C::LIST];
+  u64 red[NW], part[3][NW], found[7];
+  double sums[NW];
+  int listed;
 };
 
-// The bin that holds the cut, by wavefront 0: `want` entries (counts), or `share` of the weight (bins hold everything that
-// counts on the first pass: total < 0 asks for it).  found = bin, entries before it, entries in it, hi / lo before it.
-template <bool WEIGHTED> __device__ __forceinline__ void find_bin(Shared& S, u64 before_n, u64 before_hi, u64 before_lo, u64 want, double share, double& target) {
+template <class C> __device__ __forceinline__ u64 block_max(u64 (&red)[C::NT / 64], u64 v) {
+  v = wave_max(v);
   __syncthreads();
-  if (threadIdx.x < 64) {
-    constexpr int PER = BINS / 64;
-    const int lane = threadIdx.x, b0 = lane * PER;
-    u64 n = 0, hi = 0, lo = 0;
-    for (int k = 0; k < PER; ++k) { n += S.bins.count[b0 + k]; if (WEIGHTED) { hi += S.bins.hi[b0 + k]; lo += S.bins.lo[b0 + k]; } }
-    const u64 sn = wave_scan(n), shi = WEIGHTED ? wave_scan(hi) : 0, slo = WEIGHTED ? wave_scan(lo) : 0;
-    if (WEIGHTED && target < 0.0) target = share * mass_of(__shfl(shi, 63), __shfl(slo, 63));
-    auto reached = [&](u64 an, u64 ahi, u64 alo) { return WEIGHTED ? mass_of(before_hi + ahi, before_lo + alo) >= target : before_n + an >= want; };
-    const u64 mask = __ballot(reached(sn, shi, slo));
-    const int owner = mask ? __ffsll(mask) - 1 : 63 - __clzll(__ballot(n > 0) | 1ull);       // (always reached, but for a rounding of the target)
-    if (lane == owner) {
-      u64 an = sn - n, ahi = shi - hi, alo = slo - lo;
-      int b = b0;
-      for (int k = 0; k < PER; ++k) {
-        const u64 c = S.bins.count[b0 + k];
-        if (c == 0) continue;
-        b = b0 + k;
-        if (k + 1 == PER || reached(an + c, ahi + (WEIGHTED ? S.bins.hi[b] : 0), alo + (WEIGHTED ? S.bins.lo[b] : 0))) break;
-        bool more = false;                                      // (the last bin with entries ends the search whatever the comparison says)
-        for (int j = k + 1; j < PER; ++j) more = more || S.bins.count[b0 + j] != 0;
-        if (!more) break;
-        an += c;
-        if (WEIGHTED) { ahi += S.bins.hi[b]; alo += S.bins.lo[b]; }
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int w = 1; w < C::NT / 64; ++w) v = red[w] > v ? red[w] : v;
+  return v;
+}
+// running sum over the workgroup's threads, in thread order
+template <class C> __device__ __forceinline__ double block_scan(double (&sums)[C::NT / 64], double v) {
+  const double inc = wave_scan(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) sums[threadIdx.x >> 6] = inc;
+  __syncthreads();
+  double base = 0.0;
+  for (int w = 0; w < (int)(threadIdx.x >> 6); ++w) base += sums[w];
+  return base + inc;
+}
+
+// f(cell, this lane's keys of one unit, first index, last unit of the cell?) for the cells c0 <= c < c1 -- with SEEN only those whose
+// highest key is at least `lo`: a wavefront per cell, BATCH cells' loads in flight
+template <bool SEEN, int THREADS, class F, class Fn> __device__ __forceinline__ void for_cells(const Row<F>& R, const u64* best, int c0, int c1, u64 lo, Fn f) {
+  typedef typename F::key K;
+  constexpr int NW = THREADS / 64, VEC = Row<F>::VEC;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int c = c0 + wave; c < c1; c += NW * BATCH) {
+    if (R.units == 1) {
+      K k[BATCH][VEC];
+      bool on[BATCH];
+#pragma unroll
+      for (int s = 0; s < BATCH; ++s) {
+        const int cc = c + s * NW;
+        on[s] = cc < c1 && (!SEEN || best[cc] >= lo);
+        if (on[s]) R.load(cc, k[s]);
       }
-      S.found[0] = (u64)b; S.found[1] = before_n + an; S.found[2] = S.bins.count[b]; S.found[3] = before_hi + ahi; S.found[4] = before_lo + alo;
-      S.found[5] = (u64)__double_as_longlong(target);
+#pragma unroll
+      for (int s = 0; s < BATCH; ++s) if (on[s]) f(c + s * NW, k[s], R.at(c + s * NW), true);
+    } else {
+      for (int s = 0; s < BATCH; ++s) {
+        const int cc = c + s * NW;
+        if (cc >= c1 || (SEEN && best[cc] < lo)) continue;
+        for (int j = 0; j < R.units; ++j) {
+          K k[VEC];
+          const int64_t u = (int64_t)cc * R.units + j;
+          R.load(u, k);
+          f(cc, k, R.at(u), j == R.units - 1);
+        }
+      }
     }
+  }
+}
+
+// ---- the cut -------------------------------------------------------------------------------------------------------------------
+// The bin that holds it: `want` entries, or (WEIGHTED) `target` of weight -- `share` of all that the bins hold on the first pass,
+// where target < 0 asks for it.  found: bin, entries before it, in it, hi / lo before it, target, entries in all bins
+template <bool WEIGHTED, class C> __device__ __forceinline__ void find_bin(Shared<C>& S, u64 before_n, u64 before_hi, u64 before_lo, u64 want, double share, double target) {
+  constexpr int PER = Shared<C>::BINS / C::NT, NW = C::NT / 64;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, b0 = t * PER;
+  __syncthreads();
+  u64 n = 0, hi = 0, lo = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) { n += S.bins.count[b0 + k]; if (WEIGHTED) { hi += S.bins.hi[b0 + k]; lo += S.bins.lo[b0 + k]; } }
+  u64 sn = wave_scan(n), shi = WEIGHTED ? wave_scan(hi) : 0, slo = WEIGHTED ? wave_scan(lo) : 0;
+  if (lane == 63) { S.part[0][wave] = sn; S.part[1][wave] = shi; S.part[2][wave] = slo; }
+  __syncthreads();
+  u64 all = 0, all_hi = 0, all_lo = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w == wave) { sn += all; shi += all_hi; slo += all_lo; }
+    all += S.part[0][w]; all_hi += S.part[1][w]; all_lo += S.part[2][w];
+  }
+  if (WEIGHTED) {
+    if (target < 0.0) target = share * mass_of(all_hi, all_lo);
+    const double most = mass_of(before_hi + all_hi, before_lo + all_lo);
+    target = target < most ? target : most;                     // (a rounding of the product must not put it behind the end)
+  } else if (want > before_n + all) want = before_n + all;
+  auto reached = [&](u64 an, u64 ahi, u64 alo) { return WEIGHTED ? mass_of(before_hi + ahi, before_lo + alo) >= target : before_n + an >= want; };
+  u64 an = sn - n, ahi = shi - hi, alo = slo - lo;
+  if (n && !reached(an, ahi, alo) && reached(sn, shi, slo)) {
+    int b = b0;
+#pragma unroll
+    for (int k = 0; k < PER - 1; ++k) {
+      if (b != b0 + k) continue;
+      const u64 c = S.bins.count[b], h = WEIGHTED ? S.bins.hi[b] : 0, l = WEIGHTED ? S.bins.lo[b] : 0;
+      if (c && reached(an + c, ahi + h, alo + l)) continue;     // (this one)
+      an += c; ahi += h; alo += l; ++b;
+    }
+    S.found[0] = (u64)b; S.found[1] = before_n + an; S.found[2] = S.bins.count[b]; S.found[3] = before_hi + ahi; S.found[4] = before_lo + alo;
+    S.found[5] = (u64)__double_as_longlong(target); S.found[6] = all;
   }
   __syncthreads();
 }
-__device__ __forceinline__ void clear_bins(Shared& S) {
+template <bool WEIGHTED, class C> __device__ __forceinline__ void clear_bins(Shared<C>& S) {
   __syncthreads();
-  for (int b = threadIdx.x; b < BINS; b += NT) { S.bins.count[b] = 0; S.bins.hi[b] = 0; S.bins.lo[b] = 0; }
+  for (int b = threadIdx.x; b < Shared<C>::BINS; b += C::NT) { S.bins.count[b] = 0; if (WEIGHTED) { S.bins.hi[b] = 0; S.bins.lo[b] = 0; } }
+  if (threadIdx.x == 0) S.listed = 0;
   __syncthreads();
 }
+template <class C> __device__ __forceinline__ int shift_of(u64 span) { return span < (u64)Shared<C>::BINS ? 0 : 64 - __clzll(span) - C::BITS; }
 
-// the cut behind the first `want` entries of what `have` keeps (WEIGHTED: behind the shortest beginning with `share` of its weight)
-template <bool WEIGHTED, class F> __device__ Cut<typename F::key> select(const Row<F>& R, Shared& S, typename F::key kmin, typename F::key kmax,
-                                                                         Cut<typename F::key> have, u64 want, double share) {
+__device__ __forceinline__ bool ahead(u64 ka, uint32_t ia, u64 kb, uint32_t ib) { return ka > kb || (ka == kb && ia < ib); }
+
+// The cut behind the first `want` entries of what `have` keeps (WEIGHTED: behind the shortest beginning with `share` of its weight).
+// kmin / kmax: range of keys that can matter; S.best: the cells' highest keys
+template <bool WEIGHTED, class C, class F> __device__ Cut<typename F::key> select(const Row<F>& R, Shared<C>& S, typename F::key kmin, typename F::key kmax,
+                                                                                  Cut<typename F::key> have, u64 want, double share) {
   typedef typename F::key K;
+  constexpr int VEC = Row<F>::VEC;
   K hi = kmax, lo = kmin;
   u64 bn = 0, bhi = 0, blo = 0;
   double target = -1.0;
+  bool first = true;
   for (;;) {
-    const u64 span = (u64)(hi - lo);
-    const int shift = span < BINS ? 0 : 64 - __clzll(span) - 11;
-    clear_bins(S);
-    for (int64_t i = threadIdx.x; i < R.n; i += NT) {
-      const K k = R.key(i);
-      if (k < lo || k > hi || !before(have, k, i)) continue;
-      const int b = (int)((u64)(hi - k) >> shift);
-      atomicAdd(&S.bins.count[b], 1u);
-      if (WEIGHTED) {
-        const double w = R.weight(k) * 0x1p40;
-        const u64 whi = (u64)w, wlo = (u64)((w - (double)whi) * 0x1p40);
-        if (whi) atomicAdd(&S.bins.hi[b], whi);
-        if (wlo) atomicAdd(&S.bins.lo[b], wlo);
+    const int shift = shift_of<C>((u64)(hi - lo));
+    clear_bins<WEIGHTED>(S);
+    for_cells<true, C::NT>(R, S.best, 0, R.cells, lo, [&](int, const K (&k)[VEC], int64_t i, bool) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        if (k[e] < lo || k[e] > hi || !before(have, k[e], i + e)) continue;
+        const int b = (int)((u64)(hi - k[e]) >> shift);
+        atomicAdd(&S.bins.count[b], 1u);
+        if (WEIGHTED) {
+          const double w = exp(R.z(k[e])) * 0x1p40;
+          const u64 whi = (u64)w, wlo = (u64)((w - (double)whi) * 0x1p40);
+          if (whi) atomicAdd(&S.bins.hi[b], whi);
+          if (wlo) atomicAdd(&S.bins.lo[b], wlo);
+        }
       }
-    }
+    });
     find_bin<WEIGHTED>(S, bn, bhi, blo, want, share, target);
+    if (!WEIGHTED && first && S.found[6] <= want) return Cut<K>{lo, EVERY};       // (all of them)
+    first = false;
     const u64 bin = S.found[0], in_bin = S.found[2];
     bn = S.found[1]; bhi = S.found[3]; blo = S.found[4]; target = __longlong_as_double((long long)S.found[5]);
     const K top = (K)(hi - (K)(bin << shift));
     const u64 width = (1ull << shift) - 1;
     const K bottom = (u64)(top - lo) <= width ? lo : (K)(top - (K)width);
     Cut<K> cut{bottom, EVERY};
-    if (in_bin == 1 || (!WEIGHTED && bn + in_bin == want)) return cut;
-    if (shift == 0) {                                           // equal values: the first m of them by index
+    if (in_bin <= 1 || (!WEIGHTED && bn + in_bin == want)) return cut;
+    if (in_bin <= (u64)C::LIST) {
+      // few enough to sort: the bin's entries by (key, index), then the first that reaches the target
+      for_cells<true, C::NT>(R, S.best, 0, R.cells, bottom, [&](int, const K (&k)[VEC], int64_t i, bool) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          if (k[e] < bottom || k[e] > top || !before(have, k[e], i + e)) continue;
+          const int at = atomicAdd(&S.listed, 1);
+          S.list_key[at] = k[e]; S.list_idx[at] = (uint32_t)(i + e);
+        }
+      });
+      const int count = (int)in_bin, t = threadIdx.x;
+      int size = 2;
+      while (size < count) size <<= 1;
+      if (t >= count && t < size) { S.list_key[t] = 0; S.list_idx[t] = 0xffffffffu; }
+      for (int span = 2; span <= size; span <<= 1)
+        for (int s = span >> 1; s > 0; s >>= 1) {
+          __syncthreads();
+          const int o = t ^ s;
+          if (t < size && o > t) {
+            const u64 ka = S.list_key[t], kb = S.list_key[o];
+            const uint32_t ia = S.list_idx[t], ib = S.list_idx[o];
+            if (ahead(kb, ib, ka, ia) == ((t & span) == 0)) { S.list_key[t] = kb; S.list_key[o] = ka; S.list_idx[t] = ib; S.list_idx[o] = ia; }
+          }
+        }
+      __syncthreads();
+      int at = (int)(want - bn) - 1;
+      if (WEIGHTED) {
+        const double sum = block_scan<C>(S.sums, t < count ? exp(R.z((K)S.list_key[t])) : 0.0);
+        const bool yes = t < count && mass_of(bhi, blo) + sum >= target;
+        at = count - 1 - (int)block_max<C>(S.red, yes ? (u64)(count - 1 - t) : 0);
+      }
+      cut.key = (K)S.list_key[at]; cut.idx = (int64_t)S.list_idx[at];
+      return cut;
+    }
+    if (shift == 0) {                                           // many equal values: the first m of them by index
       u64 m = WEIGHTED ? 1 : want - bn;
       if (WEIGHTED) {
-        const double w = R.weight(top), above = mass_of(bhi, blo);
+        const double w = exp(R.z(top)), above = mass_of(bhi, blo);
         const double guess = ceil((target - above) / w);
         m = guess >= (double)in_bin ? in_bin : guess < 1.0 ? 1 : (u64)guess;
         while (m > 1 && above + (double)(m - 1) * w >= target) --m;
@@ -187,24 +345,23 @@ template <bool WEIGHTED, class F> __device__ Cut<typename F::key> select(const R
       int64_t i0 = 0, i1 = R.n - 1;
       u64 passed = 0;
       for (;;) {
-        const u64 ispan = (u64)(i1 - i0);
-        const int ishift = ispan < BINS ? 0 : 64 - __clzll(ispan) - 11;
-        clear_bins(S);
-        for (int64_t i = i0 + threadIdx.x; i <= i1; i += NT)
-          if (R.key(i) == top && before(have, top, i)) atomicAdd(&S.bins.count[(u64)(i - i0) >> ishift], 1u);
-        double none = 0.0;
-        find_bin<false>(S, passed, 0, 0, m, 0.0, none);
-        const int64_t first = i0 + (int64_t)(S.found[0] << ishift), last = first + (int64_t)((1ull << ishift) - 1);
+        const int ishift = shift_of<C>((u64)(i1 - i0));
+        clear_bins<false>(S);
+        for_cells<true, C::NT>(R, S.best, (int)(i0 / R.width()), (int)(i1 / R.width()) + 1, top, [&](int, const K (&k)[VEC], int64_t i, bool) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (k[e] == top && i + e >= i0 && i + e <= i1 && before(have, top, i + e)) atomicAdd(&S.bins.count[(u64)(i + e - i0) >> ishift], 1u);
+        });
+        find_bin<false>(S, passed, 0, 0, m, 0.0, 0.0);
+        const int64_t from = i0 + (int64_t)(S.found[0] << ishift), to = from + (int64_t)((1ull << ishift) - 1);
         passed = S.found[1];
         const u64 here = S.found[2];
-        i0 = first;
-        i1 = last < i1 ? last : i1;
+        i0 = from;
+        i1 = to < i1 ? to : i1;
         if (ishift == 0 || passed + here == m) { cut.key = top; cut.idx = i1; return cut; }
-        __syncthreads();
       }
     }
     hi = top; lo = bottom;
-    __syncthreads();                                            // (found has been read by everybody)
   }
 }
 template <class K> __device__ __forceinline__ Cut<K> tighter(const Cut<K>& a, const Cut<K>& b) {
@@ -212,126 +369,328 @@ template <class K> __device__ __forceinline__ Cut<K> tighter(const Cut<K>& a, co
   return a.idx < b.idx ? a : b;
 }
 
-template <class F> __global__ __launch_bounds__(NT) void k_draw(DrawArgs A) {
-  typedef typename F::key K;
-  __shared__ Shared S;
-  const int64_t row = blockIdx.x;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+// ---- a row's settings -------------------------------------------------------------------------------------------------------------
+struct Settings { double t, top_p, min_p; int64_t top_k; bool plain; };
+__device__ __forceinline__ Settings settings_of(const DrawArgs& A, int64_t row) {
+  Settings s;
+  const double temp = A.temperature.p ? A.temperature.p[row] : A.temperature.v;
+  s.top_p = A.top_p.p ? A.top_p.p[row] : A.top_p.v;
+  s.min_p = A.min_p.p ? A.min_p.p[row] : A.min_p.v;
+  s.top_k = A.top_k.p ? A.top_k.p[row] : A.top_k.v;
+  if (s.top_p <= 0.0 || !(temp > 0.0)) s.top_k = 1;            // the best entry alone (the first of equal ones)
+  s.t = temp > 0.0 ? (temp < 1e300 ? temp : 1e300) : 1.0;
+  if (!(s.top_p > 0.0 && s.top_p < 1.0)) s.top_p = 1.0;
+  s.min_p = s.min_p > 0.0 ? (s.min_p < 1.0 ? s.min_p : 1.0) : 0.0;
+  s.top_k = s.top_k > 0 ? s.top_k : 0;
+  s.plain = s.top_k == 0 && s.top_p == 1.0 && s.min_p == 0.0;
+  return s;
+}
+template <class F> __device__ __forceinline__ Row<F> row_of(const DrawArgs& A, int64_t row, double t) {
+  Row<F> R;
   int64_t n = A.cols;
   if (A.lengths) { n = A.lengths[row]; n = n < 0 ? 0 : n > A.cols ? A.cols : n; }
-  Row<F> R;
   R.x = static_cast<const typename F::raw*>(A.logits) + row * A.row_stride; R.stride = A.col_stride; R.n = n;
+  R.units = A.units;
+  R.cells = (int)((n + R.width() - 1) / R.width());
+  R.best = 0.0; R.t = t;
+  return R;
+}
 
-  // the best and the lowest key above -inf, and how many there are
-  K neg;
-  if constexpr (sizeof(typename F::raw) == 2) neg = F::to_key((typename F::raw)0xffffu);      // (a NaN: the key of -inf)
-  else neg = F::to_key((typename F::raw)(-__builtin_inf()));
-  u64 kmax = 0, kmin = ~0ull, valid = 0;
-  for (int64_t i = t; i < n; i += NT) {
-    const K k = R.key(i);
-    if (k <= neg) continue;
-    kmax = kmax > (u64)k ? kmax : (u64)k; kmin = kmin < (u64)k ? kmin : (u64)k; ++valid;
-  }
+// ---- the passes over a row ----------------------------------------------------------------------------------------------------------
+// highest key of the cells [c0, c1) -> keys[c]; where nothing is truncated (sums != null) also their weight relative to it.
+// Returns this lane's lowest key above -inf
+template <int THREADS, class F> __device__ __forceinline__ u64 pass_best(Row<F> R, int c0, int c1, u64* keys, double* sums) {
+  typedef typename F::key K;
+  constexpr int VEC = Row<F>::VEC;
+  const K neg = neg_key<F>();
+  u64 kmin = ~0ull;
+  K run = 0;
+  for_cells<false, THREADS>(R, (const u64*)nullptr, c0, c1, 0, [&](int c, const K (&k)[VEC], int64_t, bool last) {
 #pragma unroll
-  for (int s = 32; s > 0; s >>= 1) {
-    const u64 a = __shfl_xor(kmax, s), b = __shfl_xor(kmin, s);
-    kmax = kmax > a ? kmax : a; kmin = kmin < b ? kmin : b; valid += __shfl_xor(valid, s);
-  }
-  if (lane == 0) { S.red[wave][0] = kmax; S.red[wave][1] = kmin; S.red[wave][2] = valid; }
-  __syncthreads();
-  kmax = 0; kmin = ~0ull; valid = 0;
-  for (int w = 0; w < NW; ++w) {
-    kmax = kmax > S.red[w][0] ? kmax : S.red[w][0]; kmin = kmin < S.red[w][1] ? kmin : S.red[w][1]; valid += S.red[w][2];
-  }
-  int64_t* index = A.index + row * A.draws;
-  double* logp = A.logp ? A.logp + row * A.draws : nullptr;
-  if (valid == 0) {                                             // nothing to draw from
-    for (int64_t s = t; s < A.draws; s += NT) { index[s] = -1; if (logp) logp[s] = -__builtin_inf(); }
-    return;
-  }
-  R.best = F::of_key((K)kmax);
-  const double temp = A.temperature.p ? A.temperature.p[row] : A.temperature.v;
-  R.t = temp < 1e300 ? temp : 1e300;
-  const double top_p = A.top_p.p ? A.top_p.p[row] : A.top_p.v;
-  double min_p = A.min_p.p ? A.min_p.p[row] : A.min_p.v;
-  min_p = min_p > 1.0 ? 1.0 : min_p;
-  int64_t top_k = A.top_k.p ? A.top_k.p[row] : A.top_k.v;
-  if (!(temp > 0.0) || top_p <= 0.0) top_k = 1;                 // the best entry alone (the first of equal ones)
-  if (!(temp > 0.0)) R.t = 1.0;
-
-  Cut<K> cut{neg, -1};
-  if (top_k > 0 && (u64)top_k < valid) cut = tighter(cut, select<false, F>(R, S, (K)kmin, (K)kmax, cut, (u64)top_k, 0.0));
-  if (top_p > 0.0 && top_p < 1.0) cut = tighter(cut, select<true, F>(R, S, (K)kmin, (K)kmax, cut, 0, top_p));
-  __syncthreads();                                              // (the cells take the bins' place)
-
-  auto kept = [&](int64_t i) -> double {                        // the weight of entry i, zero if it is not kept
-    const K k = R.key(i);
-    if (k <= neg || !before(cut, k, i)) return 0.0;
-    const double w = R.weight(k);
-    return w < min_p ? 0.0 : w;
-  };
-  int64_t steps = (n + 64 * (int64_t)MAX_CELLS - 1) / (64 * (int64_t)MAX_CELLS);
-  steps = steps < 4 ? 4 : steps;
-  const int64_t width = 64 * steps;
-  const int cells = (int)((n + width - 1) / width);
-  for (int c = wave; c < cells; c += NW) {
-    const int64_t i0 = c * width + lane;
+    for (int e = 0; e < VEC; ++e) { run = k[e] > run ? k[e] : run; if (k[e] > neg && (u64)k[e] < kmin) kmin = k[e]; }
+    if (!last) return;
+    const K top = wave_max(run);
+    run = 0;
+    if ((threadIdx.x & 63) == 0) keys[c] = top > neg ? (u64)top : 0;
+    if (!sums) return;
     double s = 0.0;
-    for (int64_t j = 0; j < steps; ++j) { const int64_t i = i0 + 64 * j; if (i < n) s += kept(i); }
+    if (top > neg) {
+      R.best = F::of_key(top);
+      for (int j = 0; j < R.units; ++j) {
+        K q[VEC];
+        if (R.units > 1) R.load((int64_t)c * R.units + j, q);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) { const K x = R.units > 1 ? q[e] : k[e]; s += x > neg ? exp(R.z(x)) : 0.0; }
+      }
+    }
     s = wave_sum(s);
-    if (lane == 0) S.cells[c] = s;
+    if ((threadIdx.x & 63) == 0) sums[c] = s;
+  });
+  return kmin;
+}
+// kept weight of the cells [c0, c1) -> sums[c]
+template <int THREADS, class F> __device__ __forceinline__ void pass_weights(const Row<F>& R, const u64* best, int c0, int c1, const Cut<typename F::key>& cut, double min_p, double* sums) {
+  typedef typename F::key K;
+  constexpr int VEC = Row<F>::VEC;
+  const K neg = neg_key<F>();
+  K lo = cut.key > neg ? cut.key : neg + 1;
+  if (min_p > 0.0) {                                            // (no cell below this, with room for the roundings, has an entry of that weight)
+    double v = R.best + R.t * log(min_p);
+    v -= 1e-12 * (fabs(v) + fabs(R.best)) + 1e-9 * R.t;
+    const K m = key_below<F>(v);
+    lo = m > lo ? m : lo;
   }
+  for (int c = c0 + (int)threadIdx.x; c < c1; c += THREADS) if (best[c] < (u64)lo) sums[c] = 0.0;
+  double s = 0.0;
+  for_cells<true, THREADS>(R, best, c0, c1, (u64)lo, [&](int c, const K (&k)[VEC], int64_t i, bool last) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+      if (k[e] >= lo && before(cut, k[e], i + e)) { const double w = exp(R.z(k[e])); s += w < min_p ? 0.0 : w; }
+    if (!last) return;
+    const double total = wave_sum(s);
+    s = 0.0;
+    if ((threadIdx.x & 63) == 0) sums[c] = total;
+  });
+}
+// running sums over S.cells
+template <class C> __device__ __forceinline__ void scan_cells(Shared<C>& S, int cells) {
+  constexpr int PER = (C::CELLS + C::NT - 1) / C::NT;
+  double v[PER], s = 0.0;
   __syncthreads();
-  {                                                             // running sums over the cells: four per thread, wavefronts, workgroup
-    constexpr int PER = MAX_CELLS / NT;
-    double v[PER], s = 0.0;
 #pragma unroll
-    for (int k = 0; k < PER; ++k) { const int c = t * PER + k; s += c < cells ? S.cells[c] : 0.0; v[k] = s; }
-    const double inc = wave_scan(s);
-    if (lane == 63) S.sums[wave] = inc;
-    __syncthreads();
-    double base = inc - s;
-    for (int w = 0; w < wave; ++w) base += S.sums[w];
+  for (int k = 0; k < PER; ++k) { const int c = threadIdx.x * PER + k; s += c < cells ? S.cells[c] : 0.0; v[k] = s; }
+  const double base = block_scan<C>(S.sums, s) - s;
 #pragma unroll
-    for (int k = 0; k < PER; ++k) { const int c = t * PER + k; if (c < cells) S.cells[c] = base + v[k]; }
-    __syncthreads();
-  }
-  const double Z = S.cells[cells - 1], log_z = log(Z);
-  for (int64_t s = wave; s < A.draws; s += NW) {                // one wavefront per draw
+  for (int k = 0; k < PER; ++k) { const int c = threadIdx.x * PER + k; if (c < cells) S.cells[c] = base + v[k]; }
+  __syncthreads();
+}
+// the draws [s0, s1) of a row from its running sums, one wavefront each
+template <class C, class F> __device__ __forceinline__ void draw(const DrawArgs& A, const Row<F>& R, const Shared<C>& S, int64_t row, int64_t s0, int64_t s1,
+                                                                 const Cut<typename F::key>& cut, double min_p) {
+  typedef typename F::key K;
+  const K neg = neg_key<F>();
+  const int lane = threadIdx.x & 63;
+  const double Z = S.cells[R.cells - 1], log_z = log(Z);
+  for (int64_t s = s0 + (threadIdx.x >> 6); s < s1; s += Shared<C>::NW) {
     double target = A.u[row * A.draws + s] * Z;
     target = target > 0.0 ? target : target == target ? 0.0 : Z;   // (u outside [0, 1): the first or the last kept entry)
     auto first_above = [&](double x, bool or_equal) {
-      int a = 0, b = cells;
+      int a = 0, b = R.cells;
       while (a < b) { const int m = (a + b) >> 1; const double f = S.cells[m]; if (f > x || (or_equal && f >= x)) b = m; else a = m + 1; }
       return a;
     };
     int c = first_above(target, false);
-    if (c == cells) { c = first_above(Z, true); target = __builtin_inf(); }
+    if (c == R.cells) { c = first_above(Z, true); target = __builtin_inf(); }
     double base = c ? S.cells[c - 1] : 0.0;
+    const int64_t i0 = c * R.width();
     int64_t found = -1, last = -1;
-    for (int64_t j = 0; j < steps && found < 0; ++j) {
-      const int64_t i = c * width + 64 * j + lane;
-      const double w = i < n ? kept(i) : 0.0, inc = wave_scan(w);
+    const int steps = R.units * Row<F>::VEC;
+    for (int j = 0; j < steps && found < 0; ++j) {
+      const int64_t i = i0 + 64 * (int64_t)j + lane;
+      double w = 0.0;
+      if (i < R.n) {
+        const K k = R.key(i);
+        if (k > neg && before(cut, k, i)) { w = exp(R.z(k)); w = w < min_p ? 0.0 : w; }
+      }
+      const double inc = wave_scan(w);
       const u64 hit = __ballot(w > 0.0 && base + inc > target), some = __ballot(w > 0.0);
-      if (hit) found = c * width + 64 * j + __ffsll(hit) - 1;
-      if (some) last = c * width + 64 * j + 63 - __clzll(some);
+      if (hit) found = i0 + 64 * (int64_t)j + __ffsll(hit) - 1;
+      if (some) last = i0 + 64 * (int64_t)j + 63 - __clzll(some);
       base += __shfl(inc, 63);
     }
     if (found < 0) found = last;                                // (the cell's own sum and this one differ by a rounding)
     if (lane == 0) {
-      index[s] = found;
-      if (logp) logp[s] = R.z(R.key(found)) - log_z;
+      A.index[row * A.draws + s] = found;
+      if (A.logp) A.logp[row * A.draws + s] = R.z(R.key(found)) - log_z;
     }
   }
 }
+__device__ __forceinline__ void draw_nothing(const DrawArgs& A, int64_t row, int64_t s0, int64_t s1, int threads) {
+  for (int64_t s = s0 + threadIdx.x; s < s1; s += threads) {
+    A.index[row * A.draws + s] = -1;
+    if (A.logp) A.logp[row * A.draws + s] = -__builtin_inf();
+  }
+}
+// the cut of a row whose cells' highest keys are in S.best; R.best is set
+template <class C, class F> __device__ Cut<typename F::key> cut_of(const Row<F>& R, Shared<C>& S, const Settings& p, u64 kmin, u64 kmax) {
+  typedef typename F::key K;
+  Cut<K> cut{neg_key<F>(), -1};
+  if (p.top_k > 0) {
+    // the top_k-th highest of the cells' best is a lower bound of the cut: only cells that reach it are looked at again
+    K lo = (K)kmin;
+    if (p.top_k < R.cells) {
+      clear_bins<false>(S);
+      const int shift = shift_of<C>(kmax - kmin);
+      for (int c = threadIdx.x; c < R.cells; c += C::NT) if (S.best[c] >= kmin) atomicAdd(&S.bins.count[(kmax - S.best[c]) >> shift], 1u);
+      find_bin<false>(S, 0, 0, 0, (u64)p.top_k, 0.0, 0.0);
+      if (S.found[6] >= (u64)p.top_k) {
+        const u64 drop = ((S.found[0] + 1) << shift) - 1;       // (to the lowest key of the bin)
+        if (drop < kmax - kmin) lo = (K)(kmax - drop);
+      }
+    }
+    cut = tighter(cut, select<false, C, F>(R, S, lo, (K)kmax, cut, (u64)p.top_k, 0.0));
+  }
+  if (p.top_p < 1.0) {
+    // entries below exp(-56) < 2^-80 of the best one weigh nothing in the bins
+    const K floor = key_below<F>(R.best - 56.0 * R.t);
+    cut = tighter(cut, select<true, C, F>(R, S, (u64)floor > kmin ? floor : (K)kmin, (K)kmax, cut, 0, p.top_p));
+  }
+  return cut;
+}
 
+// ---- kernels --------------------------------------------------------------------------------------------------------------------------
+// One workgroup per row: everything, or (draws_here 0: many draws per row) all but the draws, which k_draws makes from memory
+template <class C, class F> __global__ __launch_bounds__(C::NT) void k_row(DrawArgs A, int draws_here) {
+  typedef typename F::key K;
+  __shared__ Shared<C> S;
+  const int64_t row = blockIdx.x;
+  const Settings p = settings_of(A, row);
+  Row<F> R = row_of<F>(A, row, p.t);
+  const u64 low = pass_best<C::NT, F>(R, 0, R.cells, S.best, p.plain ? S.cells : nullptr);
+  __syncthreads();
+  u64 top = 0;
+  for (int c = threadIdx.x; c < R.cells; c += C::NT) top = S.best[c] > top ? S.best[c] : top;
+  const u64 kmax = block_max<C>(S.red, top);
+  Cut<K> cut{neg_key<F>(), -1};
+  if (kmax != 0) {
+    R.best = F::of_key((K)kmax);
+    if (!p.plain) {
+      const u64 kmin = ~block_max<C>(S.red, ~low);
+      cut = cut_of<C, F>(R, S, p, kmin, kmax);
+      __syncthreads();                                          // (the cells take the bins' place)
+      pass_weights<C::NT, F>(R, S.best, 0, R.cells, cut, p.min_p, S.cells);
+    } else if (draws_here) {
+      for (int c = threadIdx.x; c < R.cells; c += C::NT) S.cells[c] *= S.best[c] ? exp(R.z((K)S.best[c])) : 0.0;
+    }
+  }
+  if (draws_here) {
+    if (kmax == 0) { draw_nothing(A, row, 0, A.draws, C::NT); return; }
+    scan_cells(S, R.cells);
+    draw<C, F>(A, R, S, row, 0, A.draws, cut, p.min_p);
+    return;
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < R.cells; c += C::NT) { A.keys[row * A.max_cells + c] = S.best[c]; A.sums[row * A.max_cells + c] = S.cells[c]; }
+  if (threadIdx.x == 0) { A.state[row * STATE] = (u64)cut.key; A.state[row * STATE + 1] = (u64)cut.idx; }
+}
+
+// The same over several launches, for a few long rows whose cells are dealt to `groups` workgroups each.  First: the cells' highest
+// keys, the lowest key of each group, and -- nothing truncated -- the cells' weights
+template <class F> __global__ __launch_bounds__(256) void k_best(DrawArgs A, int groups) {
+  __shared__ u64 red[4];
+  const int64_t row = blockIdx.x / groups;
+  const int g = blockIdx.x % groups;
+  const Settings p = settings_of(A, row);
+  const Row<F> R = row_of<F>(A, row, p.t);
+  const int c0 = (int)((int64_t)R.cells * g / groups), c1 = (int)((int64_t)R.cells * (g + 1) / groups);
+  const u64 low = pass_best<256, F>(R, c0, c1, A.keys + row * A.max_cells, p.plain ? A.sums + row * A.max_cells : nullptr);
+  const u64 kmin = ~block_max<Short>(red, ~low);
+  if (threadIdx.x == 0) {
+    A.lows[row * groups + g] = kmin;
+    if (g == 0) { A.state[row * STATE] = (u64)neg_key<F>(); A.state[row * STATE + 1] = (u64)-1; }
+  }
+}
+// ... the cut (only where one may be asked for)
+template <class F> __global__ __launch_bounds__(Long::NT) void k_cut(DrawArgs A, int groups) {
+  typedef typename F::key K;
+  __shared__ Shared<Long> S;
+  const int64_t row = blockIdx.x;
+  const Settings p = settings_of(A, row);
+  Row<F> R = row_of<F>(A, row, p.t);
+  u64 top = 0, low = ~0ull;
+  for (int c = threadIdx.x; c < R.cells; c += Long::NT) { const u64 k = A.keys[row * A.max_cells + c]; S.best[c] = k; top = k > top ? k : top; }
+  for (int g = threadIdx.x; g < groups; g += Long::NT) { const u64 k = A.lows[row * groups + g]; low = k < low ? k : low; }
+  const u64 kmax = block_max<Long>(S.red, top), kmin = ~block_max<Long>(S.red, ~low);
+  if (kmax == 0) return;
+  R.best = F::of_key((K)kmax);
+  const Cut<K> cut = cut_of<Long, F>(R, S, p, kmin, kmax);
+  if (threadIdx.x == 0) { A.state[row * STATE] = (u64)cut.key; A.state[row * STATE + 1] = (u64)cut.idx; }
+}
+template <int THREADS> __device__ __forceinline__ u64 best_of_row(const DrawArgs& A, int64_t row, int cells, u64 (&red)[THREADS / 64]) {
+  u64 top = 0;
+  for (int c = threadIdx.x; c < cells; c += THREADS) { const u64 k = A.keys[row * A.max_cells + c]; top = k > top ? k : top; }
+  if constexpr (THREADS == Short::NT) return block_max<Short>(red, top); else return block_max<Long>(red, top);
+}
+// ... the cells' kept weights
+template <class F> __global__ __launch_bounds__(256) void k_weights(DrawArgs A, int groups) {
+  typedef typename F::key K;
+  __shared__ u64 red[4];
+  const int64_t row = blockIdx.x / groups;
+  const int g = blockIdx.x % groups;
+  const Settings p = settings_of(A, row);
+  Row<F> R = row_of<F>(A, row, p.t);
+  const u64 kmax = best_of_row<256>(A, row, R.cells, red);
+  if (p.plain || kmax == 0) return;
+  R.best = F::of_key((K)kmax);
+  const Cut<K> cut{(K)A.state[row * STATE], (int64_t)A.state[row * STATE + 1]};
+  const int c0 = (int)((int64_t)R.cells * g / groups), c1 = (int)((int64_t)R.cells * (g + 1) / groups);
+  pass_weights<256, F>(R, A.keys + row * A.max_cells, c0, c1, cut, p.min_p, A.sums + row * A.max_cells);
+}
+// ... and the draws, `per` of a row in every workgroup
+template <class F> __global__ __launch_bounds__(Long::NT) void k_draws(DrawArgs A, int blocks, int per) {
+  typedef typename F::key K;
+  __shared__ Shared<Long> S;
+  const int64_t row = blockIdx.x / blocks;
+  const int64_t s0 = (int64_t)(blockIdx.x % blocks) * per, s1 = s0 + per < A.draws ? s0 + per : A.draws;
+  const Settings p = settings_of(A, row);
+  Row<F> R = row_of<F>(A, row, p.t);
+  const u64 kmax = best_of_row<Long::NT>(A, row, R.cells, S.red);
+  if (kmax == 0) { draw_nothing(A, row, s0, s1, Long::NT); return; }
+  R.best = F::of_key((K)kmax);
+  const Cut<K> cut{(K)A.state[row * STATE], (int64_t)A.state[row * STATE + 1]};
+  for (int c = threadIdx.x; c < R.cells; c += Long::NT) {
+    double w = A.sums[row * A.max_cells + c];
+    if (p.plain) { const u64 k = A.keys[row * A.max_cells + c]; w *= k ? exp(R.z((K)k)) : 0.0; }
+    S.cells[c] = w;
+  }
+  scan_cells(S, R.cells);
+  draw<Long, F>(A, R, S, row, s0, s1, cut, p.min_p);
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------------------------
+// How a call runs: cells of a row, workgroups per row (0: one workgroup does a whole row), draws apart from the rest or not
+struct Plan { int units, max_cells, groups; bool short_rows, draws_here; };
+Plan plan_of(int type, int64_t rows, int64_t cols, int64_t draws) {
+  Plan p;
+  const int64_t unit = 64 * (type == 0 ? 2 : type == 1 ? 4 : 8);
+  p.units = (int)((cols + unit * MAX_CELLS - 1) / (unit * MAX_CELLS));
+  p.max_cells = (int)((cols + unit * p.units - 1) / (unit * p.units));
+  p.short_rows = p.max_cells <= (rows >= 512 ? 64 : 16);
+  p.groups = (!p.short_rows && p.max_cells >= 64 && rows <= 64) ? (int)std::min<int64_t>(p.max_cells / 16, std::max<int64_t>(1, 512 / rows)) : 0;
+  p.draws_here = p.groups == 0 && draws <= 64;
+  return p;
+}
+int64_t scratch_of(const Plan& p, int64_t rows) { return p.draws_here ? 0 : rows * (2 * (int64_t)p.max_cells + p.groups + STATE); }
+
+template <class F> void launch(DrawArgs& A, const Plan& p, int64_t rows, hipStream_t st) {
+  if (p.groups == 0) {
+    if (p.short_rows) hipLaunchKernelGGL((k_row<Short, F>), dim3((unsigned)rows), dim3(Short::NT), 0, st, A, p.draws_here ? 1 : 0);
+    else hipLaunchKernelGGL((k_row<Long, F>), dim3((unsigned)rows), dim3(Long::NT), 0, st, A, p.draws_here ? 1 : 0);
+    if (p.draws_here) return;
+  } else {
+    const dim3 grid((unsigned)(rows * p.groups));
+    hipLaunchKernelGGL(k_best<F>, grid, dim3(256), 0, st, A, p.groups);
+    const bool cuts = A.temperature.p || A.temperature.v == 0.0 || A.top_k.p || A.top_k.v > 0 || A.top_p.p || A.top_p.v < 1.0;
+    if (cuts) hipLaunchKernelGGL(k_cut<F>, dim3((unsigned)rows), dim3(Long::NT), 0, st, A, p.groups);
+    if (cuts || A.min_p.p || A.min_p.v > 0.0) hipLaunchKernelGGL(k_weights<F>, grid, dim3(256), 0, st, A, p.groups);
+  }
+  // a wavefront makes one draw at a time: 16 per workgroup, more where that fills the chip anyway
+  const int per = (int)std::max<int64_t>(16, (A.draws * rows / 1024 + 15) / 16 * 16);
+  const int blocks = (int)((A.draws + per - 1) / per);
+  hipLaunchKernelGGL(k_draws<F>, dim3((unsigned)(rows * blocks)), dim3(Long::NT), 0, st, A, blocks, per);
+}
 }  // namespace
+
+extern "C" int64_t pgm_draw_scratch_doubles(int type, int64_t rows, int64_t cols, int64_t draws) {
+  if (type < 0 || type > 3 || rows < 1 || cols < 1 || cols >= MAX_COLS || draws < 1) return 0;
+  return scratch_of(plan_of(type, rows, cols, draws), rows);
+}
 
 extern "C" int pgm_draw_indices(const void* logits, int type, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride,
                                 const int64_t* lengths, const double* u, int64_t draws,
                                 double temperature, const double* temperature_row, int64_t top_k, const int64_t* top_k_row,
                                 double top_p, const double* top_p_row, double min_p, const double* min_p_row,
-                                int64_t* index, double* logp, void* stream) {
+                                int64_t* index, double* logp, double* scratch, int64_t scratch_doubles, void* stream) {
   if (!logits) return -1;
   if (type < 0 || type > 3) return -2;
   if (rows < 1 || rows > 0x7fffffff) return -3;
@@ -345,13 +704,23 @@ extern "C" int pgm_draw_indices(const void* logits, int type, int64_t rows, int6
   if (!top_p_row && !(top_p >= 0.0 && top_p <= 1.0)) return -14;
   if (!min_p_row && !(min_p >= 0.0 && min_p <= 1.0)) return -16;
   if (!index) return -18;
+  if (draws > 0x7fffffff || rows * draws > ((int64_t)1 << 40)) return -9;
+  const Plan p = plan_of(type, rows, cols, draws);
+  const int64_t need = scratch_of(p, rows);
+  if (need > 0 && !scratch) return -20;
+  if (need > scratch_doubles) return -21;
   DrawArgs A{logits, row_stride, col_stride, cols, lengths, u, draws, {temperature, temperature_row}, {top_p, top_p_row}, {min_p, min_p_row},
-             {top_k, top_k_row}, index, logp};
+             {top_k, top_k_row}, index, logp, p.units, p.max_cells, nullptr, nullptr, nullptr, nullptr};
+  if (need > 0) {
+    A.keys = reinterpret_cast<u64*>(scratch);
+    A.sums = scratch + rows * p.max_cells;
+    A.lows = reinterpret_cast<u64*>(scratch + 2 * rows * p.max_cells);
+    A.state = A.lows + rows * p.groups;
+  }
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)rows);
-  if (type == 0) hipLaunchKernelGGL(k_draw<F64>, grid, dim3(NT), 0, st, A);
-  else if (type == 1) hipLaunchKernelGGL(k_draw<F32>, grid, dim3(NT), 0, st, A);
-  else if (type == 2) hipLaunchKernelGGL(k_draw<Half<0>>, grid, dim3(NT), 0, st, A);
-  else hipLaunchKernelGGL(k_draw<Half<1>>, grid, dim3(NT), 0, st, A);
+  if (type == 0) launch<F64>(A, p, rows, st);
+  else if (type == 1) launch<F32>(A, p, rows, st);
+  else if (type == 2) launch<Half<0>>(A, p, rows, st);
+  else launch<Half<1>>(A, p, rows, st);
   return hipGetLastError() == hipSuccess ? 0 : -99;
 }

@@ -88,9 +88,12 @@ def draw_indices(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=N
         if V >= 1 << 24:
             raise ValueError(f"draw_indices: rows of at most {(1 << 24) - 1} entries, got {V}")
         (t, tp, _t), (k, kp, _k), (p, pp, _p), (m, mp, _m) = settings
+        lib, kind = _hip.load(), _TYPE[l.dtype]
+        n = int(lib.pgm_draw_scratch_doubles(kind, B, V, S))
+        scratch = torch.empty(n, dtype=torch.float64, device=dev) if n else None
         with torch.cuda.device(dev):
-            rc = _hip.load().pgm_draw_indices(l.data_ptr(), _TYPE[l.dtype], B, V, l.stride(0), l.stride(1), None if ln is None else ln.data_ptr(),
-                                              ud.data_ptr(), S, t, tp, k, kp, p, pp, m, mp, index.data_ptr(),
-                                              None if logp is None else logp.data_ptr(), _hip.current_stream_ptr(dev))
+            rc = lib.pgm_draw_indices(l.data_ptr(), kind, B, V, l.stride(0), l.stride(1), None if ln is None else ln.data_ptr(),
+                                      ud.data_ptr(), S, t, tp, k, kp, p, pp, m, mp, index.data_ptr(), None if logp is None else logp.data_ptr(),
+                                      None if scratch is None else scratch.data_ptr(), n, _hip.current_stream_ptr(dev))
         _hip._check(rc, "pgm_draw_indices")
     return (index, logp) if return_logprob else index

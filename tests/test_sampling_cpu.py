@@ -36,7 +36,7 @@ def test_settings(name, off, lo, hi, dtype, bad):
 
 def _call(**kw):
     a = dict(logits=64, type=0, rows=2, cols=5, row_stride=5, col_stride=1, lengths=None, u=64, draws=1, t=1.0, tp=None, k=0, kp=None, p=1.0, pp=None,
-             m=0.0, mp=None, index=64, logp=None, stream=None)
+             m=0.0, mp=None, index=64, logp=None, scratch=64, doubles=1 << 40, stream=None)
     a.update(kw)
     return _hip.load().pgm_draw_indices(*a.values())
 
@@ -44,7 +44,8 @@ def _call(**kw):
 @pytest.mark.parametrize("code, kw", [
     (-1, dict(logits=None)), (-2, dict(type=4)), (-2, dict(type=-1)), (-3, dict(rows=0)), (-3, dict(rows=1 << 31)), (-4, dict(cols=0)), (-4, dict(cols=1 << 24)),
     (-5, dict(row_stride=-1)), (-6, dict(col_stride=-1)), (-8, dict(u=None)), (-9, dict(draws=0)), (-10, dict(t=-1.0)), (-10, dict(t=math.nan)), (-10, dict(t=math.inf)),
-    (-12, dict(k=-1)), (-14, dict(p=1.5)), (-14, dict(p=math.nan)), (-16, dict(m=-0.5)), (-16, dict(m=2.0)), (-18, dict(index=None))])
+    (-12, dict(k=-1)), (-14, dict(p=1.5)), (-14, dict(p=math.nan)), (-16, dict(m=-0.5)), (-16, dict(m=2.0)), (-18, dict(index=None)),
+    (-20, dict(cols=200_000, scratch=None)), (-21, dict(cols=200_000, doubles=3)), (-21, dict(draws=1000, doubles=3))])
 def test_refusals_come_before_any_launch(code, kw):
     assert _call(**kw) == code
 
