@@ -17,6 +17,7 @@
 #include <stdint.h>
 #include <algorithm>
 #include "../../include/pgmuvi_hip.h"
+#include "pgm_exp.h"
 
 namespace {
 
@@ -102,10 +103,11 @@ template <class F> struct Row {
   static constexpr int VEC = LOAD / (int)sizeof(raw), UNIT = 64 * VEC;       // entries of one load of a lane, of a wavefront
   const raw* x; int64_t stride, n;
   int units, cells;
-  double best, t;
+  double best, t, per_t;                                        // highest value, temperature, 1 / temperature
   __device__ __forceinline__ int64_t width() const { return (int64_t)units * UNIT; }
   __device__ __forceinline__ K key(int64_t i) const { return F::to_key(x[i * stride]); }
   __device__ __forceinline__ double z(K k) const { const double l = F::of_key(k); return l == best ? 0.0 : (l - best) / t; }
+  __device__ __forceinline__ double weight(K k) const { const double l = F::of_key(k); return l == best ? 1.0 : exp_neg((l - best) * per_t); }
   // this lane's entries of unit j: VEC neighbours from at(j) on; key 0 (no value has it) behind the end
   __device__ __forceinline__ int64_t at(int64_t j) const { return j * UNIT + (threadIdx.x & 63) * VEC; }
   __device__ __forceinline__ void load(int64_t j, K (&k)[VEC]) const {
@@ -140,8 +142,8 @@ template <class F> __device__ __forceinline__ typename F::key key_below(double v
   return k <= neg + 1 ? neg + 1 : k - 1;
 }
 
-// Two builds of a row's code: 16 wavefronts for long rows, 4 for short ones and for the launches that share a row among workgroups
-struct Long { static constexpr int NT = 1024, BITS = 11, CELLS = MAX_CELLS, LIST = 1024; };
+// Two builds of a row's code: 8 wavefronts for long rows, 4 for short ones and for the launches that share a row among workgroups
+struct Long { static constexpr int NT = 512, BITS = 11, CELLS = MAX_CELLS, LIST = 512; };
 struct Short { static constexpr int NT = 256, BITS = 9, CELLS = 64, LIST = 256; };
 
 template <class C> struct Shared {
@@ -195,7 +197,10 @@ template <bool SEEN, int THREADS, class F, class Fn> __device__ __forceinline__ 
         if (on[s]) R.load(cc, k[s]);
       }
 #pragma unroll
-      for (int s = 0; s < BATCH; ++s) if (on[s]) f(c + s * NW, k[s], R.at(c + s * NW), true);
+      for (int s = 0; s < BATCH; ++s) {
+        if (on[s]) f(c + s * NW, k[s], R.at(c + s * NW), true);
+        __builtin_amdgcn_sched_barrier(0);                      // (one unit's arithmetic at a time: interleaved, four of them do not fit the registers)
+      }
     } else {
       for (int s = 0; s < BATCH; ++s) {
         const int cc = c + s * NW;
@@ -259,7 +264,22 @@ template <bool WEIGHTED, class C> __device__ __forceinline__ void clear_bins(Sha
 }
 template <class C> __device__ __forceinline__ int shift_of(u64 span) { return span < (u64)Shared<C>::BINS ? 0 : 64 - __clzll(span) - C::BITS; }
 
-__device__ __forceinline__ bool ahead(u64 ka, uint32_t ia, u64 kb, uint32_t ib) { return ka > kb || (ka == kb && ia < ib); }
+// The list in the order of the cut: every thread counts what is ahead of its entry (broadcast reads, two barriers; a sort by
+// exchanges takes 45 of them for 512 entries)
+template <class C> __device__ __forceinline__ void sort_list(Shared<C>& S, int count) {
+  const int t = threadIdx.x;
+  __syncthreads();
+  u64 key = 0; uint32_t idx = 0; int rank = 0, ties = 0;
+  if (t < count) { key = S.list_key[t]; idx = S.list_idx[t]; }
+  if (t - (t & 63) < count) {
+    for (int j = 0; j < count; ++j) { const u64 k = S.list_key[j]; rank += k > key; ties += k == key; }
+    if (__any(t < count && ties > 1))
+      for (int j = 0; j < count; ++j) rank += S.list_key[j] == key && S.list_idx[j] < idx;
+  }
+  __syncthreads();
+  if (t < count) { S.list_key[rank] = key; S.list_idx[rank] = idx; }
+  __syncthreads();
+}
 
 // The cut behind the first `want` entries of what `have` keeps (WEIGHTED: behind the shortest beginning with `share` of its weight).
 // kmin / kmax: range of keys that can matter; S.best: the cells' highest keys
@@ -281,7 +301,7 @@ template <bool WEIGHTED, class C, class F> __device__ Cut<typename F::key> selec
         const int b = (int)((u64)(hi - k[e]) >> shift);
         atomicAdd(&S.bins.count[b], 1u);
         if (WEIGHTED) {
-          const double w = exp(R.z(k[e])) * 0x1p40;
+          const double w = R.weight(k[e]) * 0x1p40;
           const u64 whi = (u64)w, wlo = (u64)((w - (double)whi) * 0x1p40);
           if (whi) atomicAdd(&S.bins.hi[b], whi);
           if (wlo) atomicAdd(&S.bins.lo[b], wlo);
@@ -309,23 +329,10 @@ template <bool WEIGHTED, class C, class F> __device__ Cut<typename F::key> selec
         }
       });
       const int count = (int)in_bin, t = threadIdx.x;
-      int size = 2;
-      while (size < count) size <<= 1;
-      if (t >= count && t < size) { S.list_key[t] = 0; S.list_idx[t] = 0xffffffffu; }
-      for (int span = 2; span <= size; span <<= 1)
-        for (int s = span >> 1; s > 0; s >>= 1) {
-          __syncthreads();
-          const int o = t ^ s;
-          if (t < size && o > t) {
-            const u64 ka = S.list_key[t], kb = S.list_key[o];
-            const uint32_t ia = S.list_idx[t], ib = S.list_idx[o];
-            if (ahead(kb, ib, ka, ia) == ((t & span) == 0)) { S.list_key[t] = kb; S.list_key[o] = ka; S.list_idx[t] = ib; S.list_idx[o] = ia; }
-          }
-        }
-      __syncthreads();
+      sort_list(S, count);
       int at = (int)(want - bn) - 1;
       if (WEIGHTED) {
-        const double sum = block_scan<C>(S.sums, t < count ? exp(R.z((K)S.list_key[t])) : 0.0);
+        const double sum = block_scan<C>(S.sums, t < count ? R.weight((K)S.list_key[t]) : 0.0);
         const bool yes = t < count && mass_of(bhi, blo) + sum >= target;
         at = count - 1 - (int)block_max<C>(S.red, yes ? (u64)(count - 1 - t) : 0);
       }
@@ -335,7 +342,7 @@ template <bool WEIGHTED, class C, class F> __device__ Cut<typename F::key> selec
     if (shift == 0) {                                           // many equal values: the first m of them by index
       u64 m = WEIGHTED ? 1 : want - bn;
       if (WEIGHTED) {
-        const double w = exp(R.z(top)), above = mass_of(bhi, blo);
+        const double w = R.weight(top), above = mass_of(bhi, blo);
         const double guess = ceil((target - above) / w);
         m = guess >= (double)in_bin ? in_bin : guess < 1.0 ? 1 : (u64)guess;
         while (m > 1 && above + (double)(m - 1) * w >= target) --m;
@@ -392,7 +399,7 @@ template <class F> __device__ __forceinline__ Row<F> row_of(const DrawArgs& A, i
   R.x = static_cast<const typename F::raw*>(A.logits) + row * A.row_stride; R.stride = A.col_stride; R.n = n;
   R.units = A.units;
   R.cells = (int)((n + R.width() - 1) / R.width());
-  R.best = 0.0; R.t = t;
+  R.best = 0.0; R.t = t; R.per_t = 1.0 / t;
   return R;
 }
 
@@ -420,7 +427,7 @@ template <int THREADS, class F> __device__ __forceinline__ u64 pass_best(Row<F> 
         K q[VEC];
         if (R.units > 1) R.load((int64_t)c * R.units + j, q);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) { const K x = R.units > 1 ? q[e] : k[e]; s += x > neg ? exp(R.z(x)) : 0.0; }
+        for (int e = 0; e < VEC; ++e) { const K x = R.units > 1 ? q[e] : k[e]; s += x > neg ? R.weight(x) : 0.0; }
       }
     }
     s = wave_sum(s);
@@ -445,7 +452,7 @@ template <int THREADS, class F> __device__ __forceinline__ void pass_weights(con
   for_cells<true, THREADS>(R, best, c0, c1, (u64)lo, [&](int c, const K (&k)[VEC], int64_t i, bool last) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e)
-      if (k[e] >= lo && before(cut, k[e], i + e)) { const double w = exp(R.z(k[e])); s += w < min_p ? 0.0 : w; }
+      if (k[e] >= lo && before(cut, k[e], i + e)) { const double w = R.weight(k[e]); s += w < min_p ? 0.0 : w; }
     if (!last) return;
     const double total = wave_sum(s);
     s = 0.0;
@@ -490,7 +497,7 @@ template <class C, class F> __device__ __forceinline__ void draw(const DrawArgs&
       double w = 0.0;
       if (i < R.n) {
         const K k = R.key(i);
-        if (k > neg && before(cut, k, i)) { w = exp(R.z(k)); w = w < min_p ? 0.0 : w; }
+        if (k > neg && before(cut, k, i)) { w = R.weight(k); w = w < min_p ? 0.0 : w; }
       }
       const double inc = wave_scan(w);
       const u64 hit = __ballot(w > 0.0 && base + inc > target), some = __ballot(w > 0.0);
@@ -511,21 +518,88 @@ __device__ __forceinline__ void draw_nothing(const DrawArgs& A, int64_t row, int
     if (A.logp) A.logp[row * A.draws + s] = -__builtin_inf();
   }
 }
-// the cut of a row whose cells' highest keys are in S.best; R.best is set
-template <class C, class F> __device__ Cut<typename F::key> cut_of(const Row<F>& R, Shared<C>& S, const Settings& p, u64 kmin, u64 kmax) {
+// All truncations on a list that holds the row's first top_k entries: sorts it and returns how many are kept (the first ones)
+template <class C, class F> __device__ __forceinline__ int keep_list(const Row<F>& R, Shared<C>& S, const Settings& p, int count) {
   typedef typename F::key K;
+  const int t = threadIdx.x;
+  sort_list(S, count);
+  int n = p.top_k < count ? (int)p.top_k : count;
+  const double w = t < n ? R.weight((K)S.list_key[t]) : 0.0;
+  const double sum = block_scan<C>(S.sums, w);
+  if (p.top_p < 1.0) {
+    __syncthreads();
+    if (t == n - 1) S.sums[0] = sum;
+    __syncthreads();
+    const bool yes = t < n && sum >= p.top_p * S.sums[0];
+    n -= (int)block_max<C>(S.red, yes ? (u64)(n - 1 - t) : 0);
+  }
+  const int heavy = (int)block_max<C>(S.red, t < n && w >= p.min_p ? (u64)(t + 1) : 0);      // (the best one always is)
+  return heavy;
+}
+// the draws from the first n entries of a sorted list: by index, running sums in S.cells, one thread per draw
+template <class C, class F> __device__ __forceinline__ void draw_list(const DrawArgs& A, const Row<F>& R, Shared<C>& S, int64_t row, int n) {
+  typedef typename F::key K;
+  static_assert(C::LIST <= C::CELLS || C::LIST <= Shared<C>::BINS, "running sums of the list");
+  const int t = threadIdx.x;
+  u64 key = 0; uint32_t idx = 0; int rank = 0;
+  if (t < n) { key = S.list_key[t]; idx = S.list_idx[t]; }
+  if (t - (t & 63) < n) for (int j = 0; j < n; ++j) rank += S.list_idx[j] < idx;
+  __syncthreads();
+  if (t < n) { S.list_key[rank] = key; S.list_idx[rank] = idx; }
+  __syncthreads();
+  const double sum = block_scan<C>(S.sums, t < n ? R.weight((K)S.list_key[t]) : 0.0);
+  double* run = reinterpret_cast<double*>(S.bins.hi);
+  if (t < n) run[t] = sum;
+  __syncthreads();
+  const double Z = run[n - 1], log_z = log(Z);
+  for (int64_t s = t; s < A.draws; s += C::NT) {
+    double target = A.u[row * A.draws + s] * Z;
+    target = target > 0.0 ? target : target == target ? 0.0 : Z;
+    auto first_above = [&](double x, bool or_equal) {
+      int a = 0, b = n;
+      while (a < b) { const int m = (a + b) >> 1; const double f = run[m]; if (f > x || (or_equal && f >= x)) b = m; else a = m + 1; }
+      return a;
+    };
+    int j = first_above(target, false);
+    if (j == n) j = first_above(Z, true);
+    A.index[row * A.draws + s] = (int64_t)S.list_idx[j];
+    if (A.logp) A.logp[row * A.draws + s] = R.z((K)S.list_key[j]) - log_z;
+  }
+}
+// The cut of a row whose cells' highest keys are in S.best; R.best is set.  listed > 0: the list holds exactly the kept entries
+template <class C, class F> __device__ Cut<typename F::key> cut_of(const Row<F>& R, Shared<C>& S, const Settings& p, u64 kmin, u64 kmax, int& listed) {
+  typedef typename F::key K;
+  constexpr int VEC = Row<F>::VEC;
   Cut<K> cut{neg_key<F>(), -1};
+  listed = 0;
   if (p.top_k > 0) {
     // the top_k-th highest of the cells' best is a lower bound of the cut: only cells that reach it are looked at again
     K lo = (K)kmin;
+    clear_bins<false>(S);
     if (p.top_k < R.cells) {
-      clear_bins<false>(S);
       const int shift = shift_of<C>(kmax - kmin);
       for (int c = threadIdx.x; c < R.cells; c += C::NT) if (S.best[c] >= kmin) atomicAdd(&S.bins.count[(kmax - S.best[c]) >> shift], 1u);
       find_bin<false>(S, 0, 0, 0, (u64)p.top_k, 0.0, 0.0);
       if (S.found[6] >= (u64)p.top_k) {
         const u64 drop = ((S.found[0] + 1) << shift) - 1;       // (to the lowest key of the bin)
         if (drop < kmax - kmin) lo = (K)(kmax - drop);
+      }
+    }
+    if (p.top_k <= C::LIST && (lo > kmin || R.n <= C::LIST)) {
+      // few: all entries that reach it, if they fit the list -- everything else happens there
+      for_cells<true, C::NT>(R, S.best, 0, R.cells, lo, [&](int, const K (&k)[VEC], int64_t i, bool) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          if (k[e] < lo) continue;
+          const int at = atomicAdd(&S.listed, 1);
+          if (at < C::LIST) { S.list_key[at] = k[e]; S.list_idx[at] = (uint32_t)(i + e); }
+        }
+      });
+      __syncthreads();
+      const int count = S.listed;
+      if (count <= C::LIST) {
+        listed = keep_list<C, F>(R, S, p, count);
+        return Cut<K>{(K)S.list_key[listed - 1], (int64_t)S.list_idx[listed - 1]};
       }
     }
     cut = tighter(cut, select<false, C, F>(R, S, lo, (K)kmax, cut, (u64)p.top_k, 0.0));
@@ -540,7 +614,7 @@ template <class C, class F> __device__ Cut<typename F::key> cut_of(const Row<F>&
 
 // ---- kernels --------------------------------------------------------------------------------------------------------------------------
 // One workgroup per row: everything, or (draws_here 0: many draws per row) all but the draws, which k_draws makes from memory
-template <class C, class F> __global__ __launch_bounds__(C::NT) void k_row(DrawArgs A, int draws_here) {
+template <class C, class F> __global__ __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(4))) void k_row(DrawArgs A, int draws_here) {
   typedef typename F::key K;
   __shared__ Shared<C> S;
   const int64_t row = blockIdx.x;
@@ -556,11 +630,13 @@ template <class C, class F> __global__ __launch_bounds__(C::NT) void k_row(DrawA
     R.best = F::of_key((K)kmax);
     if (!p.plain) {
       const u64 kmin = ~block_max<C>(S.red, ~low);
-      cut = cut_of<C, F>(R, S, p, kmin, kmax);
+      int listed;
+      cut = cut_of<C, F>(R, S, p, kmin, kmax, listed);
+      if (listed && draws_here) { draw_list<C, F>(A, R, S, row, listed); return; }
       __syncthreads();                                          // (the cells take the bins' place)
       pass_weights<C::NT, F>(R, S.best, 0, R.cells, cut, p.min_p, S.cells);
     } else if (draws_here) {
-      for (int c = threadIdx.x; c < R.cells; c += C::NT) S.cells[c] *= S.best[c] ? exp(R.z((K)S.best[c])) : 0.0;
+      for (int c = threadIdx.x; c < R.cells; c += C::NT) S.cells[c] *= S.best[c] ? R.weight((K)S.best[c]) : 0.0;
     }
   }
   if (draws_here) {
@@ -591,7 +667,7 @@ template <class F> __global__ __launch_bounds__(256) void k_best(DrawArgs A, int
   }
 }
 // ... the cut (only where one may be asked for)
-template <class F> __global__ __launch_bounds__(Long::NT) void k_cut(DrawArgs A, int groups) {
+template <class F> __global__ __launch_bounds__(Long::NT) __attribute__((amdgpu_waves_per_eu(4))) void k_cut(DrawArgs A, int groups) {
   typedef typename F::key K;
   __shared__ Shared<Long> S;
   const int64_t row = blockIdx.x;
@@ -603,7 +679,8 @@ template <class F> __global__ __launch_bounds__(Long::NT) void k_cut(DrawArgs A,
   const u64 kmax = block_max<Long>(S.red, top), kmin = ~block_max<Long>(S.red, ~low);
   if (kmax == 0) return;
   R.best = F::of_key((K)kmax);
-  const Cut<K> cut = cut_of<Long, F>(R, S, p, kmin, kmax);
+  int listed;
+  const Cut<K> cut = cut_of<Long, F>(R, S, p, kmin, kmax, listed);
   if (threadIdx.x == 0) { A.state[row * STATE] = (u64)cut.key; A.state[row * STATE + 1] = (u64)cut.idx; }
 }
 template <int THREADS> __device__ __forceinline__ u64 best_of_row(const DrawArgs& A, int64_t row, int cells, u64 (&red)[THREADS / 64]) {
@@ -640,7 +717,7 @@ template <class F> __global__ __launch_bounds__(Long::NT) void k_draws(DrawArgs 
   const Cut<K> cut{(K)A.state[row * STATE], (int64_t)A.state[row * STATE + 1]};
   for (int c = threadIdx.x; c < R.cells; c += Long::NT) {
     double w = A.sums[row * A.max_cells + c];
-    if (p.plain) { const u64 k = A.keys[row * A.max_cells + c]; w *= k ? exp(R.z((K)k)) : 0.0; }
+    if (p.plain) { const u64 k = A.keys[row * A.max_cells + c]; w *= k ? R.weight((K)k) : 0.0; }
     S.cells[c] = w;
   }
   scan_cells(S, R.cells);
@@ -674,7 +751,7 @@ template <class F> void launch(DrawArgs& A, const Plan& p, int64_t rows, hipStre
     if (cuts) hipLaunchKernelGGL(k_cut<F>, dim3((unsigned)rows), dim3(Long::NT), 0, st, A, p.groups);
     if (cuts || A.min_p.p || A.min_p.v > 0.0) hipLaunchKernelGGL(k_weights<F>, grid, dim3(256), 0, st, A, p.groups);
   }
-  // a wavefront makes one draw at a time: 16 per workgroup, more where that fills the chip anyway
+  // a wavefront makes one draw at a time: two each, more where that fills the chip anyway
   const int per = (int)std::max<int64_t>(16, (A.draws * rows / 1024 + 15) / 16 * 16);
   const int blocks = (int)((A.draws + per - 1) / per);
   hipLaunchKernelGGL(k_draws<F>, dim3((unsigned)(rows * blocks)), dim3(Long::NT), 0, st, A, blocks, per);
