@@ -27,39 +27,47 @@ constexpr int MAX_CELLS = 2048;                                 // of a row (wid
 constexpr int64_t MAX_COLS = 1 << 24;                             // (2^24 weights of at most one, in steps of 2^-40, fit 64 bits)
 constexpr int64_t EVERY = INT64_MAX;
 
-// ---- values and their keys: unsigned integers in the same order; -0 is +0, NaN is -inf ------------------------------------
+// ---- values and their keys: unsigned integers in the same order; -0 is +0, NaN is -inf.  `wide`: what maxima are formed in -----
+__device__ __forceinline__ u64 key_of_bits(u64 b) { return (b >> 63) ? ~b : b | (1ull << 63); }
+__device__ __forceinline__ uint32_t key_of_bits(uint32_t b) { return (b >> 31) ? ~b : b | (1u << 31); }
 struct F64 {
-  typedef double raw; typedef u64 key;
-  static __device__ __forceinline__ double value(raw x) { return x; }
-  static __device__ __forceinline__ key to_key(raw x) {
-    x = x != x ? -__builtin_inf() : x + 0.0;
-    const u64 b = (u64)__double_as_longlong(x);
-    return (b >> 63) ? ~b : b | (1ull << 63);
-  }
+  typedef double raw, wide; typedef u64 key;
+  static constexpr raw absent() { return -__builtin_inf(); }
+  static __device__ __forceinline__ wide widen(raw x) { return x; }
+  static __device__ __forceinline__ wide larger(wide a, wide b) { return __builtin_fmax(a, b); }        // (a NaN loses)
+  static __device__ __forceinline__ key to_key(raw x) { return key_of_bits((u64)__double_as_longlong(x != x ? absent() : x + 0.0)); }
+  static __device__ __forceinline__ key key_of_wide(wide x) { return to_key(x); }
   static __device__ __forceinline__ double of_key(key k) { return __longlong_as_double((long long)((k >> 63) ? k & ~(1ull << 63) : ~k)); }
 };
 struct F32 {
-  typedef float raw; typedef uint32_t key;
-  static __device__ __forceinline__ key to_key(float x) {
-    x = x != x ? -__builtin_inff() : x + 0.0f;
-    const uint32_t b = __float_as_uint(x);
-    return (b >> 31) ? ~b : b | (1u << 31);
-  }
+  typedef float raw, wide; typedef uint32_t key;
+  static constexpr raw absent() { return -__builtin_inff(); }
+  static __device__ __forceinline__ wide widen(raw x) { return x; }
+  static __device__ __forceinline__ wide larger(wide a, wide b) { return __builtin_fmaxf(a, b); }
+  static __device__ __forceinline__ key to_key(raw x) { return key_of_bits(__float_as_uint(x != x ? absent() : x + 0.0f)); }
+  static __device__ __forceinline__ key key_of_wide(wide x) { return to_key(x); }
   static __device__ __forceinline__ double of_key(key k) { return (double)__uint_as_float((k >> 31) ? k & ~(1u << 31) : ~k); }
 };
 template <int F16BIT> struct Half {                              // bf16 (0) and fp16 (1): the 16-bit patterns are ordered the same way
-  typedef uint16_t raw; typedef uint32_t key;
-  static __device__ __forceinline__ key to_key(uint16_t b) {
-    const uint32_t inf = F16BIT ? 0x7c00u : 0x7f80u, mag = b & 0x7fffu;
-    if (mag > inf) return 0xffffu - (0x8000u | inf);
+  typedef uint16_t raw; typedef float wide; typedef uint32_t key;
+  static constexpr uint32_t INF = F16BIT ? 0x7c00u : 0x7f80u;
+  static constexpr raw absent() { return (raw)(0x8000u | INF); }
+  static __device__ __forceinline__ wide widen(raw b) {
+    if constexpr (F16BIT) { __half_raw r; r.x = b; return __half2float(__half(r)); }
+    else return __uint_as_float((uint32_t)b << 16);
+  }
+  static __device__ __forceinline__ wide larger(wide a, wide b) { return __builtin_fmaxf(a, b); }
+  static __device__ __forceinline__ key to_key(raw b) {
+    const uint32_t mag = b & 0x7fffu;
+    if (mag > INF) return 0xffffu - (0x8000u | INF);
     if (mag == 0) return 0x8000u;
     return (b >> 15) ? 0xffffu - b : b | 0x8000u;
   }
-  static __device__ __forceinline__ double of_key(key k) {
-    const uint16_t b = (uint16_t)((k & 0x8000u) ? k & 0x7fffu : 0xffffu - k);
-    if constexpr (F16BIT) { __half_raw r; r.x = b; return (double)__half2float(__half(r)); }
-    else return (double)__uint_as_float((uint32_t)b << 16);
+  static __device__ __forceinline__ key key_of_wide(wide x) {     // (x is one of the type's values)
+    if constexpr (F16BIT) { const __half h = __float2half(x); return to_key(static_cast<__half_raw>(h).x); }
+    else return to_key((raw)(__float_as_uint(x) >> 16));
   }
+  static __device__ __forceinline__ double of_key(key k) { return (double)widen((raw)((k & 0x8000u) ? k & 0x7fffu : 0xffffu - k)); }
 };
 
 struct Param { double v; const double* p; };                    // one number for every row, or one per row
@@ -79,14 +87,26 @@ template <class K> struct Cut { K key; int64_t idx; };          // kept: key abo
 template <class K> __device__ __forceinline__ bool before(const Cut<K>& c, K key, int64_t i) { return key > c.key || (key == c.key && i <= c.idx); }
 
 // ---- wavefront reductions -------------------------------------------------------------------------------------------------
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
-  return v;
+// (within rows of 16 lanes by data-parallel moves -- a shuffle goes through the LDS, ~100 cycles a step --, the four rows by lane reads)
+template <int CTRL> __device__ __forceinline__ double moved(double v) {
+  return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, true), __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, true));
 }
-template <class V> __device__ __forceinline__ V wave_max(V v) {
+template <int CTRL> __device__ __forceinline__ float moved(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true)); }
+__device__ __forceinline__ double of_lane(double v, int l) { return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), l), __builtin_amdgcn_readlane(__double2loint(v), l)); }
+__device__ __forceinline__ float of_lane(float v, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); }
+template <class V, class Op> __device__ __forceinline__ V wave_join(V v, Op op) {
+  v = op(v, moved<0xB1>(v));                                    // neighbours, pairs, halves of a row, the row
+  v = op(v, moved<0x4E>(v));
+  v = op(v, moved<0x141>(v));
+  v = op(v, moved<0x140>(v));
+  return op(op(of_lane(v, 0), of_lane(v, 16)), op(of_lane(v, 32), of_lane(v, 48)));
+}
+__device__ __forceinline__ double wave_sum(double v) { return wave_join(v, [](double a, double b) { return a + b; }); }
+__device__ __forceinline__ float wave_max(float v) { return wave_join(v, [](float a, float b) { return __builtin_fmaxf(a, b); }); }
+__device__ __forceinline__ double wave_max(double v) { return wave_join(v, [](double a, double b) { return __builtin_fmax(a, b); }); }
+__device__ __forceinline__ u64 wave_max(u64 v) {
 #pragma unroll
-  for (int s = 32; s > 0; s >>= 1) { const V o = __shfl_xor(v, s); v = o > v ? o : v; }
+  for (int s = 32; s > 0; s >>= 1) { const u64 o = __shfl_xor(v, s); v = o > v ? o : v; }
   return v;
 }
 template <class V> __device__ __forceinline__ V wave_scan(V v) {
@@ -107,25 +127,21 @@ template <class F> struct Row {
   __device__ __forceinline__ int64_t width() const { return (int64_t)units * UNIT; }
   __device__ __forceinline__ K key(int64_t i) const { return F::to_key(x[i * stride]); }
   __device__ __forceinline__ double z(K k) const { const double l = F::of_key(k); return l == best ? 0.0 : (l - best) / t; }
-  __device__ __forceinline__ double weight(K k) const { const double l = F::of_key(k); return l == best ? 1.0 : exp_neg((l - best) * per_t); }
-  // this lane's entries of unit j: VEC neighbours from at(j) on; key 0 (no value has it) behind the end
+  __device__ __forceinline__ double weight_of(double l) const { return l == best ? 1.0 : exp_neg((l - best) * per_t); }      // (l above -inf)
+  __device__ __forceinline__ double weight(K k) const { return weight_of(F::of_key(k)); }
+  // this lane's entries of unit j: VEC neighbours from at(j) on; behind the end -inf
   __device__ __forceinline__ int64_t at(int64_t j) const { return j * UNIT + (threadIdx.x & 63) * VEC; }
-  __device__ __forceinline__ void load(int64_t j, K (&k)[VEC]) const {
+  __device__ __forceinline__ bool whole(int64_t j) const { return stride == 1 && (j + 1) * UNIT <= n; }
+  __device__ __forceinline__ void load_whole(int64_t j, raw (&r)[VEC]) const { __builtin_memcpy(r, x + at(j), LOAD); }
+  __device__ __forceinline__ void load(int64_t j, raw (&r)[VEC]) const {
     const int64_t i = at(j);
-    if (stride == 1 && (j + 1) * UNIT <= n) {
-      raw r[VEC];
-      __builtin_memcpy(r, x + i, LOAD);
+    if (whole(j)) { load_whole(j, r); return; }
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) k[e] = F::to_key(r[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) k[e] = i + e < n ? F::to_key(x[(i + e) * stride]) : (K)0;
-    }
+    for (int e = 0; e < VEC; ++e) r[e] = i + e < n ? x[(i + e) * stride] : F::absent();
   }
 };
 template <class F> __device__ __forceinline__ typename F::key neg_key() {                     // the key of -inf (and NaN)
-  if constexpr (sizeof(typename F::raw) == 2) return F::to_key((typename F::raw)0xffffu);
-  else return F::to_key((typename F::raw)(-__builtin_inf()));
+  return F::to_key(F::absent());
 }
 // a key above that of -inf and not above any whose value is at least v
 template <class F> __device__ __forceinline__ typename F::key key_below(double v) {
@@ -180,38 +196,44 @@ template <class C> __device__ __forceinline__ double block_scan(double (&sums)[C
   return base + inc;
 }
 
-// f(cell, this lane's keys of one unit, first index, last unit of the cell?) for the cells c0 <= c < c1 -- with SEEN only those whose
-// highest key is at least `lo`: a wavefront per cell, BATCH cells' loads in flight
-template <bool SEEN, int THREADS, class F, class Fn> __device__ __forceinline__ void for_cells(const Row<F>& R, const u64* best, int c0, int c1, u64 lo, Fn f) {
-  typedef typename F::key K;
-  constexpr int NW = THREADS / 64, VEC = Row<F>::VEC;
+// f(cell, this lane's entries of one unit, first index, last unit of the cell?) for the cells c0 <= c < c1 -- with SEEN only those
+// whose highest key is at least `lo`: a wavefront per cell.  The next BATCH cells' loads are in flight while the present ones are
+// worked on.
+template <bool SEEN, int THREADS, bool HEAVY = true, class F, class Fn> __device__ __forceinline__ void for_cells(const Row<F>& R, const u64* best, int c0, int c1, u64 lo, Fn f) {
+  typedef typename F::raw raw;
+  constexpr int NW = THREADS / 64, VEC = Row<F>::VEC, STEP = NW * BATCH;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  for (int c = c0 + wave; c < c1; c += NW * BATCH) {
-    if (R.units == 1) {
-      K k[BATCH][VEC];
-      bool on[BATCH];
+  int full = c0;                                                // the cells up to here are one whole load per lane
+  if (R.units == 1 && R.stride == 1) {
+    const int whole = (int)(R.n / Row<F>::UNIT);
+    full = whole < c1 ? whole : c1;
+    raw next[BATCH][VEC];
+    auto wanted = [&](int cc) { return cc < full && (!SEEN || best[cc] >= lo); };
+    auto fetch = [&](int c) {
+#pragma unroll
+      for (int s = 0; s < BATCH; ++s) if (wanted(c + s * NW)) R.load_whole(c + s * NW, next[s]);
+    };
+    int c = c0 + wave;
+    if (c < full) fetch(c);
+    for (; c < full; c += STEP) {
+      raw r[BATCH][VEC];
+      __builtin_memcpy(r, next, sizeof(r));
+      if (c + STEP < full) fetch(c + STEP);
 #pragma unroll
       for (int s = 0; s < BATCH; ++s) {
-        const int cc = c + s * NW;
-        on[s] = cc < c1 && (!SEEN || best[cc] >= lo);
-        if (on[s]) R.load(cc, k[s]);
+        if (wanted(c + s * NW)) f(c + s * NW, r[s], R.at(c + s * NW), true);
+        if (HEAVY) __builtin_amdgcn_sched_barrier(0);           // (one unit's exponentials at a time: interleaved, four units' do not fit the registers)
       }
-#pragma unroll
-      for (int s = 0; s < BATCH; ++s) {
-        if (on[s]) f(c + s * NW, k[s], R.at(c + s * NW), true);
-        __builtin_amdgcn_sched_barrier(0);                      // (one unit's arithmetic at a time: interleaved, four of them do not fit the registers)
-      }
-    } else {
-      for (int s = 0; s < BATCH; ++s) {
-        const int cc = c + s * NW;
-        if (cc >= c1 || (SEEN && best[cc] < lo)) continue;
-        for (int j = 0; j < R.units; ++j) {
-          K k[VEC];
-          const int64_t u = (int64_t)cc * R.units + j;
-          R.load(u, k);
-          f(cc, k, R.at(u), j == R.units - 1);
-        }
-      }
+    }
+    full = full > c0 ? full : c0;
+  }
+  for (int c = full + wave; c < c1; c += NW) {                  // the row's end; strided rows; very long ones
+    if (SEEN && best[c] < lo) continue;
+    for (int j = 0; j < R.units; ++j) {
+      raw r[VEC];
+      const int64_t u = (int64_t)c * R.units + j;
+      R.load(u, r);
+      f(c, r, R.at(u), j == R.units - 1);
     }
   }
 }
@@ -281,31 +303,42 @@ template <class C> __device__ __forceinline__ void sort_list(Shared<C>& S, int c
   __syncthreads();
 }
 
+// adds a weight to a bin: 2^-40 steps in one word, 2^-80 steps in the other (the magic number 2^52 leaves the rounded integer in the
+// low bits of a sum)
+template <class C> __device__ __forceinline__ void add_weight(Shared<C>& S, int b, double w) {
+  const double x = w * 0x1p40, magic = 0x1p52, h = __builtin_floor(x), l = (x - h) * 0x1p40;
+  const u64 hi = (u64)__double_as_longlong(h + magic) & ((1ull << 52) - 1), lo = (u64)__double_as_longlong(l + magic) & ((1ull << 52) - 1);
+  if (hi) atomicAdd(&S.bins.hi[b], hi);
+  if (lo) atomicAdd(&S.bins.lo[b], lo);
+}
+
 // The cut behind the first `want` entries of what `have` keeps (WEIGHTED: behind the shortest beginning with `share` of its weight).
-// kmin / kmax: range of keys that can matter; S.best: the cells' highest keys
-template <bool WEIGHTED, class C, class F> __device__ Cut<typename F::key> select(const Row<F>& R, Shared<C>& S, typename F::key kmin, typename F::key kmax,
+// lo / hi: range of keys that can matter; S.best: the cells' highest keys.  The first bins divide the range of values evenly,
+// the later ones (where a bin held too many to sort) the range of the bin's keys.
+template <bool WEIGHTED, class C, class F> __device__ Cut<typename F::key> select(const Row<F>& R, Shared<C>& S, typename F::key lo, typename F::key hi,
                                                                                   Cut<typename F::key> have, u64 want, double share) {
   typedef typename F::key K;
-  constexpr int VEC = Row<F>::VEC;
-  K hi = kmax, lo = kmin;
+  typedef typename F::raw raw;
+  constexpr int VEC = Row<F>::VEC, BINS = Shared<C>::BINS;
   u64 bn = 0, bhi = 0, blo = 0;
   double target = -1.0;
   bool first = true;
+  const double range = F::of_key(hi) - F::of_key(lo), scale = BINS / range;
+  bool even = range > 0.0 && range < 1e300 && scale < 1e300;
+  const double best = R.best;
+  auto even_bin = [&](double l) { const int b = (int)((best - l) * scale); return b < BINS ? b : BINS - 1; };
   for (;;) {
     const int shift = shift_of<C>((u64)(hi - lo));
     clear_bins<WEIGHTED>(S);
-    for_cells<true, C::NT>(R, S.best, 0, R.cells, lo, [&](int, const K (&k)[VEC], int64_t i, bool) {
+    for_cells<true, C::NT>(R, S.best, 0, R.cells, lo, [&](int, const raw (&r)[VEC], int64_t i, bool) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        if (k[e] < lo || k[e] > hi || !before(have, k[e], i + e)) continue;
-        const int b = (int)((u64)(hi - k[e]) >> shift);
+        const K k = F::to_key(r[e]);
+        if (k < lo || k > hi || !before(have, k, i + e)) continue;
+        const double l = (double)F::widen(r[e]);
+        const int b = even ? even_bin(l) : (int)((u64)(hi - k) >> shift);
         atomicAdd(&S.bins.count[b], 1u);
-        if (WEIGHTED) {
-          const double w = R.weight(k[e]) * 0x1p40;
-          const u64 whi = (u64)w, wlo = (u64)((w - (double)whi) * 0x1p40);
-          if (whi) atomicAdd(&S.bins.hi[b], whi);
-          if (wlo) atomicAdd(&S.bins.lo[b], wlo);
-        }
+        if (WEIGHTED) { add_weight(S, b, R.weight_of(l)); __builtin_amdgcn_sched_barrier(0); }
       }
     });
     find_bin<WEIGHTED>(S, bn, bhi, blo, want, share, target);
@@ -313,19 +346,22 @@ template <bool WEIGHTED, class C, class F> __device__ Cut<typename F::key> selec
     first = false;
     const u64 bin = S.found[0], in_bin = S.found[2];
     bn = S.found[1]; bhi = S.found[3]; blo = S.found[4]; target = __longlong_as_double((long long)S.found[5]);
-    const K top = (K)(hi - (K)(bin << shift));
-    const u64 width = (1ull << shift) - 1;
-    const K bottom = (u64)(top - lo) <= width ? lo : (K)(top - (K)width);
-    Cut<K> cut{bottom, EVERY};
-    if (in_bin <= 1 || (!WEIGHTED && bn + in_bin == want)) return cut;
+    K top = hi, bottom = lo;
+    if (!even) {
+      top = (K)(hi - (K)(bin << shift));
+      const u64 width = (1ull << shift) - 1;
+      bottom = (u64)(top - lo) <= width ? lo : (K)(top - (K)width);
+    }
+    auto in_it = [&](K k, raw r) { return k >= bottom && k <= top && (!even || even_bin((double)F::widen(r)) == (int)bin); };
     if (in_bin <= (u64)C::LIST) {
       // few enough to sort: the bin's entries by (key, index), then the first that reaches the target
-      for_cells<true, C::NT>(R, S.best, 0, R.cells, bottom, [&](int, const K (&k)[VEC], int64_t i, bool) {
+      for_cells<true, C::NT>(R, S.best, 0, R.cells, bottom, [&](int, const raw (&r)[VEC], int64_t i, bool) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          if (k[e] < bottom || k[e] > top || !before(have, k[e], i + e)) continue;
+          const K k = F::to_key(r[e]);
+          if (!in_it(k, r[e]) || !before(have, k, i + e)) continue;
           const int at = atomicAdd(&S.listed, 1);
-          S.list_key[at] = k[e]; S.list_idx[at] = (uint32_t)(i + e);
+          S.list_key[at] = k; S.list_idx[at] = (uint32_t)(i + e);
         }
       });
       const int count = (int)in_bin, t = threadIdx.x;
@@ -336,9 +372,24 @@ template <bool WEIGHTED, class C, class F> __device__ Cut<typename F::key> selec
         const bool yes = t < count && mass_of(bhi, blo) + sum >= target;
         at = count - 1 - (int)block_max<C>(S.red, yes ? (u64)(count - 1 - t) : 0);
       }
-      cut.key = (K)S.list_key[at]; cut.idx = (int64_t)S.list_idx[at];
-      return cut;
+      return Cut<K>{(K)S.list_key[at], (int64_t)S.list_idx[at]};
     }
+    if (even) {                                                 // the keys of the bin's entries
+      u64 high = 0, low = ~0ull;
+      for_cells<true, C::NT>(R, S.best, 0, R.cells, lo, [&](int, const raw (&r)[VEC], int64_t i, bool) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const K k = F::to_key(r[e]);
+          if (!in_it(k, r[e]) || !before(have, k, i + e)) continue;
+          high = (u64)k > high ? (u64)k : high; low = (u64)k < low ? (u64)k : low;
+        }
+      });
+      hi = (K)block_max<C>(S.red, high); lo = (K)~block_max<C>(S.red, ~low);
+      even = false;
+      if (!WEIGHTED && bn + in_bin == want) return Cut<K>{lo, EVERY};
+      continue;
+    }
+    if (!WEIGHTED && bn + in_bin == want) return Cut<K>{bottom, EVERY};
     if (shift == 0) {                                           // many equal values: the first m of them by index
       u64 m = WEIGHTED ? 1 : want - bn;
       if (WEIGHTED) {
@@ -348,16 +399,16 @@ template <bool WEIGHTED, class C, class F> __device__ Cut<typename F::key> selec
         while (m > 1 && above + (double)(m - 1) * w >= target) --m;
         while (m < in_bin && above + (double)m * w < target) ++m;
       }
-      if (m >= in_bin) return cut;
+      if (m >= in_bin) return Cut<K>{bottom, EVERY};
       int64_t i0 = 0, i1 = R.n - 1;
       u64 passed = 0;
       for (;;) {
         const int ishift = shift_of<C>((u64)(i1 - i0));
         clear_bins<false>(S);
-        for_cells<true, C::NT>(R, S.best, (int)(i0 / R.width()), (int)(i1 / R.width()) + 1, top, [&](int, const K (&k)[VEC], int64_t i, bool) {
+        for_cells<true, C::NT>(R, S.best, (int)(i0 / R.width()), (int)(i1 / R.width()) + 1, top, [&](int, const raw (&r)[VEC], int64_t i, bool) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e)
-            if (k[e] == top && i + e >= i0 && i + e <= i1 && before(have, top, i + e)) atomicAdd(&S.bins.count[(u64)(i + e - i0) >> ishift], 1u);
+            if (F::to_key(r[e]) == top && i + e >= i0 && i + e <= i1 && before(have, top, i + e)) atomicAdd(&S.bins.count[(u64)(i + e - i0) >> ishift], 1u);
         });
         find_bin<false>(S, passed, 0, 0, m, 0.0, 0.0);
         const int64_t from = i0 + (int64_t)(S.found[0] << ishift), to = from + (int64_t)((1ull << ishift) - 1);
@@ -365,7 +416,7 @@ template <bool WEIGHTED, class C, class F> __device__ Cut<typename F::key> selec
         const u64 here = S.found[2];
         i0 = from;
         i1 = to < i1 ? to : i1;
-        if (ishift == 0 || passed + here == m) { cut.key = top; cut.idx = i1; return cut; }
+        if (ishift == 0 || passed + here == m) return Cut<K>{top, i1};
       }
     }
     hi = top; lo = bottom;
@@ -403,37 +454,50 @@ template <class F> __device__ __forceinline__ Row<F> row_of(const DrawArgs& A, i
   return R;
 }
 
+// does the cut need the lowest key of the row (as the end of the bins' range)?
+__device__ __forceinline__ bool wants_lowest(const Settings& p, int cells) { return p.top_k >= cells || (p.top_k == 0 && p.top_p < 1.0); }
+
 // ---- the passes over a row ----------------------------------------------------------------------------------------------------------
-// highest key of the cells [c0, c1) -> keys[c]; where nothing is truncated (sums != null) also their weight relative to it.
-// Returns this lane's lowest key above -inf
-template <int THREADS, class F> __device__ __forceinline__ u64 pass_best(Row<F> R, int c0, int c1, u64* keys, double* sums) {
-  typedef typename F::key K;
+// highest key of the cells [c0, c1) -> keys[c]; where nothing is truncated (SUMS) also their weight relative to it.
+// Returns, where `lowest` asks for it, this lane's lowest value above -inf (else +inf)
+template <int THREADS, bool SUMS, class F> __device__ __forceinline__ typename F::wide pass_best(Row<F> R, int c0, int c1, u64* keys, double* sums, bool lowest) {
+  typedef typename F::raw raw;
+  typedef typename F::wide wide;
   constexpr int VEC = Row<F>::VEC;
-  const K neg = neg_key<F>();
-  u64 kmin = ~0ull;
-  K run = 0;
-  for_cells<false, THREADS>(R, (const u64*)nullptr, c0, c1, 0, [&](int c, const K (&k)[VEC], int64_t, bool last) {
+  const wide none = (wide)-__builtin_inf();
+  wide run = none, low = -none;
+  for_cells<false, THREADS, SUMS>(R, (const u64*)nullptr, c0, c1, 0, [&](int c, const raw (&r)[VEC], int64_t, bool last) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) { run = k[e] > run ? k[e] : run; if (k[e] > neg && (u64)k[e] < kmin) kmin = k[e]; }
+    for (int e = 0; e < VEC; ++e) run = F::larger(run, F::widen(r[e]));
+    if (lowest) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) { const wide v = F::widen(r[e]); low = v > none && v < low ? v : low; }
+    }
     if (!last) return;
-    const K top = wave_max(run);
-    run = 0;
-    if ((threadIdx.x & 63) == 0) keys[c] = top > neg ? (u64)top : 0;
-    if (!sums) return;
+    const wide top = wave_max(run);
+    run = none;
+    if ((threadIdx.x & 63) == 0) keys[c] = top > none ? (u64)F::key_of_wide(top) : 0;
+    if constexpr (!SUMS) return;
     double s = 0.0;
-    if (top > neg) {
-      R.best = F::of_key(top);
-      for (int j = 0; j < R.units; ++j) {
-        K q[VEC];
-        if (R.units > 1) R.load((int64_t)c * R.units + j, q);
+    if (top > none) {
+      R.best = (double)top;
+      auto add = [&](raw x) { const wide v = F::widen(x); s += v > none ? R.weight_of((double)v) : 0.0; };
+      if (R.units == 1) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) { const K x = R.units > 1 ? q[e] : k[e]; s += x > neg ? R.weight(x) : 0.0; }
+        for (int e = 0; e < VEC; ++e) { add(r[e]); if (e & 1) __builtin_amdgcn_sched_barrier(0); }
+      } else {
+        for (int j = 0; j < R.units; ++j) {
+          raw q[VEC];
+          R.load((int64_t)c * R.units + j, q);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) { add(q[e]); if (e & 1) __builtin_amdgcn_sched_barrier(0); }
+        }
       }
     }
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) sums[c] = s;
   });
-  return kmin;
+  return low;
 }
 // kept weight of the cells [c0, c1) -> sums[c]
 template <int THREADS, class F> __device__ __forceinline__ void pass_weights(const Row<F>& R, const u64* best, int c0, int c1, const Cut<typename F::key>& cut, double min_p, double* sums) {
@@ -449,10 +513,13 @@ template <int THREADS, class F> __device__ __forceinline__ void pass_weights(con
   }
   for (int c = c0 + (int)threadIdx.x; c < c1; c += THREADS) if (best[c] < (u64)lo) sums[c] = 0.0;
   double s = 0.0;
-  for_cells<true, THREADS>(R, best, c0, c1, (u64)lo, [&](int c, const K (&k)[VEC], int64_t i, bool last) {
+  for_cells<true, THREADS>(R, best, c0, c1, (u64)lo, [&](int c, const typename F::raw (&r)[VEC], int64_t i, bool last) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e)
-      if (k[e] >= lo && before(cut, k[e], i + e)) { const double w = R.weight(k[e]); s += w < min_p ? 0.0 : w; }
+    for (int e = 0; e < VEC; ++e) {
+      const K k = F::to_key(r[e]);
+      if (k >= lo && before(cut, k, i + e)) { const double w = R.weight_of((double)F::widen(r[e])); s += w < min_p ? 0.0 : w; }
+      if (e & 1) __builtin_amdgcn_sched_barrier(0);
+    }
     if (!last) return;
     const double total = wave_sum(s);
     s = 0.0;
@@ -573,26 +640,31 @@ template <class C, class F> __device__ Cut<typename F::key> cut_of(const Row<F>&
   Cut<K> cut{neg_key<F>(), -1};
   listed = 0;
   if (p.top_k > 0) {
-    // the top_k-th highest of the cells' best is a lower bound of the cut: only cells that reach it are looked at again
+    // The top_k-th highest of the cells' best is a lower bound of the cut: only cells that reach it are looked at again.  (kmin: the
+    // lowest key of the row where wants_lowest asked for it, else the lowest there can be)
     K lo = (K)kmin;
     clear_bins<false>(S);
     if (p.top_k < R.cells) {
-      const int shift = shift_of<C>(kmax - kmin);
-      for (int c = threadIdx.x; c < R.cells; c += C::NT) if (S.best[c] >= kmin) atomicAdd(&S.bins.count[(kmax - S.best[c]) >> shift], 1u);
+      u64 low = ~0ull;
+      for (int c = threadIdx.x; c < R.cells; c += C::NT) { const u64 k = S.best[c]; low = k && k < low ? k : low; }
+      low = ~block_max<C>(S.red, ~low);
+      const int shift = shift_of<C>(kmax - low);
+      for (int c = threadIdx.x; c < R.cells; c += C::NT) if (S.best[c]) atomicAdd(&S.bins.count[(kmax - S.best[c]) >> shift], 1u);
       find_bin<false>(S, 0, 0, 0, (u64)p.top_k, 0.0, 0.0);
       if (S.found[6] >= (u64)p.top_k) {
         const u64 drop = ((S.found[0] + 1) << shift) - 1;       // (to the lowest key of the bin)
-        if (drop < kmax - kmin) lo = (K)(kmax - drop);
+        lo = (K)(drop < kmax - low ? kmax - drop : low);
       }
     }
-    if (p.top_k <= C::LIST && (lo > kmin || R.n <= C::LIST)) {
+    if (p.top_k <= C::LIST && (lo > (K)kmin || R.n <= C::LIST)) {
       // few: all entries that reach it, if they fit the list -- everything else happens there
-      for_cells<true, C::NT>(R, S.best, 0, R.cells, lo, [&](int, const K (&k)[VEC], int64_t i, bool) {
+      for_cells<true, C::NT>(R, S.best, 0, R.cells, lo, [&](int, const typename F::raw (&r)[VEC], int64_t i, bool) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          if (k[e] < lo) continue;
+          const K k = F::to_key(r[e]);
+          if (k < lo) continue;
           const int at = atomicAdd(&S.listed, 1);
-          if (at < C::LIST) { S.list_key[at] = k[e]; S.list_idx[at] = (uint32_t)(i + e); }
+          if (at < C::LIST) { S.list_key[at] = k; S.list_idx[at] = (uint32_t)(i + e); }
         }
       });
       __syncthreads();
@@ -607,7 +679,8 @@ template <class C, class F> __device__ Cut<typename F::key> cut_of(const Row<F>&
   if (p.top_p < 1.0) {
     // entries below exp(-56) < 2^-80 of the best one weigh nothing in the bins
     const K floor = key_below<F>(R.best - 56.0 * R.t);
-    cut = tighter(cut, select<true, C, F>(R, S, (u64)floor > kmin ? floor : (K)kmin, (K)kmax, cut, 0, p.top_p));
+    const K least = cut.key > (K)kmin ? cut.key : (K)kmin;
+    cut = tighter(cut, select<true, C, F>(R, S, floor > least ? floor : least, (K)kmax, cut, 0, p.top_p));
   }
   return cut;
 }
@@ -620,7 +693,9 @@ template <class C, class F> __global__ __launch_bounds__(C::NT) __attribute__((a
   const int64_t row = blockIdx.x;
   const Settings p = settings_of(A, row);
   Row<F> R = row_of<F>(A, row, p.t);
-  const u64 low = pass_best<C::NT, F>(R, 0, R.cells, S.best, p.plain ? S.cells : nullptr);
+  const bool lowest = wants_lowest(p, R.cells);
+  const typename F::wide low = p.plain ? pass_best<C::NT, true, F>(R, 0, R.cells, S.best, S.cells, false)
+                                        : pass_best<C::NT, false, F>(R, 0, R.cells, S.best, nullptr, lowest);
   __syncthreads();
   u64 top = 0;
   for (int c = threadIdx.x; c < R.cells; c += C::NT) top = S.best[c] > top ? S.best[c] : top;
@@ -629,7 +704,7 @@ template <class C, class F> __global__ __launch_bounds__(C::NT) __attribute__((a
   if (kmax != 0) {
     R.best = F::of_key((K)kmax);
     if (!p.plain) {
-      const u64 kmin = ~block_max<C>(S.red, ~low);
+      const u64 kmin = lowest ? ~block_max<C>(S.red, ~(u64)F::key_of_wide(low)) : (u64)neg_key<F>() + 1;
       int listed;
       cut = cut_of<C, F>(R, S, p, kmin, kmax, listed);
       if (listed && draws_here) { draw_list<C, F>(A, R, S, row, listed); return; }
@@ -659,8 +734,11 @@ template <class F> __global__ __launch_bounds__(256) void k_best(DrawArgs A, int
   const Settings p = settings_of(A, row);
   const Row<F> R = row_of<F>(A, row, p.t);
   const int c0 = (int)((int64_t)R.cells * g / groups), c1 = (int)((int64_t)R.cells * (g + 1) / groups);
-  const u64 low = pass_best<256, F>(R, c0, c1, A.keys + row * A.max_cells, p.plain ? A.sums + row * A.max_cells : nullptr);
-  const u64 kmin = ~block_max<Short>(red, ~low);
+  const bool lowest = wants_lowest(p, R.cells);
+  u64* keys = A.keys + row * A.max_cells;
+  const typename F::wide low = p.plain ? pass_best<256, true, F>(R, c0, c1, keys, A.sums + row * A.max_cells, false)
+                                        : pass_best<256, false, F>(R, c0, c1, keys, nullptr, lowest);
+  const u64 kmin = lowest ? ~block_max<Short>(red, ~(u64)F::key_of_wide(low)) : (u64)neg_key<F>() + 1;
   if (threadIdx.x == 0) {
     A.lows[row * groups + g] = kmin;
     if (g == 0) { A.state[row * STATE] = (u64)neg_key<F>(); A.state[row * STATE + 1] = (u64)-1; }
