@@ -65,6 +65,8 @@ __device__ __forceinline__ double of_key(u64 k) { return __longlong_as_double((l
 struct Param { double v; const double* p; };                    // one number for every row, or one per row
 struct ParamI { int64_t v; const int64_t* p; };
 struct CutState { double value; int64_t idx; };
+constexpr int TABLE_BINS = 4096, TABLE_LIST = 1024;             // (those of the build All below)
+struct Table { u64 hi[TABLE_BINS], lo[TABLE_BINS]; double value[TABLE_LIST]; uint32_t count[TABLE_BINS], idx[TABLE_LIST]; int listed, pad; };
 struct DrawArgs {
   const void* logits; int64_t row_stride, col_stride, cols;
   const int64_t* lengths;                                       // entries of each row, or null: cols
@@ -72,7 +74,7 @@ struct DrawArgs {
   Param temperature, top_p, min_p; ParamI top_k;
   int64_t* index; double* logp;
   int mult, max_cells;                                          // loads per lane and cell over U, cells of a full row
-  double *best, *sums, *lows; CutState* cut;                    // rows whose passes are launches of their own: [row][max_cells] twice, [row][groups], [row]
+  double *best, *sums, *lows; CutState* cut; Table* tables;     // rows whose passes are launches of their own: [row][max_cells] twice, [row][groups], [row], [row][2]
 };
 
 // kept: values above the cut's, and equal ones up to its index
@@ -159,10 +161,12 @@ template <class F> struct Row {
 };
 
 // Builds of a row's code: 8 wavefronts for a row, 4 where there are rows enough to fill the chip with such workgroups (their phases
-// overlap better), and 4 with small tables for short rows
+// overlap better), 4 or one (no barriers) with small tables for short rows; All: the launches that share a long row's cut
 struct Long { static constexpr int NT = 512, BITS = 11, CELLS = MAX_CELLS, LIST = 512; };
 struct Many { static constexpr int NT = 256, BITS = 10, CELLS = MAX_CELLS, LIST = 256; };
 struct Short { static constexpr int NT = 256, BITS = 9, CELLS = 64, LIST = 256; };
+struct Tiny { static constexpr int NT = 64, BITS = 8, CELLS = 8, LIST = 64; };
+struct All { static constexpr int NT = 1024, BITS = 12, CELLS = MAX_CELLS, LIST = 1024; };
 
 template <class C> struct Shared {
   static constexpr int BINS = 1 << C::BITS, NW = C::NT / 64;
@@ -291,21 +295,26 @@ template <class C> __device__ __forceinline__ void add_weight(Shared<C>& S, int 
   if (lo) atomicAdd(&S.bins.lo[b], lo);
 }
 
+// SEEDED: the first bins, and the list of their bin's entries if it is short enough, have been made by other launches
 // The cut behind the first `want` entries of what `have` keeps (WEIGHTED: behind the shortest beginning with `share` of its weight);
 // lo <= every value that can matter.  The first bins divide the range of values evenly, the later ones (where a bin held too many
 // to sort) the range of the ordered bit patterns of the bin's values, at least a factor BINS / 2 narrower each time.
-template <bool WEIGHTED, class C, class F> __device__ Cut select(const Row<F>& R, Shared<C>& S, double lo, Cut have, u64 want, double share) {
+struct Even {                                                   // the first bins: the range of values in equal parts
+  double best, scale; bool good; int bins;
+  __device__ __forceinline__ Even(double best_, double lo, int bins_) : best(best_), scale(bins_ / (best_ - lo)), bins(bins_) { good = best - lo > 0.0 && best - lo < 1e300 && scale < 1e300; }
+  __device__ __forceinline__ int bin(double l) const { const int b = (int)((best - l) * scale); return b < bins ? b : bins - 1; }
+};
+template <bool WEIGHTED, bool SEEDED, class C, class F> __device__ Cut select(const Row<F>& R, Shared<C>& S, double lo, Cut have, u64 want, double share) {
   typedef typename F::raw raw;
   typedef typename F::wide wide;
   constexpr int VEC = Row<F>::VEC, U = F::U, UNIT = Row<F>::UNIT, BINS = Shared<C>::BINS;
   u64 bn = 0, bhi = 0, blo = 0;
   double target = -1.0;
   bool first = true;
-  const double best = R.best, scale = BINS / (best - lo);
-  bool even = best - lo > 0.0 && best - lo < 1e300 && scale < 1e300;
   lo = lo > have.value ? lo : have.value;
-  u64 khi = key_of(best), klo = key_of(lo);                     // the later bins' range
-  auto even_bin = [&](double l) { const int b = (int)((best - l) * scale); return b < BINS ? b : BINS - 1; };
+  const Even parts(R.best, lo, BINS);
+  bool even = parts.good;
+  u64 khi = key_of(R.best), klo = key_of(lo);                   // the later bins' range
   for (;;) {
     const int shift = shift_of<C>(khi - klo);
     wide quick; bound_below(lo, quick);
@@ -321,18 +330,21 @@ template <bool WEIGHTED, class C, class F> __device__ Cut select(const Row<F>& R
               const double l = (double)v;
               const int64_t i = i0 + q * UNIT + e;
               if (l >= lo && have.keeps(l, i)) {
-                if (even) f(l, i, even_bin(l));
+                if (even) f(l, i, parts.bin(l));
                 else { const u64 k = key_of(l); if (k <= khi) f(l, i, (int)((khi - k) >> shift)); }
               }
             }
           }
       });
     };
-    clear_bins<WEIGHTED>(S);
-    entries([&](double l, int64_t, int b) {
-      atomicAdd(&S.bins.count[b], 1u);
-      if (WEIGHTED) { add_weight(S, b, R.weight(l)); __builtin_amdgcn_sched_barrier(0); }
-    });
+    const bool seeded = SEEDED && first && even;
+    if (!seeded) {
+      clear_bins<WEIGHTED>(S);
+      entries([&](double l, int64_t, int b) {
+        atomicAdd(&S.bins.count[b], 1u);
+        if (WEIGHTED) { add_weight(S, b, R.weight(l)); __builtin_amdgcn_sched_barrier(0); }
+      });
+    }
     find_bin<WEIGHTED>(S, bn, bhi, blo, want, share, target);
     if (!WEIGHTED && first && S.found[6] <= want) return Cut{lo, EVERY};          // (all of them)
     first = false;
@@ -341,11 +353,12 @@ template <bool WEIGHTED, class C, class F> __device__ Cut select(const Row<F>& R
     bn = S.found[1]; bhi = S.found[3]; blo = S.found[4]; target = __longlong_as_double((long long)S.found[5]);
     if (in_bin <= (u64)C::LIST) {
       // few enough to sort: the bin's entries in the cut's order, then the first that reaches the goal
-      entries([&](double l, int64_t i, int b) {
-        if (b != bin) return;
-        const int at = atomicAdd(&S.listed, 1);
-        S.list_value[at] = l; S.list_idx[at] = (uint32_t)i;
-      });
+      if (!seeded)
+        entries([&](double l, int64_t i, int b) {
+          if (b != bin) return;
+          const int at = atomicAdd(&S.listed, 1);
+          S.list_value[at] = l; S.list_idx[at] = (uint32_t)i;
+        });
       const int count = (int)in_bin, t = threadIdx.x;
       sort_list(S, count);
       int at = (int)(want - bn) - 1;
@@ -616,6 +629,30 @@ template <class C, class F> __device__ __forceinline__ void draw_list(const Draw
     if (A.logp) A.logp[row * A.draws + s] = R.z(S.list_value[j]) - log_z;
   }
 }
+// A lower bound of the top_k-th value: the top_k-th highest of the cells' best values, from bins over them (S.best); `lowest` if there
+// are no more cells than that (bounded: false).  Only cells that reach it are looked at again
+template <class C, class F> __device__ __forceinline__ double bound_of_top_k(const Row<F>& R, Shared<C>& S, int64_t top_k, double lowest, bool& bounded) {
+  bounded = false;
+  clear_bins<false>(S);
+  if (top_k >= R.cells) return lowest;
+  double least = INF;
+  for (int c = threadIdx.x; c < R.cells; c += C::NT) { const double v = S.best[c]; least = v > -INF && v < least ? v : least; }
+  const u64 top = key_of(R.best), low = key_of(block_min<C::NT>(S.red, least));
+  const int shift = shift_of<C>(top - low);
+  for (int c = threadIdx.x; c < R.cells; c += C::NT) if (S.best[c] > -INF) atomicAdd(&S.bins.count[(top - key_of(S.best[c])) >> shift], 1u);
+  find_bin<false>(S, 0, 0, 0, (u64)top_k, 0.0, 0.0);
+  if (S.found[6] < (u64)top_k) return lowest;
+  const u64 drop = ((S.found[0] + 1) << shift) - 1;             // (to the lowest pattern of the bin)
+  bounded = true;
+  return of_key(drop < top - low ? top - drop : low);
+}
+// ... of what top_p keeps: entries below exp(-56) < 2^-80 of the best one weigh nothing in the bins
+template <class F> __device__ __forceinline__ double bound_of_top_p(const Row<F>& R, double lowest, const Cut& cut) {
+  double lo = R.best < INF ? R.best - 56.0 * R.t : INF;
+  lo = lo > lowest ? lo : lowest;
+  return lo > cut.value ? lo : cut.value;
+}
+__device__ __forceinline__ double finite_lowest(double v) { return v > -1.7976931348623157e308 ? v : -1.7976931348623157e308; }
 // The cut of a row whose cells' highest values are in S.best; R.best is set; `lowest` of the row where wants_lowest asked for it, else
 // -inf.  listed > 0: the list holds exactly the kept entries
 template <class C, class F> __device__ Cut cut_of(const Row<F>& R, Shared<C>& S, const Settings& p, double lowest, int& listed) {
@@ -624,25 +661,11 @@ template <class C, class F> __device__ Cut cut_of(const Row<F>& R, Shared<C>& S,
   constexpr int VEC = Row<F>::VEC, U = F::U;
   Cut cut = everything(R.best);
   listed = 0;
-  lowest = lowest > -1.7976931348623157e308 ? lowest : -1.7976931348623157e308;
+  lowest = finite_lowest(lowest);
   if (p.top_k > 0) {
-    // the top_k-th highest of the cells' best values is a lower bound of the cut: only cells that reach it are looked at again
-    double lo = lowest;
-    bool bounded = false;
-    clear_bins<false>(S);
-    if (p.top_k < R.cells) {
-      double least = INF;
-      for (int c = threadIdx.x; c < R.cells; c += C::NT) { const double v = S.best[c]; least = v > -INF && v < least ? v : least; }
-      const u64 top = key_of(R.best), low = key_of(block_min<C::NT>(S.red, least));
-      const int shift = shift_of<C>(top - low);
-      for (int c = threadIdx.x; c < R.cells; c += C::NT) if (S.best[c] > -INF) atomicAdd(&S.bins.count[(top - key_of(S.best[c])) >> shift], 1u);
-      find_bin<false>(S, 0, 0, 0, (u64)p.top_k, 0.0, 0.0);
-      if (S.found[6] >= (u64)p.top_k) {
-        const u64 drop = ((S.found[0] + 1) << shift) - 1;       // (to the lowest pattern of the bin)
-        lo = of_key(drop < top - low ? top - drop : low);
-        bounded = true;
-      }
-    }
+    bool bounded;
+    const double lo = bound_of_top_k<C, F>(R, S, p.top_k, lowest, bounded);
+    __syncthreads();
     if (p.top_k <= C::LIST && (bounded || R.n <= C::LIST)) {
       // few: all entries that reach it, if they fit the list -- everything else happens there
       wide quick; bound_below(lo, quick);
@@ -665,14 +688,9 @@ template <class C, class F> __device__ Cut cut_of(const Row<F>& R, Shared<C>& S,
         return Cut{S.list_value[listed - 1], (int64_t)S.list_idx[listed - 1]};
       }
     }
-    cut = tighter(cut, select<false, C, F>(R, S, lo, cut, (u64)p.top_k, 0.0));
+    cut = tighter(cut, select<false, false, C, F>(R, S, lo, cut, (u64)p.top_k, 0.0));
   }
-  if (p.top_p < 1.0) {
-    // entries below exp(-56) < 2^-80 of the best one weigh nothing in the bins
-    double lo = R.best < INF ? R.best - 56.0 * R.t : INF;
-    lo = lo > lowest ? lo : lowest;
-    cut = tighter(cut, select<true, C, F>(R, S, lo > cut.value ? lo : cut.value, cut, 0, p.top_p));
-  }
+  if (p.top_p < 1.0) cut = tighter(cut, select<true, false, C, F>(R, S, bound_of_top_p(R, lowest, cut), cut, 0, p.top_p));
   return cut;
 }
 
@@ -714,8 +732,9 @@ template <class C, class F> __global__ __launch_bounds__(C::NT) __attribute__((a
 }
 
 // The same over several launches, for a few long rows whose cells are dealt to `groups` workgroups each.  First: the cells' highest
-// values, the lowest value of each group, and -- nothing truncated -- the cells' weights
-template <class F> __global__ __launch_bounds__(256) void k_best(DrawArgs A, int groups) {
+// values, the lowest value of each group, and -- nothing truncated -- the cells' weights.  The bins and lists of the launches
+// behind it start empty
+template <class F> __global__ __launch_bounds__(256) void k_best(DrawArgs A, int groups, int stages) {
   __shared__ double red[4];
   const int64_t row = blockIdx.x / groups;
   const int g = blockIdx.x % groups;
@@ -728,21 +747,114 @@ template <class F> __global__ __launch_bounds__(256) void k_best(DrawArgs A, int
                              : pass_best<256, false, F>(R, c0, c1, best, nullptr, lowest);
   const double least = lowest ? block_min<256>(red, low) : -INF;
   if (threadIdx.x == 0) A.lows[row * groups + g] = least;
+  for (int k = 0; k < stages; ++k) {
+    Table& T = A.tables[row * 2 + k];
+    for (int b = g * 256 + threadIdx.x; b < TABLE_BINS; b += groups * 256) { T.count[b] = 0; T.hi[b] = 0; T.lo[b] = 0; }
+    if (g == 0 && threadIdx.x == 0) { T.listed = 0; if (k == 0) { const Cut c = Cut{-INF, -1}; A.cut[row] = CutState{c.value, c.idx}; } }
+  }
 }
-// ... the cut
-template <class F> __global__ __launch_bounds__(Long::NT) __attribute__((amdgpu_waves_per_eu(4))) void k_cut(DrawArgs A, int groups) {
-  __shared__ Shared<Long> S;
-  const int64_t row = blockIdx.x;
-  const Settings p = settings_of(A, row);
-  Row<F> R = row_of<F>(A, row, p.t);
+// What the launches of a stage (0: top_k, 1: top_p) start from; false: the row has no such truncation
+template <class F> __device__ __forceinline__ bool start_stage(const DrawArgs& A, int64_t row, int groups, int stage, Shared<All>& S, Settings& p, Row<F>& R, Cut& have, double& lo) {
+  p = settings_of(A, row);
+  if (stage == 0 ? p.top_k == 0 : p.top_p == 1.0) return false;
+  R = row_of<F>(A, row, p.t);
   double top = -INF, low = INF;
-  for (int c = threadIdx.x; c < R.cells; c += Long::NT) { const double v = A.best[row * A.max_cells + c]; S.best[c] = v; top = v > top ? v : top; }
-  for (int g = threadIdx.x; g < groups; g += Long::NT) { const double v = A.lows[row * groups + g]; low = v < low ? v : low; }
-  R.best = block_max<Long::NT>(S.red, top);
-  low = block_min<Long::NT>(S.red, low);
-  Cut cut = everything(R.best);
-  int listed;
-  if (R.best > -INF && !p.plain) cut = cut_of<Long, F>(R, S, p, low, listed);
+  for (int c = threadIdx.x; c < R.cells; c += All::NT) { const double v = A.best[row * A.max_cells + c]; S.best[c] = v; top = v > top ? v : top; }
+  for (int g = threadIdx.x; g < groups; g += All::NT) { const double v = A.lows[row * groups + g]; low = v < low ? v : low; }
+  R.best = block_max<All::NT>(S.red, top);
+  low = finite_lowest(block_min<All::NT>(S.red, low));
+  if (!(R.best > -INF)) return false;
+  have = everything(R.best);
+  if (stage == 1) have = tighter(have, Cut{A.cut[row].value, A.cut[row].idx});
+  bool bounded;
+  lo = stage == 0 ? bound_of_top_k<All, F>(R, S, p.top_k, low, bounded) : bound_of_top_p(R, low, have);
+  lo = lo > have.value ? lo : have.value;
+  return true;
+}
+// ... the first bins of a stage
+template <bool WEIGHTED, class F> __global__ __launch_bounds__(All::NT) void k_bins(DrawArgs A, int groups, int shares) {
+  typedef typename F::raw raw;
+  typedef typename F::wide wide;
+  constexpr int VEC = Row<F>::VEC, U = F::U;
+  __shared__ Shared<All> S;
+  const int64_t row = blockIdx.x / shares;
+  const int g = blockIdx.x % shares;
+  Settings p; Row<F> R; Cut have; double lo;
+  if (!start_stage<F>(A, row, groups, WEIGHTED ? 1 : 0, S, p, R, have, lo)) return;
+  const Even parts(R.best, lo, Shared<All>::BINS);
+  if (!parts.good) return;
+  clear_bins<WEIGHTED>(S);
+  wide quick; bound_below(lo, quick);
+  const int c0 = (int)((int64_t)R.cells * g / shares), c1 = (int)((int64_t)R.cells * (g + 1) / shares);
+  for_cells<true, All::NT>(R, S.best, c0, c1, lo, [&](int, const raw (&r)[U][VEC], int64_t i0, bool) {
+#pragma unroll
+    for (int q = 0; q < U; ++q)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const wide v = F::widen(r[q][e]);
+        const double l = (double)v;
+        if (v < quick || !(l >= lo) || !have.keeps(l, i0 + q * Row<F>::UNIT + e)) continue;
+        const int b = parts.bin(l);
+        atomicAdd(&S.bins.count[b], 1u);
+        if (WEIGHTED) { add_weight(S, b, R.weight(l)); __builtin_amdgcn_sched_barrier(0); }
+      }
+  });
+  __syncthreads();
+  Table& T = A.tables[row * 2 + (WEIGHTED ? 1 : 0)];
+  for (int b = threadIdx.x; b < TABLE_BINS; b += All::NT) {     // (sums of integers: the order of the workgroups does not matter)
+    if (!S.bins.count[b]) continue;
+    atomicAdd(&T.count[b], S.bins.count[b]);
+    if (WEIGHTED) { if (S.bins.hi[b]) atomicAdd(&T.hi[b], S.bins.hi[b]); if (S.bins.lo[b]) atomicAdd(&T.lo[b], S.bins.lo[b]); }
+  }
+}
+template <bool WEIGHTED> __device__ __forceinline__ void load_bins(Shared<All>& S, const Table& T) {
+  __syncthreads();
+  for (int b = threadIdx.x; b < TABLE_BINS; b += All::NT) { S.bins.count[b] = T.count[b]; if (WEIGHTED) { S.bins.hi[b] = T.hi[b]; S.bins.lo[b] = T.lo[b]; } }
+  if (threadIdx.x == 0) S.listed = 0;
+}
+// ... the entries of the bin that holds the cut
+template <bool WEIGHTED, class F> __global__ __launch_bounds__(All::NT) void k_list(DrawArgs A, int groups, int shares) {
+  typedef typename F::raw raw;
+  typedef typename F::wide wide;
+  constexpr int VEC = Row<F>::VEC, U = F::U;
+  __shared__ Shared<All> S;
+  const int64_t row = blockIdx.x / shares;
+  const int g = blockIdx.x % shares;
+  Settings p; Row<F> R; Cut have; double lo;
+  if (!start_stage<F>(A, row, groups, WEIGHTED ? 1 : 0, S, p, R, have, lo)) return;
+  const Even parts(R.best, lo, Shared<All>::BINS);
+  if (!parts.good) return;
+  Table& T = A.tables[row * 2 + (WEIGHTED ? 1 : 0)];
+  load_bins<WEIGHTED>(S, T);
+  find_bin<WEIGHTED>(S, 0, 0, 0, (u64)p.top_k, p.top_p, -1.0);
+  if (S.found[2] > (u64)All::LIST) return;
+  const int bin = (int)S.found[0];
+  wide quick; bound_below(lo, quick);
+  const int c0 = (int)((int64_t)R.cells * g / shares), c1 = (int)((int64_t)R.cells * (g + 1) / shares);
+  for_cells<true, All::NT, false>(R, S.best, c0, c1, lo, [&](int, const raw (&r)[U][VEC], int64_t i0, bool) {
+#pragma unroll
+    for (int q = 0; q < U; ++q)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const wide v = F::widen(r[q][e]);
+        const double l = (double)v;
+        const int64_t i = i0 + q * Row<F>::UNIT + e;
+        if (v < quick || !(l >= lo) || parts.bin(l) != bin || !have.keeps(l, i)) continue;
+        const int at = atomicAdd(&T.listed, 1);
+        T.value[at] = l; T.idx[at] = (uint32_t)i;
+      }
+  });
+}
+// ... and the cut of the stage
+template <bool WEIGHTED, class F> __global__ __launch_bounds__(All::NT) void k_cut(DrawArgs A, int groups) {
+  __shared__ Shared<All> S;
+  const int64_t row = blockIdx.x;
+  Settings p; Row<F> R; Cut have; double lo;
+  if (!start_stage<F>(A, row, groups, WEIGHTED ? 1 : 0, S, p, R, have, lo)) return;
+  const Table& T = A.tables[row * 2 + (WEIGHTED ? 1 : 0)];
+  load_bins<WEIGHTED>(S, T);
+  for (int t = threadIdx.x; t < T.listed; t += All::NT) { S.list_value[t] = T.value[t]; S.list_idx[t] = T.idx[t]; }
+  const Cut cut = tighter(have, select<WEIGHTED, true, All, F>(R, S, lo, have, (u64)p.top_k, p.top_p));
   if (threadIdx.x == 0) A.cut[row] = CutState{cut.value, cut.idx};
 }
 template <int THREADS> __device__ __forceinline__ double best_of_row(const DrawArgs& A, int64_t row, int cells, double* red) {
@@ -759,7 +871,7 @@ template <class F> __global__ __launch_bounds__(256) void k_weights(DrawArgs A, 
   Row<F> R = row_of<F>(A, row, p.t);
   R.best = best_of_row<256>(A, row, R.cells, red);
   if (p.plain || !(R.best > -INF)) return;
-  const Cut cut = cuts ? Cut{A.cut[row].value, A.cut[row].idx} : everything(R.best);
+  const Cut cut = cuts ? tighter(everything(R.best), Cut{A.cut[row].value, A.cut[row].idx}) : everything(R.best);
   const int c0 = (int)((int64_t)R.cells * g / groups), c1 = (int)((int64_t)R.cells * (g + 1) / groups);
   pass_weights<256, F>(R, A.best + row * A.max_cells, c0, c1, cut, p.min_p, A.sums + row * A.max_cells);
 }
@@ -772,7 +884,7 @@ template <class F> __global__ __launch_bounds__(Long::NT) void k_draws(DrawArgs 
   Row<F> R = row_of<F>(A, row, p.t);
   R.best = best_of_row<Long::NT>(A, row, R.cells, S.red);
   if (!(R.best > -INF)) { draw_nothing(A, row, s0, s1, Long::NT); return; }
-  const Cut cut = cuts ? Cut{A.cut[row].value, A.cut[row].idx} : everything(R.best);
+  const Cut cut = cuts ? tighter(everything(R.best), Cut{A.cut[row].value, A.cut[row].idx}) : everything(R.best);
   for (int c = threadIdx.x; c < R.cells; c += Long::NT) {
     const double w = A.sums[row * A.max_cells + c];
     S.cells[c] = p.plain ? w * cell_factor(R, A.best[row * A.max_cells + c]) : w;
@@ -783,32 +895,51 @@ template <class F> __global__ __launch_bounds__(Long::NT) void k_draws(DrawArgs 
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------------
 // How a call runs: cells of a row, workgroups per row (0: one workgroup does a whole row), which build of it, draws apart from the rest
-struct Plan { int mult, max_cells, groups, build; bool draws_here; };
+struct Plan { int mult, max_cells, groups, shares, build; bool draws_here; };
+static_assert(Shared<All>::BINS == TABLE_BINS && All::LIST == TABLE_LIST, "tables in memory");
 Plan plan_of(int type, int64_t rows, int64_t cols, int64_t draws) {
   Plan p;
   const int64_t group = type == 0 ? 2 * 128 : type == 1 ? 2 * 256 : 512;
   p.mult = (int)((cols + group * MAX_CELLS - 1) / (group * MAX_CELLS));
   p.max_cells = (int)((cols + group * p.mult - 1) / (group * p.mult));
-  p.build = p.max_cells <= (rows >= 512 ? 64 : 16) ? 2 : rows > 512 ? 1 : 0;
+  p.build = p.max_cells <= Tiny::CELLS && rows >= 1024 ? 3 : p.max_cells <= (rows >= 512 ? 64 : 16) ? 2 : rows > 512 ? 1 : 0;
   p.groups = (p.build == 0 && p.max_cells >= 32 && rows <= 64) ? (int)std::min<int64_t>(p.max_cells / 8, std::max<int64_t>(1, 512 / rows)) : 0;
+  p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(p.max_cells / 16, 256 / rows));      // (of the launches with 16 wavefronts and tables to merge)
   p.draws_here = p.groups == 0 && draws <= 64;
   return p;
 }
-int64_t scratch_of(const Plan& p, int64_t rows) { return p.draws_here ? 0 : rows * (2 * (int64_t)p.max_cells + p.groups + 2); }
+int64_t scratch_of(const Plan& p, int64_t rows) {
+  if (p.draws_here) return 0;
+  return rows * (2 * (int64_t)p.max_cells + p.groups + 2 + (p.groups ? 2 * (int64_t)(sizeof(Table) / sizeof(double)) : 0));
+}
+static_assert(sizeof(Table) % sizeof(double) == 0, "scratch in doubles");
 
 template <class F> void launch(DrawArgs& A, const Plan& p, int64_t rows, hipStream_t st) {
   int cuts = 1;
   if (p.groups == 0) {
     const dim3 grid((unsigned)rows);
-    if (p.build == 2) hipLaunchKernelGGL((k_row<Short, F>), grid, dim3(Short::NT), 0, st, A, p.draws_here ? 1 : 0);
+    if (p.build == 3) hipLaunchKernelGGL((k_row<Tiny, F>), grid, dim3(Tiny::NT), 0, st, A, p.draws_here ? 1 : 0);
+    else if (p.build == 2) hipLaunchKernelGGL((k_row<Short, F>), grid, dim3(Short::NT), 0, st, A, p.draws_here ? 1 : 0);
     else if (p.build == 1) hipLaunchKernelGGL((k_row<Many, F>), grid, dim3(Many::NT), 0, st, A, p.draws_here ? 1 : 0);
     else hipLaunchKernelGGL((k_row<Long, F>), grid, dim3(Long::NT), 0, st, A, p.draws_here ? 1 : 0);
     if (p.draws_here) return;
   } else {
     const dim3 grid((unsigned)(rows * p.groups));
-    hipLaunchKernelGGL(k_best<F>, grid, dim3(256), 0, st, A, p.groups);
-    cuts = A.temperature.p || A.temperature.v == 0.0 || A.top_k.p || A.top_k.v > 0 || A.top_p.p || A.top_p.v < 1.0;
-    if (cuts) hipLaunchKernelGGL(k_cut<F>, dim3((unsigned)rows), dim3(Long::NT), 0, st, A, p.groups);
+    const bool ks = A.temperature.p || A.temperature.v == 0.0 || A.top_k.p || A.top_k.v > 0 || A.top_p.p || A.top_p.v == 0.0;
+    const bool ps = A.top_p.p || (A.top_p.v < 1.0 && A.top_p.v > 0.0);
+    cuts = ks || ps;
+    hipLaunchKernelGGL(k_best<F>, grid, dim3(256), 0, st, A, p.groups, ks || ps ? 2 : 0);
+    const dim3 shared((unsigned)(rows * p.shares)), one((unsigned)rows), all(All::NT);
+    if (ks) {
+      hipLaunchKernelGGL((k_bins<false, F>), shared, all, 0, st, A, p.groups, p.shares);
+      hipLaunchKernelGGL((k_list<false, F>), shared, all, 0, st, A, p.groups, p.shares);
+      hipLaunchKernelGGL((k_cut<false, F>), one, all, 0, st, A, p.groups);
+    }
+    if (ps) {
+      hipLaunchKernelGGL((k_bins<true, F>), shared, all, 0, st, A, p.groups, p.shares);
+      hipLaunchKernelGGL((k_list<true, F>), shared, all, 0, st, A, p.groups, p.shares);
+      hipLaunchKernelGGL((k_cut<true, F>), one, all, 0, st, A, p.groups);
+    }
     if (cuts || A.min_p.p || A.min_p.v > 0.0) hipLaunchKernelGGL(k_weights<F>, grid, dim3(256), 0, st, A, p.groups, cuts);
   }
   // a wavefront makes one draw at a time: two each, more where that fills the chip anyway
@@ -847,12 +978,13 @@ extern "C" int pgm_draw_indices(const void* logits, int type, int64_t rows, int6
   if (need > 0 && !scratch) return -20;
   if (need > scratch_doubles) return -21;
   DrawArgs A{logits, row_stride, col_stride, cols, lengths, u, draws, {temperature, temperature_row}, {top_p, top_p_row}, {min_p, min_p_row},
-             {top_k, top_k_row}, index, logp, p.mult, p.max_cells, nullptr, nullptr, nullptr, nullptr};
+             {top_k, top_k_row}, index, logp, p.mult, p.max_cells, nullptr, nullptr, nullptr, nullptr, nullptr};
   if (need > 0) {
     A.best = scratch;
     A.sums = scratch + rows * p.max_cells;
     A.lows = scratch + 2 * rows * p.max_cells;
     A.cut = reinterpret_cast<CutState*>(A.lows + rows * p.groups);
+    A.tables = reinterpret_cast<Table*>(A.cut + rows);
   }
   hipStream_t st = (hipStream_t)stream;
   if (type == 0) launch<F64>(A, p, rows, st);

@@ -226,3 +226,33 @@ def test_more_than_32_bits_of_offset(dev):
     u = torch.full((1100, 1), 0.75, dtype=torch.float64, device=dev)
     idx = draw_indices(rows, u, min_p=0.5)
     assert int(idx[1099]) == V - 2 and int(idx[0]) == 3 * V // 4
+
+
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=20), dict(top_k=3000), dict(top_p=0.9), dict(top_k=900, top_p=0.6, min_p=0.01), dict(min_p=0.05)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B, V, S", [(2, 60_000, 3), (2, 60_000, 100), (64, 20_001, 1), (70, 20_001, 70), (600, 20_001, 2), (600, 3000, 90), (1100, 1500, 3)])
+def test_every_division_of_the_work(dev, B, V, S, dtype, settings):
+    """Rows shared by workgroups, one workgroup per row in its builds, draws apart from the rest: a few rows of each against numpy."""
+    l = _rows(B, V, dtype, B + V)
+    u = torch.as_tensor(np.random.default_rng(B).random((B, S)))
+    lengths = [V] * B
+    lengths[1] = V - 777 if V > 1000 else V
+    idx, logp = draw_indices(l.to(dev), u.to(dev), lengths=torch.as_tensor(lengths), return_logprob=True, **settings)
+    assert int(idx.min()) >= 0
+    some = sorted({0, 1, B // 2, B - 1})
+    _check(l[some], u[some], (idx[some], logp[some]), lengths=[lengths[b] for b in some], **settings)
+
+
+@pytest.mark.parametrize("V", [30_000, 300_000])
+def test_long_rows_with_settings_per_row(dev, V):
+    B = 5
+    l = _rows(B, V, torch.float64, 4)
+    l[3] = l[3].round()                                          # (many ties)
+    l[4, :] = 0.0
+    u = torch.as_tensor(np.random.default_rng(9).random((B, 20)))
+    per = dict(temperature=np.array([1.0, 0.0, 0.5, 2.0, 1.0]), top_k=np.array([0, 7, 0, V // 3, 0]), top_p=np.array([1.0, 0.5, 0.9, 0.4, 0.3]),
+               min_p=np.array([0.01, 0.0, 0.0, 0.0, 0.0]))
+    got = draw_indices(l.to(dev), u.to(dev), return_logprob=True, **{k: torch.as_tensor(v).to(dev) for k, v in per.items()})
+    _check(l, u, got, **per)
+    wide = l.to(dev).t().contiguous().t()                        # a column per frequency: strided rows
+    assert torch.equal(draw_indices(wide, u.to(dev), top_p=0.8), draw_indices(l.to(dev), u.to(dev), top_p=0.8))
