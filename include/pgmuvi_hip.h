@@ -223,6 +223,9 @@ int pgm_fit_create(pgm_fit** out, pgm_ws* ws, const double* x, const double* y, 
                    int dim_order, int linear_mean, const double* raw0, const int* ckind, const double* ca, const double* cb, int has_noise_param,
                    int optimizer, double lr, double beta1, double beta2, double eps, double weight_decay, int max_iter);
 int pgm_fit_set_priors(pgm_fit* fit, const int* kind, const double* loc, const double* scale);
+/* The step's gradient (with respect to the raw vector, priors included) is scaled to a norm of at most max_norm (>= 0, finite):
+ * times min(1, max_norm / (norm + 1e-6)), as pgm_grad_clip does.  Optional, before the first pgm_fit_run. */
+int pgm_fit_set_clip(pgm_fit* fit, double max_norm);
 int pgm_fit_run(pgm_fit* fit, int iters, void* stream);
 int pgm_fit_read(pgm_fit* fit, void* stream, int* iters_done, double* loss_hist, double* raw_hist, double* raw, int* info);
 int pgm_fit_destroy(pgm_fit* fit);

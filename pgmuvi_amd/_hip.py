@@ -57,6 +57,7 @@ SYMBOLS = {
     "pgm_fit_create": (c_int, [POINTER(c_void_p), c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
                                c_void_p, c_void_p, c_int, c_int, c_double, c_double, c_double, c_double, c_double, c_int]),
     "pgm_fit_set_priors": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),
+    "pgm_fit_set_clip": (c_int, [c_void_p, c_double]),
     "pgm_fit_run": (c_int, [c_void_p, c_int, c_void_p]),
     "pgm_fit_read": (c_int, [c_void_p, c_void_p, POINTER(c_int), c_void_p, c_void_p, c_void_p, POINTER(c_int)]),
     "pgm_fit_destroy": (c_int, [c_void_p]),
@@ -715,6 +716,11 @@ class NativeFit:
         with torch.cuda.device(self.dev):
             _check(load().pgm_fit_set_priors(self.handle, k.ctypes.data_as(c_void_p), l.ctypes.data_as(c_void_p),
                                              s.ctypes.data_as(c_void_p)), "pgm_fit_set_priors")
+
+    def set_clip(self, max_norm: float):
+        """Largest norm of the gradient a step takes (``pgm_fit_set_clip``); before the first run."""
+        with torch.cuda.device(self.dev):
+            _check(load().pgm_fit_set_clip(self.handle, float(max_norm)), "pgm_fit_set_clip")
 
     def run(self, iters: int):
         with torch.cuda.device(self.dev):

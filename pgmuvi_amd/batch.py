@@ -39,12 +39,16 @@ def balanced_assignment(costs: Sequence[float], world: int):
 
 
 def evaluate_batch(x, y, mean, noise, w, mu, v, noise_scalar=None, dim_order=0, need_grad=True, chunk: Optional[int] = None,
-                   _compute=None) -> Dict[str, torch.Tensor]:
+                   _compute=None, max_grad_norm: Optional[float] = None, clip=("g_w", "g_mu", "g_v")) -> Dict[str, torch.Tensor]:
     """MLL (+ gradients) of ``B`` equal-length light curves on the local device.
 
     x (B,N,d) y (B,N) mean (B,N) noise (B,N)|None w (B,Q) mu (B,Q,d) v (B,Q,d).  ``chunk``
-    bounds how many problems share the workspace at once (memory = chunk * 8 N^2 bytes).
+    bounds how many problems share the workspace at once (memory = chunk * 8 N^2 bytes).  ``max_grad_norm``: every light
+    curve's gradients named by ``clip`` are scaled to at most this norm, taken over them together
+    (:func:`pgmuvi_amd.gradients.clip_grads_`, one norm per light curve); ``"grad_norm"`` (B,) is what it was.
     """
+    if max_grad_norm is not None and not need_grad:
+        raise ValueError("evaluate_batch: max_grad_norm without need_grad")
     compute = _compute or _hip.mll_value_grad
     B = y.shape[0]
     chunk = B if chunk is None else max(1, min(chunk, B))
@@ -56,7 +60,11 @@ def evaluate_batch(x, y, mean, noise, w, mu, v, noise_scalar=None, dim_order=0, 
                     None if noise_scalar is None else noise_scalar[sl], w[sl], mu[sl], v[sl], dim_order, 0.0, need_grad)
         outs.append(o)
     keys = ["mll", "info"] + (["g_w", "g_mu", "g_v", "g_noise", "g_mean"] if need_grad else [])
-    return {k: torch.cat([o[k] for o in outs]) for k in keys}
+    out = {k: torch.cat([o[k] for o in outs]) for k in keys}
+    if max_grad_norm is not None:
+        from . import gradients
+        out["grad_norm"] = gradients.clip_grads_([out[k] for k in clip], max_grad_norm, members=True)
+    return out
 
 
 def pad_curves(curves: Sequence[Dict[str, torch.Tensor]], device=None) -> Tuple[Dict[str, torch.Tensor], List[int]]:

@@ -269,6 +269,7 @@ struct FitDev {
   const int* pkind;     // [P] 0 none, 1 Normal(loc, scale), 2 LogNormal(loc, scale)
   const double* ploc;   // [P]
   const double* pscale; // [P]
+  const double* clip;   // [1] largest norm of the gradient with respect to the raw vector a step takes, or -1: no limit
 };
 
 __device__ __forceinline__ double softplus_d(double x) { return x > 20.0 ? x : log1p(exp(x)); }
@@ -2662,13 +2663,14 @@ __global__ __launch_bounds__(256) void k_fit_pre(FitDev F) {
 // What one parameter's thread reads from memory for the step: loaded where the kernel starts (k_small: the loads complete behind
 // the whole evaluation instead of in front of the step).
 struct FitLoads {
-  double raw, ca, cb, ploc, pscale, m1, m2;
+  double raw, ca, cb, ploc, pscale, m1, m2, clip;
   int ckind, pkind, it;
 };
 __device__ __forceinline__ FitLoads fit_loads(const FitDev& F) {
   FitLoads L;
   const int t = threadIdx.x;
   L.it = F.it[0];
+  L.clip = F.clip[0];
   L.raw = L.ca = L.cb = L.ploc = L.pscale = L.m1 = L.m2 = 0.0; L.ckind = L.pkind = 0;
   if (t < F.P) {
     L.raw = F.raw[t]; L.ckind = F.ckind[t]; L.ca = F.ca[t]; L.cb = F.cb[t];
@@ -2744,6 +2746,7 @@ __device__ __forceinline__ void fit_post_body(const FitDev& F, const FitLoads& L
   // log holds the NaN loss for the host to find at its next read
   const bool ok = isfinite(mll[0]);
   if (t < F.P && it < F.max_iter && !ok) F.raw_hist[(int64_t)it * F.P + t] = L.raw;
+  double g = 0.0;                                           // d(-mll)/d raw_p
   if (t < F.P && it < F.max_iter && ok) {
     const int p = t, o = F.nmean;
     double gth;                                             // d(-mll)/d theta_p
@@ -2758,7 +2761,21 @@ __device__ __forceinline__ void fit_post_body(const FitDev& F, const FitLoads& L
     if (L.ckind == 1) dth = sigmoid_d(r);
     else if (L.ckind == 2) dth = sigmoid_d(-r);
     else if (L.ckind == 3) { const double sg = sigmoid_d(r); dth = L.cb * sg * (1.0 - sg); }
-    const double g = gth * dth;
+    g = gth * dth;
+  }
+  if (L.clip >= 0.0 && t < 64) {
+    // the gradient's norm (P <= 52 entries: wavefront 0 holds them all), scaled by the largest entry so that no square overflows
+    double top = fabs(g);
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) { const double v = __shfl_xor(top, s); top = (v > top || v != v) ? v : top; }
+    const double q = top > 0.0 ? g / top : 0.0;
+    const double norm = top > 0.0 ? top * sqrt(wave_sum_dpp(q * q)) : top;
+    const double c = L.clip / (norm + 1e-6);
+    if (!(c >= 1.0)) g *= c;
+  }
+  if (t < F.P && it < F.max_iter && ok) {
+    const int p = t;
+    const double r = L.raw;
     double x = r;
     if (F.optimizer == 0) {
       x = r - F.lr * g;
@@ -2890,7 +2907,7 @@ __global__ __launch_bounds__(DIAG_THREADS) void k_small(PgmDev P, FitDev F) {
   double* misc = outs + 64;                         // [8] 0: log det, 1: status
   double* wpart = misc + 8;                         // [16][nslot]
   double* red = wpart + 16 * (3 * PGM_MAX_QD + 1);  // [256] (FIT)
-  double* sums = red + 256;                         // [8]   (FIT)
+  double* sums = red + 256;                         // [8]   (FIT) [7]: the gradient's limit
   double* fitl = sums + 8;                          // [10][64] (FIT) what the optimiser step reads from memory, parked here meanwhile
   const int cb = caller_slot(P, b), n = pts(P, b);
   const int nse = __builtin_amdgcn_readfirstlane((n + DB - 1) / DB);
@@ -2925,6 +2942,7 @@ __global__ __launch_bounds__(DIAG_THREADS) void k_small(PgmDev P, FitDev F) {
     if (t < 64) {
       fitl[0 * 64 + t] = L.raw; fitl[1 * 64 + t] = L.ca; fitl[2 * 64 + t] = L.cb; fitl[3 * 64 + t] = L.ploc; fitl[4 * 64 + t] = L.pscale;
       fitl[5 * 64 + t] = L.m1; fitl[6 * 64 + t] = L.m2; fitl[7 * 64 + t] = (double)L.ckind; fitl[8 * 64 + t] = (double)L.pkind; fitl[9 * 64 + t] = (double)L.it;
+      if (t == 0) sums[7] = L.clip;                             // (the sums take the first PGM_MAX_D + 2 places)
     }
     if (t < F.P) { const double th = fit_theta_of(L); thl[t] = th; F.theta[t] = th; if (F.has_noise && t == F.P - 1) F.noise_scalar[0] = th; }
     lds_barrier();
@@ -3318,6 +3336,7 @@ __global__ __launch_bounds__(DIAG_THREADS) void k_small(PgmDev P, FitDev F) {
     const int tl = t & 63;                                      // (P <= 51 parameters: wavefront 0 holds them; the others only need `it`)
     L.raw = fitl[0 * 64 + tl]; L.ca = fitl[1 * 64 + tl]; L.cb = fitl[2 * 64 + tl]; L.ploc = fitl[3 * 64 + tl]; L.pscale = fitl[4 * 64 + tl];
     L.m1 = fitl[5 * 64 + tl]; L.m2 = fitl[6 * 64 + tl]; L.ckind = (int)fitl[7 * 64 + tl]; L.pkind = (int)fitl[8 * 64 + tl]; L.it = (int)fitl[9 * 64 + tl];
+    L.clip = sums[7];
     fit_post_body<DIAG_THREADS>(F, L, outs, outs + 1, outs + 1 + Q, outs + 1 + Q + QD, gno, gme, red, sums);
   }
   SSTAMP();

@@ -200,19 +200,43 @@ class LombScargleMultiband:
         return f, self.power(f, method=method, sb_method=sb_method, normalization=normalization)
 
 
+def _shared_grid(t, y, nyquist_factor, samples_per_peak):
+    """``LombScargle.autofrequency`` of light curves (B, N) that share one sampling span."""
+    baseline = float(t.max()) - float(t.min())
+    df = 1.0 / baseline / samples_per_peak
+    f0 = 0.5 * df
+    nf = 1 + int(np.round((nyquist_factor * 0.5 * y.shape[-1] / baseline - f0) / df))
+    return f0 + df * torch.arange(nf, dtype=torch.float64, device=y.device)
+
+
+def draw_frequencies(t: torch.Tensor, y: torch.Tensor, dy: Optional[torch.Tensor], u: torch.Tensor, temperature=1.0, top_k=None,
+                     top_p=None, min_p=None, nyquist_factor=5, samples_per_peak=5):
+    """Frequencies drawn from the periodograms of light curves (B, N) that share one sampling span, one for each of the uniform
+    random numbers ``u`` (B, S): starts for several fits or chains that differ in proportion to what the data say, where
+    :func:`seed_frequencies` always returns the highest peaks.
+
+    The log odds of a grid frequency are ``-log FAP_single = -(n - 3) / 2 log(1 - P)`` (:meth:`LombScargle.false_alarm_probability`,
+    'single': the likelihood ratio of a sinusoid of that frequency, its amplitude and the noise level fitted).  ``top_p`` keeps the
+    smallest set of frequencies with that share of the posterior, ``min_p`` those within a likelihood ratio of the best,
+    ``top_k`` the k best, ``temperature`` > 1 flattens it (:func:`pgmuvi_amd.sampling.draw_indices`).  Returns (freqs (B, S),
+    their log-probabilities (B, S), grid), all on the device; NaN where a light curve has no finite periodogram."""
+    from .sampling import draw_indices
+    grid = _shared_grid(t, y, nyquist_factor, samples_per_peak)
+    P = periodogram_batched(t, y, dy, grid)
+    odds = torch.log1p(-P.clamp(max=1.0 - 2.0 ** -52)).mul_(-0.5 * (y.shape[-1] - 3))      # (a noiseless sinusoid's P rounds to one)
+    index, logp = draw_indices(odds, u, temperature, top_k, top_p, min_p, return_logprob=True)
+    freqs = torch.where(index >= 0, grid[index.clamp(min=0)], torch.full((), float("nan"), dtype=grid.dtype, device=grid.device))
+    return freqs, logp, grid
+
+
 def seed_frequencies(t: torch.Tensor, y: torch.Tensor, dy: Optional[torch.Tensor], num_peaks=1, nyquist_factor=5,
                      samples_per_peak=5):
     """Batched seeding for many light curves (B, N) that share one sampling span: the ``num_peaks`` highest
     periodogram peaks of each (peaks at least ``nyquist_factor`` grid points apart, like
     ``find_peaks(power, distance=Nyquist_factor)`` in ``fit_LS``).  Returns (freqs (B, num_peaks), powers, grid)."""
     from scipy.signal import find_peaks
-    B, n = y.shape
-    tmin, tmax = float(t.min()), float(t.max())
-    baseline = tmax - tmin
-    df = 1.0 / baseline / samples_per_peak
-    f0 = 0.5 * df
-    nf = 1 + int(np.round((nyquist_factor * 0.5 * n / baseline - f0) / df))
-    grid = f0 + df * torch.arange(nf, dtype=torch.float64, device=y.device)
+    B = y.shape[0]
+    grid = _shared_grid(t, y, nyquist_factor, samples_per_peak)
     P = periodogram_batched(t, y, dy, grid).cpu().numpy()
     g = grid.cpu().numpy()
     freqs = np.full((B, num_peaks), np.nan)

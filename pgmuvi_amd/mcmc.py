@@ -529,7 +529,7 @@ def effective_sample_size(x: np.ndarray) -> np.ndarray:
 
 
 def run_mcmc(x, y, noise=None, num_mixtures=4, sampler="NUTS", num_samples=500, warmup_steps=100, num_chains=1, seed=0,
-             initial_values: Optional[Dict[str, np.ndarray]] = None, priors=None, dim_order=0, group=None, compute=None,
+             initial_values=None, priors=None, dim_order=0, group=None, compute=None,
              group_by_chain=False, **sampler_kwargs):
     """The run ``Lightcurve.mcmc`` describes (``lightcurve.py:5882-6003``: sampler 'NUTS'|'HMC', ``num_samples=500``,
     ``warmup_steps=100``, ``num_chains``): posterior samples of the SM hyper-parameters under the default priors.
@@ -537,7 +537,10 @@ def run_mcmc(x, y, noise=None, num_mixtures=4, sampler="NUTS", num_samples=500, 
     ``y`` (N,) -> ``num_chains`` chains on that light curve; ``y`` (C,N) -> one chain per row (config 5: each chain its own
     light curve).  With ``torch.distributed`` initialised the chains are block-partitioned over the ranks
     (``batch.shard_bounds``), each rank advances its chains with batched evaluations on its own GPU, and one
-    ``all_gather`` of the draws closes the run (the only collective).  Returns pyro-style ``{site name: draws}`` with
+    ``all_gather`` of the draws closes the run (the only collective).  ``initial_values``: a dictionary of sites, None (pyro's
+    uniform start) or ``"periodogram"`` -- the same, but every chain's mixture means start on frequencies drawn from the 95 %
+    highest-density set of its Lomb-Scargle periodogram, so that the chains start on the light curve's own peaks and not all on
+    the same one (one input dimension; GPU).  Returns pyro-style ``{site name: draws}`` with
     chains flattened unless ``group_by_chain``, plus ``"_diagnostics"``.
     """
     import torch.distributed as dist
@@ -556,7 +559,9 @@ def run_mcmc(x, y, noise=None, num_mixtures=4, sampler="NUTS", num_samples=500, 
     if hi > lo:
         pot = SMPotential(xs[lo:hi].contiguous(), ys[lo:hi].contiguous(), None if nz is None else nz[lo:hi].contiguous(),
                           num_mixtures, dim_order, priors, compute)
-        if initial_values is not None:      # {site: value of site.shape (all chains) or (C, *site.shape)}
+        if isinstance(initial_values, str) and initial_values != "periodogram":
+            raise ValueError(f"initial_values must be a dictionary of sites, 'periodogram' or None, got {initial_values!r}")
+        if initial_values is not None and not isinstance(initial_values, str):      # {site: value of site.shape (all chains) or (C, *site.shape)}
             vals = {}
             for st in pot.sites:
                 v = np.asarray(initial_values[st.name], dtype=float)
@@ -566,6 +571,14 @@ def run_mcmc(x, y, noise=None, num_mixtures=4, sampler="NUTS", num_samples=500, 
         else:                                # pyro's default: uniform(-2, 2) in the unconstrained space
             z0 = np.stack([np.random.default_rng([seed, 7919, c]).uniform(-2.0, 2.0, pot.P) for c in range(lo, hi)])
             z0[:, 0] += np.broadcast_to(pot.sites[0].loc, (hi - lo, 1))[:, 0]
+            if initial_values is not None:   # 'periodogram': the mixture means start on draws from the frequency posterior
+                if pot.d != 1:
+                    raise NotImplementedError("initial_values='periodogram' needs light curves with one input dimension")
+                from .lombscargle import draw_frequencies
+                u = np.stack([np.random.default_rng([seed, 104729, c]).random(pot.Q) for c in range(lo, hi)])
+                freqs, _, _ = draw_frequencies(pot.x[..., 0], pot.y, None if pot.noise is None else pot.noise.sqrt(),
+                                               torch.as_tensor(u, device=pot.y.device), top_p=0.95)
+                z0[:, pot.slices()["covar_module.mixture_means_prior"]] = np.log(freqs.cpu().numpy())
         res = sample(pot, z0, num_samples, warmup_steps, sampler, seed, chain_ids=range(lo, hi), **sampler_kwargs)
         P = pot.P
         local = np.concatenate([res["samples"].reshape(hi - lo, -1), res["stats"]["accept_prob"], res["stats"]["n_leapfrog"].astype(float),

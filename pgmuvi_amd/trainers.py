@@ -71,6 +71,16 @@ def _optimiser(optim, params, lr, eps, instances=True, **kw):
     raise ValueError("optim must be 'SGD', 'Adam', 'AdamW'" + (" or a torch optimiser instance" if instances else ""))
 
 
+def _gradient_limit(max_grad_norm):
+    """The argument of the three loops, checked: None (or infinity) for no limit."""
+    if max_grad_norm is None:
+        return None
+    limit = float(max_grad_norm)
+    if not limit >= 0.0:
+        raise ValueError(f"max_grad_norm must not be negative, got {max_grad_norm}")
+    return None if limit == float("inf") else limit
+
+
 _NP_DTYPE = {torch.float64: np.float64, torch.float32: np.float32, torch.float16: np.float16}
 
 
@@ -156,18 +166,21 @@ class _Log:
 
 
 def train(lightcurve=None, model=None, likelihood=None, train_x=None, train_y=None, maxiter=100, miniter=10,
-          stop=None, lr=1e-4, lossfn="mll", optim="SGD", eps=1e-8, stopavg=9, progress=True, **kwargs):
+          stop=None, lr=1e-4, lossfn="mll", optim="SGD", eps=1e-8, stopavg=9, progress=True, max_grad_norm=None, **kwargs):
     """The reference's loop with its arguments, ``results`` and stop rule; the body is ``trainers.py:177-182`` verbatim in
     meaning: zero_grad, ``model(x)``, ``-mll``, backward, step -- one fused HIP evaluation per iteration -- then the
-    per-iteration host read of the loss and the parameters (``:184-195``)."""
+    per-iteration host read of the loss and the parameters (``:184-195``).  ``max_grad_norm``: the gradient of every step is
+    scaled to at most this norm (:func:`pgmuvi_amd.gradients.clip_grad_norm_`; the reference has no such limit)."""
+    max_grad_norm = _gradient_limit(max_grad_norm)
     model, likelihood, train_x, train_y = _problem(lightcurve, model, likelihood, train_x, train_y)
     model.train()
     likelihood.train()
     objective = _mll_objective(lossfn, likelihood, model)
     optimizer = _optimiser(optim, model.parameters(), lr, eps)
-    from . import mll_function
+    from . import gradients, mll_function
     from .gpytorch import settings
     log = _Log(lightcurve, model)
+    parameters = list(model.parameters())
     mll_function.take_deferred_failure()                     # (nothing of an earlier caller's is left pending)
     # Model mode on the GPU with an optimiser made here: the loop runs one iteration ahead of its own log.  The reference's
     # loop copies the loss and every parameter to the host at the end of each iteration (five synchronising copies); here
@@ -199,6 +212,8 @@ def train(lightcurve=None, model=None, likelihood=None, train_x=None, train_y=No
             optimizer.zero_grad()
             loss = -objective(model(train_x), train_y)
             loss.backward()
+        if max_grad_norm is not None:
+            gradients.clip_grad_norm_(parameters, max_grad_norm)
         optimizer.step()
         if not ahead:
             log.loss_and_parameters(loss)
@@ -223,7 +238,7 @@ def train(lightcurve=None, model=None, likelihood=None, train_x=None, train_y=No
 
 
 def train_device(lightcurve=None, model=None, likelihood=None, train_x=None, train_y=None, maxiter=100, miniter=10,
-                 stop=None, lr=1e-4, lossfn="mll", optim="SGD", eps=1e-8, stopavg=9, check_every=25, **kwargs):
+                 stop=None, lr=1e-4, lossfn="mll", optim="SGD", eps=1e-8, stopavg=9, check_every=25, max_grad_norm=None, **kwargs):
     """Device-resident variant of :func:`train`.
 
     One full iteration -- constraint transforms, the fused HIP evaluation, backward, the optimiser
@@ -237,9 +252,10 @@ def train_device(lightcurve=None, model=None, likelihood=None, train_x=None, tra
     factorisation surfaces as a non-finite loss (``NanError``, with the last good parameters
     restored) instead of the jitter retry, and ``optim`` must be one of the string choices.
     """
-    from . import _hip
+    from . import _hip, gradients
     from .gpytorch import settings
     from .gpytorch.utils.errors import NanError
+    max_grad_norm = _gradient_limit(max_grad_norm)
     model, likelihood, train_x, train_y = _problem(lightcurve, model, likelihood, train_x, train_y)
     if not train_x.is_cuda:
         raise RuntimeError("train_device needs the model and data on the GPU")
@@ -260,6 +276,8 @@ def train_device(lightcurve=None, model=None, likelihood=None, train_x=None, tra
         optimizer.zero_grad(set_to_none=False)
         loss = -mll(model(train_x), train_y)
         loss.backward()
+        if max_grad_norm is not None:
+            gradients.clip_grad_norm_(params, max_grad_norm)
         optimizer.step()
         static_loss.copy_(loss.detach())
 
@@ -479,7 +497,7 @@ def _lightcurve_traces(lightcurve, raw_hist):
 
 
 def train_native(lightcurve=None, model=None, likelihood=None, train_x=None, train_y=None, maxiter=100, miniter=10, stop=None,
-                 lr=1e-4, lossfn="mll", optim="SGD", eps=1e-8, stopavg=9, check_every=25, **kwargs):
+                 lr=1e-4, lossfn="mll", optim="SGD", eps=1e-8, stopavg=9, check_every=25, max_grad_norm=None, **kwargs):
     """:func:`train` with the whole optimiser loop on the device (``pgm_fit_*``): constraint
     transforms, evaluation, chain rule, SGD / Adam / AdamW step and the loss / parameter log are one hipGraph replay per
     iteration; the host only reads the log every ``check_every`` iterations for the stop rule of ``pgmuvi/trainers.py:200-207``.
@@ -496,7 +514,10 @@ def train_native(lightcurve=None, model=None, likelihood=None, train_x=None, tra
     _mll_objective(lossfn, likelihood, model)                  # (argument check only: the native loop is the exact MLL)
     if optim not in _hip.NativeFit.OPT:
         _optimiser(optim, [], lr, eps, instances=False)         # raises the loop's own error for anything else
+    max_grad_norm = _gradient_limit(max_grad_norm)
     fit, pieces, raw0 = _native_fit_handle(model, likelihood, train_x, train_y, maxiter, lr, optim, eps)
+    if max_grad_norm is not None:
+        fit.set_clip(max_grad_norm)
     log = _Log(lightcurve, model)
     results = log.results
     names = [n_ for n_, _ in model.named_parameters()]
