@@ -357,13 +357,14 @@ int pgm_lomb_scargle_fast_f64(const double* t, const double* y, const double* dy
  *   layout_host         NULL, or [count][12]: four sizes, four strides of in, four of out (entries, outermost first) of a tensor
  *                       whose entries per member are not one contiguous run; first size 0 = they are.
  * p: 1, 2 or 0 (largest magnitude).  max_norm >= 0 (infinity: nothing is clipped).  norm: [batch] fp64 (norm_f64 != 0) or fp32,
- * device.  scratch: pgm_grad_scratch_doubles(batch, count) doubles of device memory owned by the caller, used by this call only.
+ * device.  scratch: pgm_grad_scratch_doubles doubles of device memory owned by the caller, used by this call only (NULL where
+ * that is 0; bytes: of one member's gradients together, strided: is there a layout_host).
  * Sums are fp64; fp64 tensors' squares are held in three ranges, so that the norm neither overflows nor vanishes where the
  * result does not.  A NaN norm makes every output NaN, an infinite one zero (NaN where the gradient is infinite).  Memory that
  * is written must not be shared with another tensor of the call (-12; interleaved columns of one buffer are fine).
  * Nothing is kept between calls; the call may be captured.  -98: out of host memory.
  */
-int64_t pgm_grad_scratch_doubles(int batch, int count);
+int64_t pgm_grad_scratch_doubles(int batch, int count, int64_t bytes, int strided);
 int pgm_grad_clip(int batch, int count, const uint64_t* in_host, const uint64_t* out_host, const int64_t* numel_host,
                   const unsigned char* type_host, const int64_t* member_host, const int64_t* layout_host, int p,
                   double max_norm, void* norm, int norm_f64, double* scratch, int64_t scratch_doubles, void* stream);

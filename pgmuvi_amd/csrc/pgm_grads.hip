@@ -46,8 +46,8 @@ struct Acc { double mid, big, small; };
 
 constexpr double BIG = 0x1p480, SMALL = 0x1p-480, UP = 0x1p600, DOWN = 0x1p-600;
 
-template <int TYPE> __device__ __forceinline__ void take(Acc& a, double x, int p) {
-  if (p == 2) {
+template <int TYPE, int P> __device__ __forceinline__ void take(Acc& a, double x) {
+  if constexpr (P == 2) {
     if constexpr (TYPE == T_F64) {
       const double m = fabs(x);
       const bool b = m > BIG, s = m < SMALL;
@@ -58,7 +58,7 @@ template <int TYPE> __device__ __forceinline__ void take(Acc& a, double x, int p
     } else {
       a.mid = __builtin_fma(x, x, a.mid);
     }
-  } else if (p == 1) {
+  } else if constexpr (P == 1) {
     a.mid += fabs(x);
   } else {
     const double m = fabs(x);
@@ -118,7 +118,7 @@ template <int TYPE> __device__ __forceinline__ void store1(char* p, int64_t i, d
 }
 
 // entries [lo, hi) of one contiguous run, by the whole workgroup
-template <int TYPE, int THREADS> __device__ __forceinline__ void run_norm(Acc& a, const char* in, int64_t lo, int64_t hi, int p) {
+template <int TYPE, int THREADS, int P> __device__ __forceinline__ void run_norm_p(Acc& a, const char* in, int64_t lo, int64_t hi) {
   using V = Vec<TYPE>;
   constexpr int N = V::N, S = type_bytes(TYPE);
   int64_t i = lo + (int64_t)threadIdx.x * N;
@@ -129,15 +129,23 @@ template <int TYPE, int THREADS> __device__ __forceinline__ void run_norm(Acc& a
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int j = 0; j < N; ++j) take<TYPE>(a, v[k].get(j), p);
+      for (int j = 0; j < N; ++j) take<TYPE, P>(a, v[k].get(j));
   }
   for (; i + N <= hi; i += THREADS * N) {
     V v;
     __builtin_memcpy(&v, in + i * S, 16);
 #pragma unroll
-    for (int j = 0; j < N; ++j) take<TYPE>(a, v.get(j), p);
+    for (int j = 0; j < N; ++j) take<TYPE, P>(a, v.get(j));
   }
-  for (int64_t k = i; k < hi && k < i + N; ++k) take<TYPE>(a, load1<TYPE>(in, k), p);    // (the one thread whose vector ends past hi)
+  for (int64_t k = i; k < hi && k < i + N; ++k) take<TYPE, P>(a, load1<TYPE>(in, k));    // (the one thread whose vector ends past hi)
+}
+template <int TYPE, int THREADS> __device__ __forceinline__ void run_norm(Acc& a, const char* in, int64_t lo, int64_t hi, int p) {
+  if (p == 2) run_norm_p<TYPE, THREADS, 2>(a, in, lo, hi);
+  else if (p == 1) run_norm_p<TYPE, THREADS, 1>(a, in, lo, hi);
+  else run_norm_p<TYPE, THREADS, 0>(a, in, lo, hi);
+}
+template <int TYPE> __device__ __forceinline__ void take_p(Acc& a, double x, int p) {
+  if (p == 2) take<TYPE, 2>(a, x); else if (p == 1) take<TYPE, 1>(a, x); else take<TYPE, 0>(a, x);
 }
 template <int TYPE, int THREADS> __device__ __forceinline__ void run_scale(const char* in, char* out, int64_t lo, int64_t hi, double c) {
   using V = Vec<TYPE>;
@@ -269,6 +277,63 @@ template <int THREADS> __global__ __launch_bounds__(THREADS) void k_member(Table
   }
 }
 
+// The same for members of one type and at most KEEP 16-byte vectors per thread: they stay in registers between the norm and the
+// scaling, so that every gradient is read once (from the cache a second time, 4096 members of 64 KB took 188 us).  Vector
+// k THREADS + thread of the member; `first`: number of the tensors' first vectors
+struct VectorTable { Table T; int first[TABLE + 1]; };
+static_assert(sizeof(VectorTable) <= 3900, "kernel arguments");
+template <int TYPE, int THREADS, int KEEP> __global__ __launch_bounds__(THREADS) void k_member_kept(VectorTable V, int scale, double max_norm, void* norm, int norm_f64) {
+  typedef Vec<TYPE> Reg;
+  constexpr int N = Reg::N, S = type_bytes(TYPE);
+  __shared__ Acc red[THREADS / 64];
+  const Table& T = V.T;
+  const int64_t b = blockIdx.x;
+  Reg v[KEEP];
+  char* to[KEEP];
+  int have[KEEP];                                               // entries of the vector (N, or fewer at a tensor's end; 0: none)
+  bool moved[KEEP];
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k) {
+    have[k] = 0; to[k] = nullptr; moved[k] = false;
+    const int w = k * THREADS + (int)threadIdx.x;
+    if (w >= V.first[T.count]) continue;
+    int t = 0;
+    while (w >= V.first[t + 1]) ++t;
+    const Entry& e = T.e[t];
+    const int64_t i = (int64_t)(w - V.first[t]) * N;
+    const char* in = e.in + (b * e.in_stride + i) * S;
+    to[k] = e.out + (b * e.out_stride + i) * S;
+    moved[k] = to[k] != in;
+    if (i + N <= e.n) {
+      have[k] = N;
+      __builtin_memcpy(&v[k], in, 16);
+    } else {
+      have[k] = (int)(e.n - i);
+#pragma unroll
+      for (int j = 0; j < N; ++j) if (j < have[k]) v[k].v[j] = reinterpret_cast<const Reg*>(in)->v[j];
+    }
+  }
+  Acc a{0.0, 0.0, 0.0};
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k)
+#pragma unroll
+    for (int j = 0; j < N; ++j) if (j < have[k]) take_p<TYPE>(a, v[k].get(j), T.p);
+  const double n = norm_of(block_join<THREADS>(a, T.p, red), T.p);
+  if (threadIdx.x == 0) store_norm(norm, norm_f64, b, n);
+  if (!scale) return;
+  const double c = factor_of(n, max_norm);
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k) {
+    if (have[k] == 0 || (c == 1.0 && !moved[k])) continue;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[k].set(j, v[k].get(j) * c);
+    if (have[k] == N) __builtin_memcpy(to[k], &v[k], 16);
+    else
+#pragma unroll
+      for (int j = 0; j < N; ++j) if (j < have[k]) reinterpret_cast<Reg*>(to[k])->v[j] = v[k].v[j];
+  }
+}
+
 // ---- tensors whose entries are not one run: one entry per thread and step, its address from the four sizes -----------------
 template <class F> __device__ __forceinline__ void for_strided(const StridedTable& T, int64_t b, int g, int groups, F f) {
   for (int t = 0; t < T.count; ++t) {
@@ -292,7 +357,7 @@ __global__ __launch_bounds__(NT) void k_norm_part_strided(StridedTable T, int gr
   const int g = blockIdx.x % groups;
   Acc a{0.0, 0.0, 0.0};
   for_strided(T, b, g, groups, [&](const StridedEntry& e, int64_t in, int64_t) {
-#define PGM_CALL(TY) take<TY>(a, load1<TY>(e.in, in), T.p)
+#define PGM_CALL(TY) take_p<TY>(a, load1<TY>(e.in, in), T.p)
     PGM_BY_TYPE(e.type, PGM_CALL)
 #undef PGM_CALL
   });
@@ -335,6 +400,10 @@ bool any_clash(std::vector<Span>& v) {
 }
 
 struct Item { int type; int64_t n; const char* in; char* out; int64_t in_member, out_member; const int64_t* layout; int64_t bytes, chunks; };
+
+// One workgroup per member, in one launch: a small set (one CU streams 64 KB in the time a second launch takes), or members enough
+// to fill the chip with whole workgroups
+bool one_launch(int batch, int64_t count, int64_t bytes, bool strided) { return !strided && count <= TABLE && (bytes <= 65536 || batch >= 512); }
 
 int run_clip(int batch, int count, const uint64_t* in, const uint64_t* out, const int64_t* numel, const unsigned char* type,
              const int64_t* member, const int64_t* layout, int p, double max_norm, void* norm, int norm_f64, double* scratch,
@@ -394,15 +463,31 @@ int run_clip(int batch, int count, const uint64_t* in, const uint64_t* out, cons
     }
     T.chunks = (int)c;
   };
-  // One workgroup per member: a small set (one launch instead of two; one CU streams ~100 KB in the time a launch takes), or
-  // members enough to fill the chip with whole workgroups.
-  if (loose.empty() && flat.size() <= (size_t)TABLE && (per_member <= 65536 || batch >= 512)) {
-    Table T;
-    fill(T, 0, flat.size());
-    if (per_member <= 8192) hipLaunchKernelGGL(k_member<NT>, dim3(batch), dim3(NT), 0, st, T, scale, max_norm, norm, norm_f64);
-    else hipLaunchKernelGGL(k_member<1024>, dim3(batch), dim3(1024), 0, st, T, scale, max_norm, norm, norm_f64);
+  if (one_launch(batch, (int64_t)flat.size(), per_member, !loose.empty())) {
+    bool same = true;
+    int64_t vectors = 0;
+    for (const Item& it : flat) { same = same && it.type == flat[0].type; vectors += (it.bytes + 15) / 16; }
+    constexpr int SMALL = NT, LARGE = 1024, FEW = 4, KEEP = 8;
+    if (!flat.empty() && same && vectors <= KEEP * LARGE) {
+      VectorTable V;
+      fill(V.T, 0, flat.size());
+      int at = 0;
+      for (size_t i = 0; i < flat.size(); ++i) { V.first[i] = at; at += (int)((flat[i].bytes + 15) / 16); }
+      V.first[flat.size()] = at;
+      // (256 threads while four vectors each cover the member, so that 8 members share a CU; else 1024 with up to eight)
+#define PGM_CALL(TY) do { if (vectors <= FEW * SMALL) hipLaunchKernelGGL((k_member_kept<TY, SMALL, FEW>), dim3(batch), dim3(SMALL), 0, st, V, scale, max_norm, norm, norm_f64); \
+                          else hipLaunchKernelGGL((k_member_kept<TY, LARGE, KEEP>), dim3(batch), dim3(LARGE), 0, st, V, scale, max_norm, norm, norm_f64); } while (0)
+      PGM_BY_TYPE(flat[0].type, PGM_CALL)
+#undef PGM_CALL
+    } else {
+      Table T;
+      fill(T, 0, flat.size());
+      if (per_member <= 8192) hipLaunchKernelGGL(k_member<NT>, dim3(batch), dim3(NT), 0, st, T, scale, max_norm, norm, norm_f64);
+      else hipLaunchKernelGGL(k_member<1024>, dim3(batch), dim3(1024), 0, st, T, scale, max_norm, norm, norm_f64);
+    }
     return hipGetLastError() == hipSuccess ? 0 : -99;
   }
+  if (!scratch) return -13;
   struct Launch { size_t i0, i1; int64_t chunks; int groups; bool strided; int64_t slot0; };
   std::vector<Launch> launches;
   auto plan = [&](const std::vector<Item>& items, size_t width, bool strided) {
@@ -456,8 +541,9 @@ int run_clip(int batch, int count, const uint64_t* in, const uint64_t* out, cons
 
 }  // namespace
 
-extern "C" int64_t pgm_grad_scratch_doubles(int batch, int count) {
-  if (batch < 1 || count < 0) return 0;
+extern "C" int64_t pgm_grad_scratch_doubles(int batch, int count, int64_t bytes, int strided) {
+  if (batch < 1 || count < 0 || bytes < 0) return 0;
+  if (one_launch(batch, count, bytes, strided != 0)) return 0;
   // one partial sum of three doubles per workgroup: PARTS of them, and at most one more per launch and member
   const int64_t launches = (int64_t)count / TABLE + 1 + (int64_t)count / STRIDED_TABLE + 1;
   return 3 * ((int64_t)PARTS + launches * batch);
@@ -474,7 +560,6 @@ extern "C" int pgm_grad_clip(int batch, int count, const uint64_t* in_host, cons
   if (p < 0 || p > 2) return -9;
   if (out_host && !(max_norm >= 0.0)) return -10;
   if (!norm) return -11;
-  if (!scratch) return -13;
   try {
     return run_clip(batch, count, in_host, out_host, numel_host, type_host, member_host, layout_host, p, max_norm, norm, norm_f64,
                     scratch, scratch_doubles, (hipStream_t)stream);

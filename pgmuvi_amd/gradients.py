@@ -12,16 +12,15 @@ There is no CPU path: tensors on the GPU or an error.  Nothing synchronises the 
 """
 from __future__ import annotations
 
-import ctypes
 import math
-from ctypes import c_void_p
+from array import array
 
-import numpy as np
 import torch
 
 from . import _hip
 
 _TYPE = {torch.float64: 0, torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}
+_BYTES = (8, 4, 2, 2)
 _POWER = {1.0: 1, 2.0: 2, math.inf: 0}
 
 
@@ -54,58 +53,63 @@ def _dense_order(t):
 
 
 def _describe(tensors, outs, batch):
-    """Host arrays of ``pgm_grad_clip``: (in, out, numel, type, member strides | None, layouts | None)."""
-    count = len(tensors)
-    numel = np.fromiter((t.numel() for t in tensors), dtype=np.int64, count=count)
-    types = np.fromiter((_TYPE[t.dtype] for t in tensors), dtype=np.uint8, count=count)
-    src = np.fromiter((t.data_ptr() for t in tensors), dtype=np.uint64, count=count)
-    dst = src if outs is tensors else None if outs is None else np.fromiter((o.data_ptr() for o in outs), dtype=np.uint64, count=count)
+    """Host arrays of ``pgm_grad_clip``: (in, out | None, numel, type, member strides | None, layouts | None).  (A training step calls
+    this between two launches: one C call per tensor and property, no array library.)"""
+    T = torch.Tensor
+    numel = array("q", map(T.numel, tensors))
+    kinds = {t.dtype for t in tensors}
+    types = bytearray([_TYPE[kinds.pop()]]) * len(tensors) if len(kinds) == 1 else bytearray(_TYPE[t.dtype] for t in tensors)
+    src = array("Q", map(T.data_ptr, tensors))
+    dst = src if outs is tensors else None if outs is None else array("Q", map(T.data_ptr, outs))
     member = layout = None
     if batch is not None:
-        numel //= batch
-        member = np.empty((count, 2), dtype=np.int64)
-        member[:, 0] = member[:, 1] = numel
-    plain = [t.is_contiguous() for t in tensors]
-    if outs is not None and outs is not tensors:
-        plain = [p and o.is_contiguous() for p, o in zip(plain, outs)]
-    if all(plain):
+        numel = array("q", [n // batch for n in numel])
+        member = array("q", [n for n in numel for _ in (0, 1)])
+    if all(map(T.is_contiguous, tensors)) and (dst is src or dst is None or all(map(T.is_contiguous, outs))):
         return src, dst, numel, types, member, layout
     first = 0 if batch is None else 1
-    for i, ok in enumerate(plain):
-        t = tensors[i]
-        if ok or t.numel() == 0:
-            continue
+    for i, t in enumerate(tensors):
         o = t if outs is None else outs[i]
+        if t.numel() == 0 or (t.is_contiguous() and o.is_contiguous()):
+            continue
         if outs is not None and _overlaps_itself(o.shape, o.stride()):
             raise ValueError(f"gradient {i}: a tensor whose entries share memory (an expanded view) cannot be written")
         order = [k for k in _dense_order(t) if first == 0 or k != 0]
         dims = _coalesced([t.shape[k] for k in order], [t.stride(k) for k in order], [o.stride(k) for k in order])
         if batch is not None:
-            member[i] = t.stride(0), o.stride(0)
+            member[2 * i], member[2 * i + 1] = t.stride(0), o.stride(0)
         if len(dims) == 0 or (len(dims) == 1 and dims[0][1] == 1 and dims[0][2] == 1):
             continue                                             # (permuted, padded between members, ...: one run per member)
         if len(dims) > 4:
             raise ValueError(f"gradient {i}: more than four strided dimensions; make it contiguous")
         if layout is None:
-            layout = np.zeros((count, 12), dtype=np.int64)
+            layout = array("q", bytes(96 * len(tensors)))
         dims = [(1, 0, 0)] * (4 - len(dims)) + dims
-        layout[i] = [d[0] for d in dims] + [d[1] for d in dims] + [d[2] for d in dims]
+        layout[12 * i:12 * i + 12] = array("q", [d[k] for k in range(3) for d in dims])
     return src, dst, numel, types, member, layout
+
+
+_PLAIN = {torch.Tensor, torch.nn.Parameter}
 
 
 def _tensors(tensors, what):
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
-    for t in tensors:
-        if not torch.is_tensor(t):
-            raise TypeError(f"{what}: tensors expected, got {type(t).__name__}")
-        if t.layout is not torch.strided or t.dtype not in _TYPE:
-            raise TypeError(f"{what}: dense float64, float32, bfloat16 or float16 tensors expected, got {t.dtype} ({t.layout})")
+    if not _PLAIN.issuperset(map(type, tensors)):
+        for t in tensors:
+            if not torch.is_tensor(t):
+                raise TypeError(f"{what}: tensors expected, got {type(t).__name__}")
+    if not _TYPE.keys() >= {t.dtype for t in tensors} or not {torch.strided} >= {t.layout for t in tensors}:
+        raise TypeError(f"{what}: dense float64, float32, bfloat16 or float16 tensors expected, got "
+                        f"{sorted({str(t.dtype) + ' ' + str(t.layout) for t in tensors})}")
     if tensors:
         _hip.require_gpu(tensors[0], what)
-        where = tensors[0].get_device()
-        if any(t.get_device() != where for t in tensors):
+        if len(set(map(torch.Tensor.get_device, tensors))) != 1:
             raise ValueError(f"{what}: all tensors must be on one device")
     return tensors
+
+
+def _address(a):
+    return None if a is None else a.buffer_info()[0]
 
 
 def _run(tensors, outs, max_norm, norm_type, members, what):
@@ -128,12 +132,14 @@ def _run(tensors, outs, max_norm, norm_type, members, what):
         return norm
     src, dst, numel, types, member, layout = _describe(tensors, outs, batch)
     lib = _hip.load()
-    n = int(lib.pgm_grad_scratch_doubles(batch or 1, len(tensors)))
-    scratch = torch.empty(n, dtype=torch.float64, device=dev)
-    at = lambda a: None if a is None else a.ctypes.data_as(c_void_p)
-    with torch.cuda.device(dev):
-        rc = lib.pgm_grad_clip(batch or 1, len(tensors), at(src), at(dst), at(numel), at(types), at(member), at(layout), p,
-                               float(max_norm), norm.data_ptr(), 1 if f64 else 0, scratch.data_ptr(), n, _hip.current_stream_ptr(dev))
+    members, count = batch or 1, len(tensors)
+    same = types.count(types[0]) == count
+    bytes_ = sum(numel) * _BYTES[types[0]] if same else sum(n * _BYTES[k] for n, k in zip(numel, types))
+    n = lib.pgm_grad_scratch_doubles(members, count, bytes_, layout is not None)
+    scratch = torch.empty(n, dtype=torch.float64, device=dev) if n else None
+    with _hip.on_device(dev.index):
+        rc = lib.pgm_grad_clip(members, count, _address(src), _address(dst), _address(numel), bytes(types), _address(member), _address(layout), p,
+                               max_norm, norm.data_ptr(), f64, None if scratch is None else scratch.data_ptr(), n, _hip.stream_of(dev.index))
     if rc == -12:
         raise ValueError(f"{what}: tensors that share memory cannot be clipped together (the same gradient given twice?)")
     _hip._check(rc, "pgm_grad_clip")
@@ -144,8 +150,7 @@ def total_norm(tensors, norm_type: float = 2.0, members: bool = False) -> torch.
     """Norm over every entry of every tensor (on the device; no synchronisation): a 0-dim tensor, float64 if any of the
     tensors is, else float32.  ``members``: the tensors share a leading axis of independent fits and each gets its own norm,
     (B,).  ``norm_type``: 1, 2 or ``inf``."""
-    with torch.no_grad():
-        return _run(_tensors(tensors, "total_norm"), None, 0.0, norm_type, members, "total_norm")
+    return _run(_tensors(tensors, "total_norm"), None, 0.0, norm_type, members, "total_norm")
 
 
 def clip_grads_(grads, max_norm: float, norm_type: float = 2.0, out=None, members: bool = False,
@@ -165,14 +170,14 @@ def clip_grads_(grads, max_norm: float, norm_type: float = 2.0, out=None, member
             raise ValueError("clip_grads_: out must hold one tensor of the same shape and type for every gradient")
         if grads and outs[0].device != grads[0].device:
             raise ValueError("clip_grads_: all tensors must be on one device")
-    with torch.no_grad():
-        if error_if_nonfinite:
-            norm = _run(grads, None, 0.0, norm_type, members, "clip_grads_")
-            if not bool(torch.isfinite(norm).all()):
-                raise RuntimeError("clip_grads_: the norm of the gradients is not finite, so they were not clipped")
-        norm = _run(grads, outs, max_norm, norm_type, members, "clip_grads_")
+    if error_if_nonfinite:
+        norm = _run(grads, None, 0.0, norm_type, members, "clip_grads_")
+        if not bool(torch.isfinite(norm).all()):
+            raise RuntimeError("clip_grads_: the norm of the gradients is not finite, so they were not clipped")
+    norm = _run(grads, outs, max_norm, norm_type, members, "clip_grads_")
+    if outs:
         torch.autograd.graph.increment_version(outs)             # (autograd does not see the kernel's writes by itself)
-        return norm
+    return norm
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:

@@ -49,19 +49,19 @@ def test_strided_tensors_are_described_entry_by_entry(make):
     _, dst, numel, _, member, layout = G._describe([t, torch.zeros(3)], None, None)
     assert dst is None and member is None and numel.tolist() == [t.numel(), 3]
     want = sorted(sum(i * s for i, s in zip(idx, t.stride())) for idx in np.ndindex(*t.shape))
-    assert _walk(None if layout is None else layout[0], 0, t.numel()) == want
+    assert _walk(None if layout is None else layout[:12], 0, t.numel()) == want
 
 
 def test_members_of_columns_are_runs_with_the_buffer_as_distance():
     buf = torch.zeros(6, 11)
     cols = [buf[:, :4], buf[:, 4:5], buf[:, 5:]]
     src, dst, numel, _, member, layout = G._describe(cols, cols, 6)
-    assert numel.tolist() == [4, 1, 6] and member.tolist() == [[11, 11]] * 3 and layout is None
+    assert numel.tolist() == [4, 1, 6] and member.tolist() == [11, 11] * 3 and layout is None
     t = torch.zeros(6, 5, 4).transpose(1, 2)                     # permuted inside the member: still one run, read in memory order
     _, _, numel, _, member, layout = G._describe([t], [t], 6)
-    assert numel.tolist() == [20] and member.tolist() == [[20, 20]] and layout is None
+    assert numel.tolist() == [20] and member.tolist() == [20, 20] and layout is None
     _, _, _, _, _, layout = G._describe([t], [torch.zeros(6, 4, 5)], 6)
-    assert layout is not None and sorted(layout[0][:4].tolist()) == [1, 1, 4, 5]
+    assert layout is not None and sorted(layout[:4].tolist()) == [1, 1, 4, 5]
 
 
 def test_expanded_outputs_are_refused():
@@ -97,7 +97,7 @@ A = 1 << 20
     (-10, dict(src=[A], dst=[A], numel=[8], types=[0], max_norm=-1.0)),
     (-10, dict(src=[A], dst=[A], numel=[8], types=[0], max_norm=math.nan)),
     (-11, dict(src=[A], dst=None, numel=[8], types=[0], norm=None)),
-    (-13, dict(src=[A], dst=None, numel=[8], types=[0], scratch=None)),
+    (-13, dict(src=[A], dst=None, numel=[1 << 24], types=[0], scratch=None)),
     (-14, dict(src=[A], dst=None, numel=[1 << 24], types=[0], doubles=3)),
     (-12, dict(src=[A, A], dst=[A, A], numel=[8, 8], types=[0, 0])),                                        # the same gradient twice
     (-12, dict(src=[A, A + 56], dst=[A, A + 56], numel=[8, 8], types=[0, 0])),                              # overlapping by one entry
@@ -112,8 +112,10 @@ def test_refusals_come_before_any_launch(code, kw):
 
 
 def test_scratch_covers_every_launch():
-    lib = _hip.load()
-    assert lib.pgm_grad_scratch_doubles(0, 3) == 0 and lib.pgm_grad_scratch_doubles(1, -1) == 0
-    for batch in (1, 7, 4096):
-        for count in (0, 1, 64, 65, 5000):
-            assert lib.pgm_grad_scratch_doubles(batch, count) >= 3 * (2048 + batch * (count // 64 + 1))
+    need = _hip.load().pgm_grad_scratch_doubles
+    assert need(0, 3, 8, 0) == 0 and need(1, -1, 8, 0) == 0 and need(1, 3, -8, 0) == 0
+    assert need(1, 5, 112, 0) == 0 and need(4096, 5, 1 << 20, 0) == 0            # (one launch: no partial sums)
+    for batch in (1, 7, 300):
+        for count in (1, 64, 65, 5000):
+            assert need(batch, count, 1 << 24, 0) >= 3 * (2048 + batch * (count // 64 + 1))
+            assert need(batch, count, 64, 1) >= 3 * (2048 + batch * (count // 24 + 1))
