@@ -23,7 +23,7 @@
 namespace {
 
 typedef unsigned long long u64;
-constexpr int LOAD = 16, BATCH = 4;                             // bytes of a lane's load; loads of a wavefront in flight
+constexpr int LOAD = 16, CB = 2;                                // bytes of a lane's load; cells a wavefront works on at a time
 constexpr int MAX_CELLS = 1024;                                 // of a row (longer rows: wider cells)
 constexpr int64_t MAX_COLS = 1 << 24;                           // 2^24 weights of at most one, in steps of 2^-40, fit 64 bits
 constexpr int64_t EVERY = INT64_MAX;
@@ -161,10 +161,9 @@ template <class F> struct Row {
 };
 
 // Builds of a row's code: 8 wavefronts for a row, 4 where there are rows enough to fill the chip with such workgroups (their phases
-// overlap better), 4 or one (no barriers) with small tables for short rows; All: the launches that share a long row's cut
+// overlap better), one with small tables for very short rows (no barriers); All: the launches that share a long row's cut
 struct Long { static constexpr int NT = 512, BITS = 11, CELLS = MAX_CELLS, LIST = 512; };
 struct Many { static constexpr int NT = 256, BITS = 10, CELLS = MAX_CELLS, LIST = 256; };
-struct Short { static constexpr int NT = 256, BITS = 9, CELLS = 64, LIST = 256; };
 struct Tiny { static constexpr int NT = 64, BITS = 8, CELLS = 8, LIST = 64; };
 struct All { static constexpr int NT = 1024, BITS = 12, CELLS = MAX_CELLS, LIST = 1024; };
 
@@ -182,44 +181,59 @@ template <class C> struct Shared {
 };
 
 // f(cell, this lane's entries, number of its first one, last group of the cell?) for the cells c0 <= c < c1 -- with SEEN only those
-// whose highest value is at least `lo`: a wavefront per cell.  The next cells' loads are in flight while the present ones are
-// worked on.
-template <bool SEEN, int THREADS, bool HEAVY = true, class F, class Fn> __device__ __forceinline__ void for_cells(const Row<F>& R, const double* best, int c0, int c1, double lo, Fn f) {
+// whose highest value is at least `lo`: a wavefront per cell.  The next CB cells' loads are in flight while the present ones are
+// worked on; the row's end, strided rows and very long ones go one group of loads after the other.
+template <bool SEEN, int THREADS, class F, class Fn> __device__ __forceinline__ void for_cells(const Row<F>& R, const double* best, int c0, int c1, double lo, Fn f) {
   typedef typename F::raw raw;
-  constexpr int NW = THREADS / 64, VEC = Row<F>::VEC, U = F::U, CB = BATCH / U, STEP = NW * CB;
+  constexpr int NW = THREADS / 64, VEC = Row<F>::VEC, U = F::U, STEP = NW * CB;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int full = c0;                                                // the cells up to here are one whole group of loads
   if (R.mult == 1 && R.stride == 1) {
     const int whole = (int)(R.n / (U * Row<F>::UNIT));
     full = whole < c1 ? whole : c1;
-    raw next[CB][U][VEC];
-    auto wanted = [&](int cc) { return cc < full && (!SEEN || best[cc] >= lo); };
-    auto fetch = [&](int c) {
-#pragma unroll
-      for (int s = 0; s < CB; ++s) if (wanted(c + s * NW)) R.load_whole(c + s * NW, next[s]);
-    };
-    int c = c0 + wave;
-    if (c < full) fetch(c);
-    for (; c < full; c += STEP) {
-      raw r[CB][U][VEC];
-      __builtin_memcpy(r, next, sizeof(r));
-      if (c + STEP < full) fetch(c + STEP);
-#pragma unroll
-      for (int s = 0; s < CB; ++s) {
-        if (wanted(c + s * NW)) f(c + s * NW, r[s], R.first(c + s * NW), true);
-        if (HEAVY) __builtin_amdgcn_sched_barrier(0);           // (one cell's exponentials at a time: interleaved, they do not fit the registers)
-      }
-    }
     full = full > c0 ? full : c0;
   }
-  for (int c = full + wave; c < c1; c += NW) {                  // the row's end; strided rows; very long ones
-    if (SEEN && !(best[c] >= lo)) continue;
+  raw next[CB][U][VEC];
+  auto wanted = [&](int cc) { return !SEEN || best[cc] >= lo; };
+  auto fetch = [&](int c) {
+#pragma unroll
+    for (int s = 0; s < CB; ++s) if (c + s * NW < full && wanted(c + s * NW)) R.load_whole(c + s * NW, next[s]);
+  };
+  // (two loops: in one, the compiler's wait for the loads of the slow kind would hold up those in flight as well)
+  int c = c0 + wave;
+  if (c < full) fetch(c);
+  for (; c < full; c += STEP) {
+    raw r[CB][U][VEC];
+    __builtin_memcpy(r, next, sizeof(r));
+    if (c + STEP < full) fetch(c + STEP);
+#pragma unroll
+    for (int s = 0; s < CB; ++s)
+      if (c + s * NW < full && wanted(c + s * NW)) f(c + s * NW, r[s], R.first(c + s * NW), true);
+  }
+  for (c = full + wave; c < c1; c += NW) {
+    if (!wanted(c)) continue;
     for (int j = 0; j < R.mult; ++j) {
       raw r[U][VEC];
       const int64_t g = (int64_t)c * R.mult + j;
       if (R.stride == 1 && (g + 1) * (U * Row<F>::UNIT) <= R.n) R.load_whole(g, r); else R.load_part(g, r);
       f(c, r, R.first(g), j == R.mult - 1);
     }
+  }
+}
+// g(value, number) for this lane's entries of a group, two at a time in a loop (unrolled, the exponentials of all of them fill the
+// registers several times over)
+template <class F, class Fn> __device__ __forceinline__ void each(const typename F::raw (&r)[F::U][Row<F>::VEC], int64_t i0, Fn g) {
+  constexpr int VEC = Row<F>::VEC, M = F::U * VEC;
+  typename F::wide v[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) v[m] = F::widen(r[m / VEC][m % VEC]);
+#pragma unroll 1
+  for (int m = 0; m < M; m += 2) {
+    const int64_t i = i0 + (m / VEC) * Row<F>::UNIT + m % VEC;
+    g(v[0], i);
+    g(v[1], i + 1);
+#pragma unroll
+    for (int k = 0; k + 2 < M; ++k) v[k] = v[k + 2];
   }
 }
 
@@ -307,7 +321,7 @@ struct Even {                                                   // the first bin
 template <bool WEIGHTED, bool SEEDED, class C, class F> __device__ Cut select(const Row<F>& R, Shared<C>& S, double lo, Cut have, u64 want, double share) {
   typedef typename F::raw raw;
   typedef typename F::wide wide;
-  constexpr int VEC = Row<F>::VEC, U = F::U, UNIT = Row<F>::UNIT, BINS = Shared<C>::BINS;
+  constexpr int VEC = Row<F>::VEC, U = F::U, BINS = Shared<C>::BINS;
   u64 bn = 0, bhi = 0, blo = 0;
   double target = -1.0;
   bool first = true;
@@ -321,20 +335,12 @@ template <bool WEIGHTED, bool SEEDED, class C, class F> __device__ Cut select(co
     // all the entries in the range, f(value, index, bin)
     auto entries = [&](auto f) {
       for_cells<true, C::NT>(R, S.best, 0, R.cells, lo, [&](int, const raw (&r)[U][VEC], int64_t i0, bool) {
-#pragma unroll
-        for (int q = 0; q < U; ++q)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const wide v = F::widen(r[q][e]);
-            if (!(v < quick)) {
-              const double l = (double)v;
-              const int64_t i = i0 + q * UNIT + e;
-              if (l >= lo && have.keeps(l, i)) {
-                if (even) f(l, i, parts.bin(l));
-                else { const u64 k = key_of(l); if (k <= khi) f(l, i, (int)((khi - k) >> shift)); }
-              }
-            }
-          }
+        each<F>(r, i0, [&](wide v, int64_t i) {
+          const double l = (double)v;
+          if (v < quick || !(l >= lo) || !have.keeps(l, i)) return;
+          if (even) f(l, i, parts.bin(l));
+          else { const u64 k = key_of(l); if (k <= khi) f(l, i, (int)((khi - k) >> shift)); }
+        });
       });
     };
     const bool seeded = SEEDED && first && even;
@@ -342,7 +348,7 @@ template <bool WEIGHTED, bool SEEDED, class C, class F> __device__ Cut select(co
       clear_bins<WEIGHTED>(S);
       entries([&](double l, int64_t, int b) {
         atomicAdd(&S.bins.count[b], 1u);
-        if (WEIGHTED) { add_weight(S, b, R.weight(l)); __builtin_amdgcn_sched_barrier(0); }
+        if (WEIGHTED) add_weight(S, b, R.weight(l));
       });
     }
     find_bin<WEIGHTED>(S, bn, bhi, blo, want, share, target);
@@ -388,13 +394,9 @@ template <bool WEIGHTED, bool SEEDED, class C, class F> __device__ Cut select(co
         const int ishift = shift_of<C>((u64)(i1 - i0));
         clear_bins<false>(S);
         for_cells<true, C::NT>(R, S.best, (int)(i0 / R.width()), (int)(i1 / R.width()) + 1, low, [&](int, const raw (&r)[U][VEC], int64_t at, bool) {
-#pragma unroll
-          for (int q = 0; q < U; ++q)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              const int64_t i = at + q * UNIT + e;
-              if ((double)F::widen(r[q][e]) == low && i >= i0 && i <= i1 && have.keeps(low, i)) atomicAdd(&S.bins.count[(u64)(i - i0) >> ishift], 1u);
-            }
+          each<F>(r, at, [&](wide v, int64_t i) {
+            if ((double)v == low && i >= i0 && i <= i1 && have.keeps(low, i)) atomicAdd(&S.bins.count[(u64)(i - i0) >> ishift], 1u);
+          });
         });
         find_bin<false>(S, passed, 0, 0, m, 0.0, 0.0);
         const int64_t from = i0 + (int64_t)(S.found[0] << ishift), to = from + (int64_t)((1ull << ishift) - 1);
@@ -450,7 +452,7 @@ template <int THREADS, bool SUMS, class F> __device__ __forceinline__ double pas
   constexpr int VEC = Row<F>::VEC, U = F::U;
   const wide none = (wide)-INF;
   wide run = none, low = -none;
-  for_cells<false, THREADS, SUMS>(R, (const double*)nullptr, c0, c1, 0.0, [&](int c, const raw (&r)[U][VEC], int64_t, bool last) {
+  for_cells<false, THREADS>(R, (const double*)nullptr, c0, c1, 0.0, [&](int c, const raw (&r)[U][VEC], int64_t, bool last) {
 #pragma unroll
     for (int q = 0; q < U; ++q)
 #pragma unroll
@@ -471,15 +473,10 @@ template <int THREADS, bool SUMS, class F> __device__ __forceinline__ double pas
       R.best = (double)top;
       const bool certain = top == -none;                        // (an infinite entry: the finite ones beside it weigh nothing)
       auto add = [&](const raw (&x)[U][VEC]) {
-#pragma unroll
-        for (int q = 0; q < U; ++q)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const wide v = F::widen(x[q][e]);
-            const double w = R.weight((double)v);
-            s += v > none && (!certain || v == top) ? w : 0.0;
-            if (e & 1) __builtin_amdgcn_sched_barrier(0);
-          }
+        each<F>(x, 0, [&](wide v, int64_t) {
+          const double w = R.weight((double)v);
+          s += v > none && (!certain || v == top) ? w : 0.0;
+        });
       };
       if (R.mult == 1) add(r);
       else for (int j = 0; j < R.mult; ++j) {
@@ -514,17 +511,12 @@ template <int THREADS, class F> __device__ __forceinline__ void pass_weights(con
   for (int c = c0 + (int)threadIdx.x; c < c1; c += THREADS) if (!(best[c] >= lo)) sums[c] = 0.0;
   double s = 0.0;
   for_cells<true, THREADS>(R, best, c0, c1, lo, [&](int c, const raw (&r)[U][VEC], int64_t i0, bool last) {
-#pragma unroll
-    for (int q = 0; q < U; ++q)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const wide v = F::widen(r[q][e]);
-        if (!(v < quick)) {
-          const double l = (double)v;
-          if (l >= lo && cut.keeps(l, i0 + q * Row<F>::UNIT + e)) { const double w = R.weight(l); s += w < min_p ? 0.0 : w; }
-        }
-        if (e & 1) __builtin_amdgcn_sched_barrier(0);
-      }
+    each<F>(r, i0, [&](wide v, int64_t i) {
+      const double l = (double)v;
+      if (v < quick || !(l >= lo) || !cut.keeps(l, i)) return;
+      const double w = R.weight(l);
+      s += w < min_p ? 0.0 : w;
+    });
     if (!last) return;
     const double total = wave_sum(s);
     s = 0.0;
@@ -562,20 +554,40 @@ template <class C, class F> __device__ __forceinline__ void draw(const DrawArgs&
     int c = first_above(S.cells, R.cells, target, false);
     if (c == R.cells) { c = first_above(S.cells, R.cells, Z, true); target = INF; }
     double base = c ? S.cells[c - 1] : 0.0;
-    const int64_t i0 = c * R.width();
+    // the cell's running weight: every lane sums PER neighbouring entries, one scan over the lanes, and the lane that reaches the
+    // target looks through its own
+    constexpr int PER = F::U * Row<F>::VEC;
     int64_t found = -1, last = -1;
-    const int steps = (int)(R.width() / 64);
-    for (int j = 0; j < steps && found < 0; ++j) {
-      const int64_t i = i0 + 64 * (int64_t)j + lane;
-      double w = 0.0;
-      if (i < R.n) {
-        const double l = R.value(i);
-        if (l > -INF && cut.keeps(l, i)) { w = R.weight(l); w = w < min_p ? 0.0 : w; }
+    for (int j = 0; j < R.mult && found < 0; ++j) {
+      const int64_t i0 = c * R.width() + (int64_t)j * 64 * PER + lane * PER;
+      double w[PER], sum = 0.0;
+      int some = -1;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) {
+        w[e] = 0.0;
+        if (i0 + e < R.n) {
+          const double l = R.value(i0 + e);
+          if (l > -INF && cut.keeps(l, i0 + e)) { const double x = R.weight(l); w[e] = x < min_p ? 0.0 : x; }
+        }
+        sum += w[e];
+        some = w[e] > 0.0 ? e : some;
       }
-      const double inc = wave_scan(w);
-      const u64 hit = __ballot(w > 0.0 && base + inc > target), some = __ballot(w > 0.0);
-      if (hit) found = i0 + 64 * (int64_t)j + __ffsll(hit) - 1;
-      if (some) last = i0 + 64 * (int64_t)j + 63 - __clzll(some);
+      const double inc = wave_scan(sum);
+      const u64 hit = __ballot(sum > 0.0 && base + inc > target), any = __ballot(sum > 0.0);
+      if (any) { const int l = 63 - __clzll(any); last = i0 - lane * PER + l * PER + __shfl(some, l); }
+      if (hit) {
+        const int l = __ffsll(hit) - 1;
+        double run = base + (inc - sum);
+        int e = some;                                           // (its last kept one, should the sums differ by a rounding)
+#pragma unroll
+        for (int k = PER - 1; k >= 0; --k) {                    // run before entry k, from the back: the first that passes the target stays
+          double r = run;
+#pragma unroll
+          for (int m = 0; m <= k; ++m) r += w[m];
+          if (w[k] > 0.0 && r > target) e = k;
+        }
+        found = i0 - lane * PER + l * PER + __shfl(e, l);
+      }
       base += __shfl(inc, 63);
     }
     if (found < 0) found = last;                                // (the cell's own sum and this one differ by a rounding)
@@ -666,20 +678,29 @@ template <class C, class F> __device__ Cut cut_of(const Row<F>& R, Shared<C>& S,
     bool bounded;
     const double lo = bound_of_top_k<C, F>(R, S, p.top_k, lowest, bounded);
     __syncthreads();
+    int upto = -1;                                              // (bins the list takes; -1: everything from the bound on)
+    const Even parts(R.best, lo > cut.value ? lo : cut.value, Shared<C>::BINS);
+    if (p.top_k <= C::LIST && !bounded && R.n > C::LIST && parts.good) {
+      // no bound from the cells: from bins over all entries
+      const double floor = lo > cut.value ? lo : cut.value;
+      for_cells<true, C::NT>(R, S.best, 0, R.cells, floor, [&](int, const raw (&r)[U][VEC], int64_t i0, bool) {
+        each<F>(r, i0, [&](wide v, int64_t) { const double l = (double)v; if (l >= floor) atomicAdd(&S.bins.count[parts.bin(l)], 1u); });
+      });
+      find_bin<false>(S, 0, 0, 0, (u64)p.top_k, 0.0, 0.0);
+      if (S.found[1] + S.found[2] <= (u64)C::LIST) { upto = (int)S.found[0]; bounded = true; }
+    }
     if (p.top_k <= C::LIST && (bounded || R.n <= C::LIST)) {
       // few: all entries that reach it, if they fit the list -- everything else happens there
       wide quick; bound_below(lo, quick);
       const double floor = lo > cut.value ? lo : cut.value;
-      for_cells<true, C::NT, false>(R, S.best, 0, R.cells, lo, [&](int, const raw (&r)[U][VEC], int64_t i0, bool) {
-#pragma unroll
-        for (int q = 0; q < U; ++q)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const wide v = F::widen(r[q][e]);
-            if (v < quick || !((double)v >= floor) || !((double)v > -INF)) continue;
-            const int at = atomicAdd(&S.listed, 1);
-            if (at < C::LIST) { S.list_value[at] = (double)v; S.list_idx[at] = (uint32_t)(i0 + q * Row<F>::UNIT + e); }
-          }
+      for_cells<true, C::NT>(R, S.best, 0, R.cells, lo, [&](int, const raw (&r)[U][VEC], int64_t i0, bool) {
+        each<F>(r, i0, [&](wide v, int64_t i) {
+          const double l = (double)v;
+          if (v < quick || !(l >= floor) || !(l > -INF)) return;
+          if (upto >= 0 && parts.bin(l) > upto) return;
+          const int at = atomicAdd(&S.listed, 1);
+          if (at < C::LIST) { S.list_value[at] = l; S.list_idx[at] = (uint32_t)i; }
+        });
       });
       __syncthreads();
       const int count = S.listed;
@@ -787,17 +808,13 @@ template <bool WEIGHTED, class F> __global__ __launch_bounds__(All::NT) void k_b
   wide quick; bound_below(lo, quick);
   const int c0 = (int)((int64_t)R.cells * g / shares), c1 = (int)((int64_t)R.cells * (g + 1) / shares);
   for_cells<true, All::NT>(R, S.best, c0, c1, lo, [&](int, const raw (&r)[U][VEC], int64_t i0, bool) {
-#pragma unroll
-    for (int q = 0; q < U; ++q)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const wide v = F::widen(r[q][e]);
-        const double l = (double)v;
-        if (v < quick || !(l >= lo) || !have.keeps(l, i0 + q * Row<F>::UNIT + e)) continue;
-        const int b = parts.bin(l);
-        atomicAdd(&S.bins.count[b], 1u);
-        if (WEIGHTED) { add_weight(S, b, R.weight(l)); __builtin_amdgcn_sched_barrier(0); }
-      }
+    each<F>(r, i0, [&](wide v, int64_t i) {
+      const double l = (double)v;
+      if (v < quick || !(l >= lo) || !have.keeps(l, i)) return;
+      const int b = parts.bin(l);
+      atomicAdd(&S.bins.count[b], 1u);
+      if (WEIGHTED) add_weight(S, b, R.weight(l));
+    });
   });
   __syncthreads();
   Table& T = A.tables[row * 2 + (WEIGHTED ? 1 : 0)];
@@ -831,18 +848,13 @@ template <bool WEIGHTED, class F> __global__ __launch_bounds__(All::NT) void k_l
   const int bin = (int)S.found[0];
   wide quick; bound_below(lo, quick);
   const int c0 = (int)((int64_t)R.cells * g / shares), c1 = (int)((int64_t)R.cells * (g + 1) / shares);
-  for_cells<true, All::NT, false>(R, S.best, c0, c1, lo, [&](int, const raw (&r)[U][VEC], int64_t i0, bool) {
-#pragma unroll
-    for (int q = 0; q < U; ++q)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const wide v = F::widen(r[q][e]);
-        const double l = (double)v;
-        const int64_t i = i0 + q * Row<F>::UNIT + e;
-        if (v < quick || !(l >= lo) || parts.bin(l) != bin || !have.keeps(l, i)) continue;
-        const int at = atomicAdd(&T.listed, 1);
-        T.value[at] = l; T.idx[at] = (uint32_t)i;
-      }
+  for_cells<true, All::NT>(R, S.best, c0, c1, lo, [&](int, const raw (&r)[U][VEC], int64_t i0, bool) {
+    each<F>(r, i0, [&](wide v, int64_t i) {
+      const double l = (double)v;
+      if (v < quick || !(l >= lo) || parts.bin(l) != bin || !have.keeps(l, i)) return;
+      const int at = atomicAdd(&T.listed, 1);
+      T.value[at] = l; T.idx[at] = (uint32_t)i;
+    });
   });
 }
 // ... and the cut of the stage
@@ -902,7 +914,7 @@ Plan plan_of(int type, int64_t rows, int64_t cols, int64_t draws) {
   const int64_t group = type == 0 ? 2 * 128 : type == 1 ? 2 * 256 : 512;
   p.mult = (int)((cols + group * MAX_CELLS - 1) / (group * MAX_CELLS));
   p.max_cells = (int)((cols + group * p.mult - 1) / (group * p.mult));
-  p.build = p.max_cells <= Tiny::CELLS && rows >= 1024 ? 3 : p.max_cells <= (rows >= 512 ? 64 : 16) ? 2 : rows > 512 ? 1 : 0;
+  p.build = p.max_cells <= Tiny::CELLS && rows >= 1024 ? 2 : rows > 512 ? 1 : 0;
   p.groups = (p.build == 0 && p.max_cells >= 32 && rows <= 64) ? (int)std::min<int64_t>(p.max_cells / 8, std::max<int64_t>(1, 512 / rows)) : 0;
   p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(p.max_cells / 16, 256 / rows));      // (of the launches with 16 wavefronts and tables to merge)
   p.draws_here = p.groups == 0 && draws <= 64;
@@ -918,8 +930,7 @@ template <class F> void launch(DrawArgs& A, const Plan& p, int64_t rows, hipStre
   int cuts = 1;
   if (p.groups == 0) {
     const dim3 grid((unsigned)rows);
-    if (p.build == 3) hipLaunchKernelGGL((k_row<Tiny, F>), grid, dim3(Tiny::NT), 0, st, A, p.draws_here ? 1 : 0);
-    else if (p.build == 2) hipLaunchKernelGGL((k_row<Short, F>), grid, dim3(Short::NT), 0, st, A, p.draws_here ? 1 : 0);
+    if (p.build == 2) hipLaunchKernelGGL((k_row<Tiny, F>), grid, dim3(Tiny::NT), 0, st, A, p.draws_here ? 1 : 0);
     else if (p.build == 1) hipLaunchKernelGGL((k_row<Many, F>), grid, dim3(Many::NT), 0, st, A, p.draws_here ? 1 : 0);
     else hipLaunchKernelGGL((k_row<Long, F>), grid, dim3(Long::NT), 0, st, A, p.draws_here ? 1 : 0);
     if (p.draws_here) return;

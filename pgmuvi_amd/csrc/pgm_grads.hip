@@ -289,48 +289,54 @@ template <int TYPE, int THREADS, int KEEP> __global__ __launch_bounds__(THREADS)
   const Table& T = V.T;
   const int64_t b = blockIdx.x;
   Reg v[KEEP];
-  char* to[KEEP];
-  int have[KEEP];                                               // entries of the vector (N, or fewer at a tensor's end; 0: none)
-  bool moved[KEEP];
+  // vector k of this thread: its tensor, first entry and number of entries (fewer than N at a tensor's end; 0: there is none)
+  auto find = [&](int k, int& t, int64_t& i) {
+    const int w = k * THREADS + (int)threadIdx.x;
+    t = 0; i = 0;
+    if (w >= V.first[T.count]) return 0;
+    while (w >= V.first[t + 1]) ++t;
+    i = (int64_t)(w - V.first[t]) * N;
+    const int64_t left = T.e[t].n - i;
+    return left < N ? (int)left : N;
+  };
 #pragma unroll
   for (int k = 0; k < KEEP; ++k) {
-    have[k] = 0; to[k] = nullptr; moved[k] = false;
-    const int w = k * THREADS + (int)threadIdx.x;
-    if (w >= V.first[T.count]) continue;
-    int t = 0;
-    while (w >= V.first[t + 1]) ++t;
-    const Entry& e = T.e[t];
-    const int64_t i = (int64_t)(w - V.first[t]) * N;
-    const char* in = e.in + (b * e.in_stride + i) * S;
-    to[k] = e.out + (b * e.out_stride + i) * S;
-    moved[k] = to[k] != in;
-    if (i + N <= e.n) {
-      have[k] = N;
-      __builtin_memcpy(&v[k], in, 16);
-    } else {
-      have[k] = (int)(e.n - i);
+    int t; int64_t i;
+    const int have = find(k, t, i);
 #pragma unroll
-      for (int j = 0; j < N; ++j) if (j < have[k]) v[k].v[j] = reinterpret_cast<const Reg*>(in)->v[j];
-    }
+    for (int j = 0; j < N; ++j) v[k].set(j, 0.0);
+    if (have == 0) continue;
+    const char* in = T.e[t].in + (b * T.e[t].in_stride + i) * S;
+    if (have == N) __builtin_memcpy(&v[k], in, 16);
+    else
+#pragma unroll
+      for (int j = 0; j < N; ++j) if (j < have) v[k].v[j] = reinterpret_cast<const Reg*>(in)->v[j];
   }
   Acc a{0.0, 0.0, 0.0};
 #pragma unroll
-  for (int k = 0; k < KEEP; ++k)
+  for (int k = 0; k < KEEP; ++k) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) if (j < have[k]) take_p<TYPE>(a, v[k].get(j), T.p);
+    for (int j = 0; j < N; ++j) take_p<TYPE>(a, v[k].get(j), T.p);                            // (zeros add nothing)
+    __builtin_amdgcn_sched_barrier(0);                          // (one vector's conversions at a time: all of them do not fit the registers)
+  }
   const double n = norm_of(block_join<THREADS>(a, T.p, red), T.p);
   if (threadIdx.x == 0) store_norm(norm, norm_f64, b, n);
   if (!scale) return;
   const double c = factor_of(n, max_norm);
 #pragma unroll
   for (int k = 0; k < KEEP; ++k) {
-    if (have[k] == 0 || (c == 1.0 && !moved[k])) continue;
+    int t; int64_t i;
+    const int have = find(k, t, i);
+    if (have == 0) continue;
+    char* out = T.e[t].out + (b * T.e[t].out_stride + i) * S;
+    if (c == 1.0 && out == T.e[t].in + (b * T.e[t].in_stride + i) * S) continue;              // (nothing to change: times one)
 #pragma unroll
     for (int j = 0; j < N; ++j) v[k].set(j, v[k].get(j) * c);
-    if (have[k] == N) __builtin_memcpy(to[k], &v[k], 16);
+    if (have == N) __builtin_memcpy(out, &v[k], 16);
     else
 #pragma unroll
-      for (int j = 0; j < N; ++j) if (j < have[k]) reinterpret_cast<Reg*>(to[k])->v[j] = v[k].v[j];
+      for (int j = 0; j < N; ++j) if (j < have) reinterpret_cast<Reg*>(out)->v[j] = v[k].v[j];
+    __builtin_amdgcn_sched_barrier(0);
   }
 }
 
@@ -467,14 +473,14 @@ int run_clip(int batch, int count, const uint64_t* in, const uint64_t* out, cons
     bool same = true;
     int64_t vectors = 0;
     for (const Item& it : flat) { same = same && it.type == flat[0].type; vectors += (it.bytes + 15) / 16; }
-    constexpr int SMALL = NT, LARGE = 1024, FEW = 4, KEEP = 8;
+    constexpr int SMALL = NT, LARGE = 512, FEW = 4, KEEP = 12;
     if (!flat.empty() && same && vectors <= KEEP * LARGE) {
       VectorTable V;
       fill(V.T, 0, flat.size());
       int at = 0;
       for (size_t i = 0; i < flat.size(); ++i) { V.first[i] = at; at += (int)((flat[i].bytes + 15) / 16); }
       V.first[flat.size()] = at;
-      // (256 threads while four vectors each cover the member, so that 8 members share a CU; else 1024 with up to eight)
+      // (256 threads while four vectors each cover the member, so that 8 members share a CU; else 512 with up to twelve)
 #define PGM_CALL(TY) do { if (vectors <= FEW * SMALL) hipLaunchKernelGGL((k_member_kept<TY, SMALL, FEW>), dim3(batch), dim3(SMALL), 0, st, V, scale, max_norm, norm, norm_f64); \
                           else hipLaunchKernelGGL((k_member_kept<TY, LARGE, KEEP>), dim3(batch), dim3(LARGE), 0, st, V, scale, max_norm, norm, norm_f64); } while (0)
       PGM_BY_TYPE(flat[0].type, PGM_CALL)

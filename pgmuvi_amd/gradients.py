@@ -58,7 +58,7 @@ def _describe(tensors, outs, batch):
     T = torch.Tensor
     numel = array("q", map(T.numel, tensors))
     kinds = {t.dtype for t in tensors}
-    types = bytearray([_TYPE[kinds.pop()]]) * len(tensors) if len(kinds) == 1 else bytearray(_TYPE[t.dtype] for t in tensors)
+    types = bytearray(_TYPE[k] for k in kinds) * len(tensors) if len(kinds) == 1 else bytearray(_TYPE[t.dtype] for t in tensors)
     src = array("Q", map(T.data_ptr, tensors))
     dst = src if outs is tensors else None if outs is None else array("Q", map(T.data_ptr, outs))
     member = layout = None
@@ -89,16 +89,21 @@ def _describe(tensors, outs, batch):
     return src, dst, numel, types, member, layout
 
 
+def _sparse(t):
+    return t.layout is not torch.strided
+
+
 _PLAIN = {torch.Tensor, torch.nn.Parameter}
 
 
 def _tensors(tensors, what):
+    """The tensors as a list, checked: dense, of the four types, on one GPU."""
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
     if not _PLAIN.issuperset(map(type, tensors)):
         for t in tensors:
             if not torch.is_tensor(t):
                 raise TypeError(f"{what}: tensors expected, got {type(t).__name__}")
-    if not _TYPE.keys() >= {t.dtype for t in tensors} or not {torch.strided} >= {t.layout for t in tensors}:
+    if any(map(_sparse, tensors)) or not _TYPE.keys() >= {t.dtype for t in tensors}:
         raise TypeError(f"{what}: dense float64, float32, bfloat16 or float16 tensors expected, got "
                         f"{sorted({str(t.dtype) + ' ' + str(t.layout) for t in tensors})}")
     if tensors:
@@ -126,11 +131,11 @@ def _run(tensors, outs, max_norm, norm_type, members, what):
             raise ValueError(f"{what}: with members=True every tensor needs the same leading size, got {[tuple(t.shape) for t in tensors]}")
         batch = tensors[0].shape[0]
     dev = tensors[0].device
-    f64 = any(t.dtype is torch.float64 for t in tensors)
-    norm = torch.empty(() if batch is None else (batch,), dtype=torch.float64 if f64 else torch.float32, device=dev)
     if batch == 0:
-        return norm
+        return torch.empty(0, dtype=torch.float64 if any(t.dtype is torch.float64 for t in tensors) else torch.float32, device=dev)
     src, dst, numel, types, member, layout = _describe(tensors, outs, batch)
+    f64 = 0 in types
+    norm = torch.empty(() if batch is None else (batch,), dtype=torch.float64 if f64 else torch.float32, device=dev)
     lib = _hip.load()
     members, count = batch or 1, len(tensors)
     same = types.count(types[0]) == count

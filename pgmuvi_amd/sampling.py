@@ -20,6 +20,8 @@ _TYPE = {torch.float64: 0, torch.float32: 1, torch.bfloat16: 2, torch.float16: 3
 
 def _setting(value, off, lo, hi, name, rows, dev, dtype):
     """(scalar, device pointer or None, tensor kept alive) of a truncation argument: a number for all rows, or one per row."""
+    if value is None:
+        return off, None, None
     if torch.is_tensor(value) and value.dim() > 0:
         if tuple(value.shape) != (rows,):
             raise ValueError(f"draw_indices: {name} must be a number or one per row ({rows}), got {tuple(value.shape)}")
@@ -28,8 +30,6 @@ def _setting(value, off, lo, hi, name, rows, dev, dtype):
             raise TypeError(f"draw_indices: {name} takes whole numbers")
         t = value.detach().to(device=dev, dtype=dtype).contiguous()
         return off, t.data_ptr(), t
-    if value is None:
-        return off, None, None
     number = int(value) if dtype is torch.int64 else float(value)
     if not lo <= number <= hi or (dtype is torch.int64 and number != value):
         raise ValueError(f"draw_indices: {name} must be in [{lo}, {hi}], got {value}")
@@ -61,11 +61,11 @@ def draw_indices(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=N
     single = logits.dim() == 1
     if logits.dim() not in (1, 2):
         raise ValueError(f"draw_indices: logits must be (B, V) or (V,), got {tuple(logits.shape)}")
-    l = logits.detach().unsqueeze(0) if single else logits.detach()
-    B, V = l.shape
+    B, V = (1, logits.shape[0]) if single else logits.shape
+    row_stride, col_stride = (0, logits.stride(0)) if single else logits.stride()
     if u.dim() > 2 - single or (not single and (u.dim() == 0 or u.shape[0] != B)):
         raise ValueError(f"draw_indices: u must be {'(S,) or ()' if single else f'({B}, S) or ({B},)'}, got {tuple(u.shape)}")
-    ud = u.detach().to(torch.float64).contiguous()
+    ud = u if u.dtype is torch.float64 and u.is_contiguous() else u.detach().to(torch.float64).contiguous()
     S = ud.numel() // B if B else 0
     settings = [_setting(temperature, 1.0, 0.0, 1e300, "temperature", B, dev, torch.float64),
                 _setting(top_k, 0, 1, (1 << 62), "top_k", B, dev, torch.int64),
@@ -88,12 +88,12 @@ def draw_indices(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=N
         if V >= 1 << 24:
             raise ValueError(f"draw_indices: rows of at most {(1 << 24) - 1} entries, got {V}")
         (t, tp, _t), (k, kp, _k), (p, pp, _p), (m, mp, _m) = settings
-        lib, kind = _hip.load(), _TYPE[l.dtype]
+        lib, kind = _hip.load(), _TYPE[logits.dtype]
         n = int(lib.pgm_draw_scratch_doubles(kind, B, V, S))
         scratch = torch.empty(n, dtype=torch.float64, device=dev) if n else None
-        with torch.cuda.device(dev):
-            rc = lib.pgm_draw_indices(l.data_ptr(), kind, B, V, l.stride(0), l.stride(1), None if ln is None else ln.data_ptr(),
+        with _hip.on_device(dev.index):
+            rc = lib.pgm_draw_indices(logits.data_ptr(), kind, B, V, row_stride, col_stride, None if ln is None else ln.data_ptr(),
                                       ud.data_ptr(), S, t, tp, k, kp, p, pp, m, mp, index.data_ptr(), None if logp is None else logp.data_ptr(),
-                                      None if scratch is None else scratch.data_ptr(), n, _hip.current_stream_ptr(dev))
+                                      None if scratch is None else scratch.data_ptr(), n, _hip.stream_of(dev.index))
         _hip._check(rc, "pgm_draw_indices")
     return (index, logp) if return_logprob else index
