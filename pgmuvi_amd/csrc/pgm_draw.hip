@@ -138,7 +138,11 @@ __device__ __forceinline__ double mass_of(u64 hi, u64 lo) { return (double)hi * 
 template <class F> struct Row {
   typedef typename F::raw raw;
   static constexpr int U = F::U, VEC = LOAD / (int)sizeof(raw), UNIT = 64 * VEC;       // entries of one load of a lane, of a wavefront
-  const raw* x; int64_t stride, n;
+  // (global memory by type: through a generic pointer the loads would count as LDS accesses as well, and every wait for the LDS would
+  // hold up the loads in flight)
+  typedef const __attribute__((address_space(1))) raw* Global;
+  typedef raw Lot __attribute__((ext_vector_type(VEC), aligned(sizeof(raw))));
+  Global x; int64_t stride, n;
   int mult, cells;
   double best, t, per_t;                                        // highest value, temperature, 1 / temperature
   __device__ __forceinline__ int64_t width() const { return (int64_t)mult * (U * UNIT); }
@@ -150,7 +154,11 @@ template <class F> struct Row {
   __device__ __forceinline__ int64_t first(int64_t g) const { return g * (U * UNIT) + (threadIdx.x & 63) * VEC; }
   __device__ __forceinline__ void load_whole(int64_t g, raw (&r)[U][VEC]) const {
 #pragma unroll
-    for (int q = 0; q < U; ++q) __builtin_memcpy(r[q], x + first(g) + q * UNIT, LOAD);
+    for (int q = 0; q < U; ++q) {
+      const Lot v = *reinterpret_cast<const __attribute__((address_space(1))) Lot*>(x + first(g) + q * UNIT);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) r[q][e] = v[e];
+    }
   }
   __device__ __forceinline__ void load_part(int64_t g, raw (&r)[U][VEC]) const {
 #pragma unroll
@@ -318,7 +326,10 @@ struct Even {                                                   // the first bin
   __device__ __forceinline__ Even(double best_, double lo, int bins_) : best(best_), scale(bins_ / (best_ - lo)), bins(bins_) { good = best - lo > 0.0 && best - lo < 1e300 && scale < 1e300; }
   __device__ __forceinline__ int bin(double l) const { const int b = (int)((best - l) * scale); return b < bins ? b : bins - 1; }
 };
-template <bool WEIGHTED, bool SEEDED, class C, class F> __device__ Cut select(const Row<F>& R, Shared<C>& S, double lo, Cut have, u64 want, double share) {
+// `summed` (WEIGHTED; may be null): where the first bin is short enough, the pass that collects its entries also forms the cells' kept
+// weights (S.cells; of entries with a weight of at least min_p), and says so
+template <bool WEIGHTED, bool SEEDED, class C, class F> __device__ __forceinline__ Cut select(const Row<F>& R, Shared<C>& S, double lo, Cut have, u64 want, double share,
+                                                                             double min_p = 0.0, bool* summed = nullptr) {
   typedef typename F::raw raw;
   typedef typename F::wide wide;
   constexpr int VEC = Row<F>::VEC, U = F::U, BINS = Shared<C>::BINS;
@@ -359,7 +370,26 @@ template <bool WEIGHTED, bool SEEDED, class C, class F> __device__ Cut select(co
     bn = S.found[1]; bhi = S.found[3]; blo = S.found[4]; target = __longlong_as_double((long long)S.found[5]);
     if (in_bin <= (u64)C::LIST) {
       // few enough to sort: the bin's entries in the cut's order, then the first that reaches the goal
-      if (!seeded)
+      const bool sums = WEIGHTED && !SEEDED && summed && even;
+      if (sums) {
+        // (no entry of this bin or a higher one is below this; the bins' place is free)
+        const double least = bin + 1 < BINS ? R.best - (bin + 1.001) / parts.scale : lo;
+        for (int c = threadIdx.x; c < R.cells; c += C::NT) if (!(S.best[c] >= least)) S.cells[c] = 0.0;
+        double w = 0.0;
+        for_cells<true, C::NT>(R, S.best, 0, R.cells, least, [&](int c, const raw (&r)[U][VEC], int64_t i0, bool last) {
+          each<F>(r, i0, [&](wide v, int64_t i) {
+            const double l = (double)v;
+            if (!(l >= lo) || !have.keeps(l, i)) return;
+            const int b = parts.bin(l);
+            if (b < bin) { const double x = R.weight(l); w += x < min_p ? 0.0 : x; }
+            if (b == bin) { const int at = atomicAdd(&S.listed, 1); S.list_value[at] = l; S.list_idx[at] = (uint32_t)i; }
+          });
+          if (!last) return;
+          const double total = wave_sum(w);
+          w = 0.0;
+          if ((threadIdx.x & 63) == 0) S.cells[c] = total;
+        });
+      } else if (!seeded)
         entries([&](double l, int64_t i, int b) {
           if (b != bin) return;
           const int at = atomicAdd(&S.listed, 1);
@@ -372,7 +402,24 @@ template <bool WEIGHTED, bool SEEDED, class C, class F> __device__ Cut select(co
         const double sum = block_scan<C::NT>(S.red, t < count ? R.weight(S.list_value[t]) : 0.0);
         at = (int)block_min<C::NT>(S.red, t < count && mass_of(bhi, blo) + sum >= target ? (double)t : (double)(count - 1));
       }
-      return Cut{S.list_value[at], (int64_t)S.list_idx[at]};
+      const Cut cut{S.list_value[at], (int64_t)S.list_idx[at]};
+      if (sums) {
+        // the kept entries of the bin join their cells, one thread per cell and in the list's order
+        __syncthreads();
+        if (t < count) {
+          const double w = R.weight(S.list_value[t]);
+          S.list_value[t] = t <= at && w >= min_p ? w : 0.0;
+          S.list_idx[t] = (uint32_t)((int64_t)S.list_idx[t] / R.width());
+        }
+        __syncthreads();
+        for (int c = t; c < R.cells; c += C::NT) {
+          double w = S.cells[c];
+          for (int j = 0; j <= at; ++j) w += S.list_idx[j] == (uint32_t)c ? S.list_value[j] : 0.0;
+          S.cells[c] = w;
+        }
+        *summed = true;
+      }
+      return cut;
     }
     double high = -INF, low = INF;                              // the range of the bin's values
     entries([&](double l, int64_t, int b) { if (b == bin) { high = l > high ? l : high; low = l < low ? l : low; } });
@@ -432,7 +479,7 @@ template <class F> __device__ __forceinline__ Row<F> row_of(const DrawArgs& A, i
   Row<F> R;
   int64_t n = A.cols;
   if (A.lengths) { n = A.lengths[row]; n = n < 0 ? 0 : n > A.cols ? A.cols : n; }
-  R.x = static_cast<const typename F::raw*>(A.logits) + row * A.row_stride; R.stride = A.col_stride; R.n = n;
+  R.x = (typename Row<F>::Global)static_cast<const typename F::raw*>(A.logits) + row * A.row_stride; R.stride = A.col_stride; R.n = n;
   R.mult = A.mult;
   R.cells = (int)((n + R.width() - 1) / R.width());
   R.best = 0.0; R.t = t; R.per_t = 1.0 / t;
@@ -666,13 +713,14 @@ template <class F> __device__ __forceinline__ double bound_of_top_p(const Row<F>
 }
 __device__ __forceinline__ double finite_lowest(double v) { return v > -1.7976931348623157e308 ? v : -1.7976931348623157e308; }
 // The cut of a row whose cells' highest values are in S.best; R.best is set; `lowest` of the row where wants_lowest asked for it, else
-// -inf.  listed > 0: the list holds exactly the kept entries
-template <class C, class F> __device__ Cut cut_of(const Row<F>& R, Shared<C>& S, const Settings& p, double lowest, int& listed) {
+// -inf.  listed > 0: the list holds exactly the kept entries; summed: S.cells the cells' kept weights
+template <class C, class F> __device__ __forceinline__ Cut cut_of(const Row<F>& R, Shared<C>& S, const Settings& p, double lowest, int& listed, bool& summed) {
   typedef typename F::raw raw;
   typedef typename F::wide wide;
   constexpr int VEC = Row<F>::VEC, U = F::U;
   Cut cut = everything(R.best);
   listed = 0;
+  summed = false;
   lowest = finite_lowest(lowest);
   if (p.top_k > 0) {
     bool bounded;
@@ -711,7 +759,7 @@ template <class C, class F> __device__ Cut cut_of(const Row<F>& R, Shared<C>& S,
     }
     cut = tighter(cut, select<false, false, C, F>(R, S, lo, cut, (u64)p.top_k, 0.0));
   }
-  if (p.top_p < 1.0) cut = tighter(cut, select<true, false, C, F>(R, S, bound_of_top_p(R, lowest, cut), cut, 0, p.top_p));
+  if (p.top_p < 1.0) cut = tighter(cut, select<true, false, C, F>(R, S, bound_of_top_p(R, lowest, cut), cut, 0, p.top_p, p.min_p, &summed));
   return cut;
 }
 
@@ -733,10 +781,11 @@ template <class C, class F> __global__ __launch_bounds__(C::NT) __attribute__((a
   if (R.best > -INF) {
     if (!p.plain) {
       int listed;
-      cut = cut_of<C, F>(R, S, p, lowest ? block_min<C::NT>(S.red, low) : -INF, listed);
+      bool summed;
+      cut = cut_of<C, F>(R, S, p, lowest ? block_min<C::NT>(S.red, low) : -INF, listed, summed);
       if (listed && draws_here) { draw_list<C, F>(A, R, S, row, listed); return; }
       __syncthreads();                                          // (the cells take the bins' place)
-      pass_weights<C::NT, F>(R, S.best, 0, R.cells, cut, p.min_p, S.cells);
+      if (!summed) pass_weights<C::NT, F>(R, S.best, 0, R.cells, cut, p.min_p, S.cells);
     } else if (draws_here) {
       for (int c = threadIdx.x; c < R.cells; c += C::NT) S.cells[c] *= cell_factor(R, S.best[c]);
     }
