@@ -308,6 +308,36 @@ template <class C> __device__ __forceinline__ void sort_list(Shared<C>& S, int c
   if (t < count) { S.list_value[rank] = value; S.list_idx[rank] = idx; }
   __syncthreads();
 }
+// The same where the bins hold the counts of the listed entries (bin(value) of theirs): by bins first, then each entry counts what is
+// ahead of it in its own bin (512 entries of a 16-bit type, many of them equal: 21 -> 4 us)
+template <class C, class Bin> __device__ __forceinline__ void sort_list_by_bins(Shared<C>& S, int count, Bin bin) {
+  constexpr int PER = Shared<C>::BINS / C::NT;
+  uint32_t* start = reinterpret_cast<uint32_t*>(S.bins.hi);      // entries before each bin
+  uint32_t* taken = reinterpret_cast<uint32_t*>(S.bins.lo);
+  const int t = threadIdx.x, b0 = t * PER;
+  __syncthreads();
+  uint32_t n = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) n += S.bins.count[b0 + k];
+  uint32_t before = (uint32_t)block_scan<C::NT>(S.red, (double)n) - n;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) { start[b0 + k] = before; taken[b0 + k] = 0; before += S.bins.count[b0 + k]; }
+  double value = 0.0; uint32_t idx = 0; int b = 0;
+  if (t < count) { value = S.list_value[t]; idx = S.list_idx[t]; b = bin(value); }
+  __syncthreads();
+  if (t < count) { const uint32_t at = start[b] + atomicAdd(&taken[b], 1u); S.list_value[at] = value; S.list_idx[at] = idx; }
+  __syncthreads();
+  int rank = 0;
+  if (t < count) {                                              // (the entry that came to place t)
+    value = S.list_value[t]; idx = S.list_idx[t]; b = bin(value);
+    const int from = (int)start[b], to = from + (int)S.bins.count[b];
+    rank = from;
+    for (int j = from; j < to; ++j) { const double v = S.list_value[j]; rank += v > value || (v == value && S.list_idx[j] < idx); }
+  }
+  __syncthreads();
+  if (t < count) { S.list_value[rank] = value; S.list_idx[rank] = idx; }
+  __syncthreads();
+}
 // adds a weight to a bin: 2^-40 steps in one word, 2^-80 steps in the other (the magic number 2^52 leaves the rounded integer in the
 // low bits of a sum)
 template <class C> __device__ __forceinline__ void add_weight(Shared<C>& S, int b, double w) {
@@ -650,10 +680,9 @@ __device__ __forceinline__ void draw_nothing(const DrawArgs& A, int64_t row, int
     if (A.logp) A.logp[row * A.draws + s] = -INF;
   }
 }
-// All truncations on a list that holds the row's first top_k entries: sorts it and returns how many are kept (the first ones)
+// All truncations on a sorted list that holds the row's first top_k entries: how many are kept (the first ones)
 template <class C, class F> __device__ __forceinline__ int keep_list(const Row<F>& R, Shared<C>& S, const Settings& p, int count) {
   const int t = threadIdx.x;
-  sort_list(S, count);
   int n = p.top_k < count ? (int)p.top_k : count;
   const double w = t < n ? R.weight(S.list_value[t]) : 0.0;
   const double sum = block_scan<C::NT>(S.red, w);
@@ -728,7 +757,7 @@ template <class C, class F> __device__ __forceinline__ Cut cut_of(const Row<F>& 
     __syncthreads();
     int upto = -1;                                              // (bins the list takes; -1: everything from the bound on)
     const Even parts(R.best, lo > cut.value ? lo : cut.value, Shared<C>::BINS);
-    if (p.top_k <= C::LIST && !bounded && R.n > C::LIST && parts.good) {
+    if (p.top_k <= C::LIST && !bounded && R.n > 64 && parts.good) {
       // no bound from the cells: from bins over all entries
       const double floor = lo > cut.value ? lo : cut.value;
       for_cells<true, C::NT>(R, S.best, 0, R.cells, floor, [&](int, const raw (&r)[U][VEC], int64_t i0, bool) {
@@ -753,6 +782,7 @@ template <class C, class F> __device__ __forceinline__ Cut cut_of(const Row<F>& 
       __syncthreads();
       const int count = S.listed;
       if (count <= C::LIST) {
+        if (upto >= 0) sort_list_by_bins(S, count, [&](double l) { return parts.bin(l); }); else sort_list(S, count);
         listed = keep_list<C, F>(R, S, p, count);
         return Cut{S.list_value[listed - 1], (int64_t)S.list_idx[listed - 1]};
       }
@@ -763,6 +793,49 @@ template <class C, class F> __device__ __forceinline__ Cut cut_of(const Row<F>& 
   return cut;
 }
 
+// A row of one wavefront's build: running sums lane by lane (PER neighbouring entries each) in LDS, then one lane per draw
+template <class C, class F> __device__ __forceinline__ void draw_tiny(const DrawArgs& A, const Row<F>& R, Shared<C>& S, int64_t row, const Cut& cut, double min_p) {
+  constexpr int PER = F::U * Row<F>::VEC;
+  static_assert(C::NT == 64 && C::CELLS * 64 <= 2 * Shared<C>::BINS, "running sums in the bins' place");
+  double* run = reinterpret_cast<double*>(S.bins.hi);            // (hi and lo)
+  const int lane = threadIdx.x;
+  auto weight = [&](int64_t i) {
+    if (i >= R.n) return 0.0;
+    const double l = R.value(i);
+    if (!(l > -INF) || !cut.keeps(l, i)) return 0.0;
+    const double w = R.weight(l);
+    return w < min_p ? 0.0 : w;
+  };
+  const int lots = (int)((R.n + PER - 1) / PER), rounds = (lots + 63) / 64;
+  double base = 0.0;
+  __syncthreads();
+  for (int c = 0; c < rounds; ++c) {
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) sum += weight((int64_t)(c * 64 + lane) * PER + e);
+    const double inc = wave_scan(sum);
+    run[c * 64 + lane] = base + inc;
+    base += __shfl(inc, 63);
+  }
+  __syncthreads();
+  const double Z = run[lots - 1], log_z = log(Z);
+  for (int64_t s = lane; s < A.draws; s += 64) {
+    double target = target_of(A.u[row * A.draws + s], Z);
+    int j = first_above(run, lots, target, false);
+    if (j == lots) { j = first_above(run, lots, Z, true); target = INF; }
+    double r = j ? run[j - 1] : 0.0;
+    int64_t found = -1;
+    for (int e = 0; e < PER; ++e) {
+      const int64_t i = (int64_t)j * PER + e;
+      const double w = weight(i);
+      r += w;
+      if (w > 0.0) { found = i; if (r > target) break; }        // (else its last kept one: the sums differ by a rounding)
+    }
+    A.index[row * A.draws + s] = found;
+    if (A.logp) A.logp[row * A.draws + s] = R.z(R.value(found)) - log_z;
+  }
+}
+
 // ---- kernels --------------------------------------------------------------------------------------------------------------------------
 // One workgroup per row: everything, or (draws_here 0: many draws per row) all but the draws, which k_draws makes from memory
 template <class C, class F> __global__ __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(4))) void k_row(DrawArgs A, int draws_here) {
@@ -771,8 +844,10 @@ template <class C, class F> __global__ __launch_bounds__(C::NT) __attribute__((a
   const Settings p = settings_of(A, row);
   Row<F> R = row_of<F>(A, row, p.t);
   const bool lowest = wants_lowest(p, R.cells);
-  const double low = p.plain ? pass_best<C::NT, true, F>(R, 0, R.cells, S.best, S.cells, false)
-                             : pass_best<C::NT, false, F>(R, 0, R.cells, S.best, nullptr, lowest);
+  constexpr bool TINY = C::NT == 64;
+  const bool plain = p.plain && !(TINY && draws_here);
+  const double low = plain ? pass_best<C::NT, true, F>(R, 0, R.cells, S.best, S.cells, false)
+                           : pass_best<C::NT, false, F>(R, 0, R.cells, S.best, nullptr, lowest);
   __syncthreads();
   double top = -INF;
   for (int c = threadIdx.x; c < R.cells; c += C::NT) top = S.best[c] > top ? S.best[c] : top;
@@ -784,8 +859,12 @@ template <class C, class F> __global__ __launch_bounds__(C::NT) __attribute__((a
       bool summed;
       cut = cut_of<C, F>(R, S, p, lowest ? block_min<C::NT>(S.red, low) : -INF, listed, summed);
       if (listed && draws_here) { draw_list<C, F>(A, R, S, row, listed); return; }
+      if constexpr (TINY) if (draws_here) { draw_tiny<C, F>(A, R, S, row, cut, p.min_p); return; }
       __syncthreads();                                          // (the cells take the bins' place)
       if (!summed) pass_weights<C::NT, F>(R, S.best, 0, R.cells, cut, p.min_p, S.cells);
+    } else if (TINY && draws_here) {
+      if constexpr (TINY) draw_tiny<C, F>(A, R, S, row, cut, 0.0);
+      return;
     } else if (draws_here) {
       for (int c = threadIdx.x; c < R.cells; c += C::NT) S.cells[c] *= cell_factor(R, S.best[c]);
     }
