@@ -277,65 +277,57 @@ template <int THREADS> __global__ __launch_bounds__(THREADS) void k_member(Table
   }
 }
 
-// The same for members of one type and at most KEEP 16-byte vectors per thread: they stay in registers between the norm and the
-// scaling, so that every gradient is read once (from the cache a second time, 4096 members of 64 KB took 188 us).  Vector
-// k THREADS + thread of the member; `first`: number of the tensors' first vectors
-struct VectorTable { Table T; int first[TABLE + 1]; };
-static_assert(sizeof(VectorTable) <= 3900, "kernel arguments");
-template <int TYPE, int THREADS, int KEEP> __global__ __launch_bounds__(THREADS) void k_member_kept(VectorTable V, int scale, double max_norm, void* norm, int norm_f64) {
+// The same for members of one type that fit the workgroup's registers: KEEP slots of one 16-byte vector per thread, each slot a stretch
+// of one tensor.  The entries stay there between the norm and the scaling, so that every gradient is read once (4096 members of
+// 64 KB: 188 us with a second pass through the cache).  Which tensor a slot belongs to is the host's arithmetic: a lookup per vector
+// in the table of tensors held up the loads (175 us)
+constexpr int SLOTS = 12;
+struct Slot { const char* in; char* out; int64_t n, in_stride, out_stride, first; };
+struct SlotTable { int count, p; Slot s[SLOTS]; };
+template <int TYPE, int THREADS, int KEEP> __global__ __launch_bounds__(THREADS) void k_member_kept(SlotTable V, int scale, double max_norm, void* norm, int norm_f64) {
   typedef Vec<TYPE> Reg;
   constexpr int N = Reg::N, S = type_bytes(TYPE);
+  static_assert(KEEP <= SLOTS, "slots");
   __shared__ Acc red[THREADS / 64];
-  const Table& T = V.T;
   const int64_t b = blockIdx.x;
   Reg v[KEEP];
-  // vector k of this thread: its tensor, first entry and number of entries (fewer than N at a tensor's end; 0: there is none)
-  auto find = [&](int k, int& t, int64_t& i) {
-    const int w = k * THREADS + (int)threadIdx.x;
-    t = 0; i = 0;
-    if (w >= V.first[T.count]) return 0;
-    while (w >= V.first[t + 1]) ++t;
-    i = (int64_t)(w - V.first[t]) * N;
-    const int64_t left = T.e[t].n - i;
-    return left < N ? (int)left : N;
-  };
 #pragma unroll
   for (int k = 0; k < KEEP; ++k) {
-    int t; int64_t i;
-    const int have = find(k, t, i);
 #pragma unroll
     for (int j = 0; j < N; ++j) v[k].set(j, 0.0);
-    if (have == 0) continue;
-    const char* in = T.e[t].in + (b * T.e[t].in_stride + i) * S;
-    if (have == N) __builtin_memcpy(&v[k], in, 16);
+    if (k >= V.count) continue;
+    const Slot& e = V.s[k];
+    const int64_t i = e.first + (int64_t)threadIdx.x * N;
+    const char* in = e.in + (b * e.in_stride + i) * S;
+    if (i + N <= e.n) __builtin_memcpy(&v[k], in, 16);
     else
 #pragma unroll
-      for (int j = 0; j < N; ++j) if (j < have) v[k].v[j] = reinterpret_cast<const Reg*>(in)->v[j];
+      for (int j = 0; j < N; ++j) if (i + j < e.n) v[k].v[j] = reinterpret_cast<const Reg*>(in)->v[j];
   }
   Acc a{0.0, 0.0, 0.0};
 #pragma unroll
   for (int k = 0; k < KEEP; ++k) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) take_p<TYPE>(a, v[k].get(j), T.p);                            // (zeros add nothing)
+    for (int j = 0; j < N; ++j) take_p<TYPE>(a, v[k].get(j), V.p);                            // (zeros add nothing)
     __builtin_amdgcn_sched_barrier(0);                          // (one vector's conversions at a time: all of them do not fit the registers)
   }
-  const double n = norm_of(block_join<THREADS>(a, T.p, red), T.p);
+  const double n = norm_of(block_join<THREADS>(a, V.p, red), V.p);
   if (threadIdx.x == 0) store_norm(norm, norm_f64, b, n);
   if (!scale) return;
   const double c = factor_of(n, max_norm);
 #pragma unroll
   for (int k = 0; k < KEEP; ++k) {
-    int t; int64_t i;
-    const int have = find(k, t, i);
-    if (have == 0) continue;
-    char* out = T.e[t].out + (b * T.e[t].out_stride + i) * S;
-    if (c == 1.0 && out == T.e[t].in + (b * T.e[t].in_stride + i) * S) continue;              // (nothing to change: times one)
+    if (k >= V.count) continue;
+    const Slot& e = V.s[k];
+    const int64_t i = e.first + (int64_t)threadIdx.x * N;
+    char* out = e.out + (b * e.out_stride + i) * S;
+    if (c == 1.0 && out == e.in + (b * e.in_stride + i) * S) continue;                        // (nothing to change: times one)
 #pragma unroll
     for (int j = 0; j < N; ++j) v[k].set(j, v[k].get(j) * c);
-    if (have == N) __builtin_memcpy(out, &v[k], 16);
+    if (i + N <= e.n) __builtin_memcpy(out, &v[k], 16);
     else
 #pragma unroll
-      for (int j = 0; j < N; ++j) if (j < have) reinterpret_cast<Reg*>(out)->v[j] = v[k].v[j];
+      for (int j = 0; j < N; ++j) if (i + j < e.n) reinterpret_cast<Reg*>(out)->v[j] = v[k].v[j];
     __builtin_amdgcn_sched_barrier(0);
   }
 }
@@ -407,9 +399,11 @@ bool any_clash(std::vector<Span>& v) {
 
 struct Item { int type; int64_t n; const char* in; char* out; int64_t in_member, out_member; const int64_t* layout; int64_t bytes, chunks; };
 
-// One workgroup per member, in one launch: a small set (one CU streams 64 KB in the time a second launch takes), or members enough
-// to fill the chip with whole workgroups
-bool one_launch(int batch, int64_t count, int64_t bytes, bool strided) { return !strided && count <= TABLE && (bytes <= 65536 || batch >= 512); }
+// One workgroup per member, in one launch: a small set of few tensors (one CU streams 64 KB in the time a second launch takes; more
+// tensors, one after the other, take longer than two launches), or members enough to fill the chip with whole workgroups
+bool one_launch(int batch, int64_t count, int64_t bytes, bool strided) {
+  return !strided && ((count <= 8 && bytes <= 65536) || (count <= TABLE && batch >= 512));
+}
 
 int run_clip(int batch, int count, const uint64_t* in, const uint64_t* out, const int64_t* numel, const unsigned char* type,
              const int64_t* member, const int64_t* layout, int p, double max_norm, void* norm, int norm_f64, double* scratch,
@@ -469,20 +463,25 @@ int run_clip(int batch, int count, const uint64_t* in, const uint64_t* out, cons
     }
     T.chunks = (int)c;
   };
-  if (one_launch(batch, (int64_t)flat.size(), per_member, !loose.empty())) {
+  if (one_launch(batch, count, per_member, layout != nullptr)) {
+    // slots of 256 threads while eight of them cover the member (8 members share a CU), else of 512 while twelve do
+    constexpr int SMALL = 256, FEW = 8, LARGE = 512;
+    auto slots = [&](int threads) {
+      int64_t n = 0;
+      for (const Item& it : flat) n += (it.bytes + 16 * threads - 1) / (16 * threads);
+      return n;
+    };
     bool same = true;
-    int64_t vectors = 0;
-    for (const Item& it : flat) { same = same && it.type == flat[0].type; vectors += (it.bytes + 15) / 16; }
-    constexpr int SMALL = NT, LARGE = 512, FEW = 4, KEEP = 12;
-    if (!flat.empty() && same && vectors <= KEEP * LARGE) {
-      VectorTable V;
-      fill(V.T, 0, flat.size());
-      int at = 0;
-      for (size_t i = 0; i < flat.size(); ++i) { V.first[i] = at; at += (int)((flat[i].bytes + 15) / 16); }
-      V.first[flat.size()] = at;
-      // (256 threads while four vectors each cover the member, so that 8 members share a CU; else 512 with up to twelve)
-#define PGM_CALL(TY) do { if (vectors <= FEW * SMALL) hipLaunchKernelGGL((k_member_kept<TY, SMALL, FEW>), dim3(batch), dim3(SMALL), 0, st, V, scale, max_norm, norm, norm_f64); \
-                          else hipLaunchKernelGGL((k_member_kept<TY, LARGE, KEEP>), dim3(batch), dim3(LARGE), 0, st, V, scale, max_norm, norm, norm_f64); } while (0)
+    for (const Item& it : flat) same = same && it.type == flat[0].type;
+    const int threads = slots(SMALL) <= FEW ? SMALL : slots(LARGE) <= SLOTS ? LARGE : 0;
+    if (!flat.empty() && same && threads) {
+      SlotTable V;
+      V.count = 0; V.p = p;
+      for (const Item& it : flat)
+        for (int64_t i = 0; i < it.n; i += (int64_t)threads * (16 / type_bytes(it.type)))
+          V.s[V.count++] = Slot{it.in, it.out, it.n, it.in_member, it.out_member, i};
+#define PGM_CALL(TY) do { if (threads == SMALL) hipLaunchKernelGGL((k_member_kept<TY, SMALL, FEW>), dim3(batch), dim3(SMALL), 0, st, V, scale, max_norm, norm, norm_f64); \
+                          else hipLaunchKernelGGL((k_member_kept<TY, LARGE, SLOTS>), dim3(batch), dim3(LARGE), 0, st, V, scale, max_norm, norm, norm_f64); } while (0)
       PGM_BY_TYPE(flat[0].type, PGM_CALL)
 #undef PGM_CALL
     } else {
