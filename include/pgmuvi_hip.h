@@ -224,7 +224,7 @@ int pgm_fit_create(pgm_fit** out, pgm_ws* ws, const double* x, const double* y, 
                    int optimizer, double lr, double beta1, double beta2, double eps, double weight_decay, int max_iter);
 int pgm_fit_set_priors(pgm_fit* fit, const int* kind, const double* loc, const double* scale);
 /* The step's gradient (with respect to the raw vector, priors included) is scaled to a norm of at most max_norm (>= 0, finite):
- * times min(1, max_norm / (norm + 1e-6)), as pgm_grad_clip does.  Optional, before the first pgm_fit_run. */
+ * times min(1, max_norm / (norm + 1e-6)), as pgm_grad_clip does.  Optional, before the first pgm_fit_run (-3 behind it). */
 int pgm_fit_set_clip(pgm_fit* fit, double max_norm);
 int pgm_fit_run(pgm_fit* fit, int iters, void* stream);
 int pgm_fit_read(pgm_fit* fit, void* stream, int* iters_done, double* loss_hist, double* raw_hist, double* raw, int* info);
@@ -363,6 +363,7 @@ int pgm_lomb_scargle_fast_f64(const double* t, const double* y, const double* dy
  * result does not.  A NaN norm makes every output NaN, an infinite one zero (NaN where the gradient is infinite).  Memory that
  * is written must not be shared with another tensor of the call (-12; interleaved columns of one buffer are fine).
  * Nothing is kept between calls; the call may be captured.  -98: out of host memory.
+ * norm and scratch lie outside the tensors.
  */
 int64_t pgm_grad_scratch_doubles(int batch, int count, int64_t bytes, int strided);
 int pgm_grad_clip(int batch, int count, const uint64_t* in_host, const uint64_t* out_host, const int64_t* numel_host,

@@ -347,15 +347,15 @@ template <class C> __device__ __forceinline__ void add_weight(Shared<C>& S, int 
   if (lo) atomicAdd(&S.bins.lo[b], lo);
 }
 
-// SEEDED: the first bins, and the list of their bin's entries if it is short enough, have been made by other launches
-// The cut behind the first `want` entries of what `have` keeps (WEIGHTED: behind the shortest beginning with `share` of its weight);
-// lo <= every value that can matter.  The first bins divide the range of values evenly, the later ones (where a bin held too many
-// to sort) the range of the ordered bit patterns of the bin's values, at least a factor BINS / 2 narrower each time.
 struct Even {                                                   // the first bins: the range of values in equal parts
   double best, scale; bool good; int bins;
   __device__ __forceinline__ Even(double best_, double lo, int bins_) : best(best_), scale(bins_ / (best_ - lo)), bins(bins_) { good = best - lo > 0.0 && best - lo < 1e300 && scale < 1e300; }
   __device__ __forceinline__ int bin(double l) const { const int b = (int)((best - l) * scale); return b < bins ? b : bins - 1; }
 };
+// The cut behind the first `want` entries of what `have` keeps (WEIGHTED: behind the shortest beginning with `share` of its weight);
+// lo <= every value that can matter.  The first bins divide the range of values evenly, the later ones (where a bin held too many
+// to sort) the range of the ordered bit patterns of the bin's values, at least a factor BINS / 2 narrower each time.
+// SEEDED: the first bins, and the list of their bin's entries if it is short enough, have been made by other launches
 // `summed` (WEIGHTED; may be null): where the first bin is short enough, the pass that collects its entries also forms the cells' kept
 // weights (S.cells; of entries with a weight of at least min_p), and says so
 template <bool WEIGHTED, bool SEEDED, class C, class F> __device__ __forceinline__ Cut select(const Row<F>& R, Shared<C>& S, double lo, Cut have, u64 want, double share,
@@ -844,8 +844,8 @@ template <class C, class F> __global__ __launch_bounds__(C::NT) __attribute__((a
   const Settings p = settings_of(A, row);
   Row<F> R = row_of<F>(A, row, p.t);
   const bool lowest = wants_lowest(p, R.cells);
-  constexpr bool TINY = C::NT == 64;
-  const bool plain = p.plain && !(TINY && draws_here);
+  constexpr bool TINY = C::NT == 64;                            // (makes its own draws always)
+  const bool plain = p.plain && !TINY;
   const double low = plain ? pass_best<C::NT, true, F>(R, 0, R.cells, S.best, S.cells, false)
                            : pass_best<C::NT, false, F>(R, 0, R.cells, S.best, nullptr, lowest);
   __syncthreads();
@@ -858,18 +858,18 @@ template <class C, class F> __global__ __launch_bounds__(C::NT) __attribute__((a
       int listed;
       bool summed;
       cut = cut_of<C, F>(R, S, p, lowest ? block_min<C::NT>(S.red, low) : -INF, listed, summed);
-      if (listed && draws_here) { draw_list<C, F>(A, R, S, row, listed); return; }
-      if constexpr (TINY) if (draws_here) { draw_tiny<C, F>(A, R, S, row, cut, p.min_p); return; }
+      if (listed && (TINY || draws_here)) { draw_list<C, F>(A, R, S, row, listed); return; }
+      if constexpr (TINY) { draw_tiny<C, F>(A, R, S, row, cut, p.min_p); return; }
       __syncthreads();                                          // (the cells take the bins' place)
       if (!summed) pass_weights<C::NT, F>(R, S.best, 0, R.cells, cut, p.min_p, S.cells);
-    } else if (TINY && draws_here) {
-      if constexpr (TINY) draw_tiny<C, F>(A, R, S, row, cut, 0.0);
+    } else if constexpr (TINY) {
+      draw_tiny<C, F>(A, R, S, row, cut, 0.0);
       return;
     } else if (draws_here) {
       for (int c = threadIdx.x; c < R.cells; c += C::NT) S.cells[c] *= cell_factor(R, S.best[c]);
     }
   }
-  if (draws_here) {
+  if (TINY || draws_here) {
     if (!(R.best > -INF)) { draw_nothing(A, row, 0, A.draws, C::NT); return; }
     scan_cells(S, R.cells);
     draw<C, F>(A, R, S, row, 0, A.draws, cut, p.min_p);
@@ -1045,7 +1045,7 @@ Plan plan_of(int type, int64_t rows, int64_t cols, int64_t draws) {
   p.build = p.max_cells <= Tiny::CELLS && rows >= 1024 ? 2 : rows > 512 ? 1 : 0;
   p.groups = (p.build == 0 && p.max_cells >= 32 && rows <= 64) ? (int)std::min<int64_t>(p.max_cells / 8, std::max<int64_t>(1, 512 / rows)) : 0;
   p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(p.max_cells / 16, 256 / rows));      // (of the launches with 16 wavefronts and tables to merge)
-  p.draws_here = p.groups == 0 && draws <= 64;
+  p.draws_here = p.groups == 0 && (p.build == 2 || draws <= 64);
   return p;
 }
 int64_t scratch_of(const Plan& p, int64_t rows) {

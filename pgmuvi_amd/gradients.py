@@ -175,6 +175,9 @@ def clip_grads_(grads, max_norm: float, norm_type: float = 2.0, out=None, member
             raise ValueError("clip_grads_: out must hold one tensor of the same shape and type for every gradient")
         if grads and outs[0].device != grads[0].device:
             raise ValueError("clip_grads_: all tensors must be on one device")
+        if any(o.is_neg() for o in outs):
+            raise ValueError("clip_grads_: out must not be a negated view")
+        grads = [g.resolve_neg() for g in grads]                 # (in place the kernel scales the memory behind the view: the same)
     if error_if_nonfinite:
         norm = _run(grads, None, 0.0, norm_type, members, "clip_grads_")
         if not bool(torch.isfinite(norm).all()):

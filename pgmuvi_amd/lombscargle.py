@@ -221,6 +221,8 @@ def draw_frequencies(t: torch.Tensor, y: torch.Tensor, dy: Optional[torch.Tensor
     ``top_k`` the k best, ``temperature`` > 1 flattens it (:func:`pgmuvi_amd.sampling.draw_indices`).  Returns (freqs (B, S),
     their log-probabilities (B, S), grid), all on the device; NaN where a light curve has no finite periodogram."""
     from .sampling import draw_indices
+    if y.shape[-1] < 4:
+        raise ValueError(f"draw_frequencies: light curves of at least four points, got {y.shape[-1]}")      # (the odds' power: (n - 3) / 2)
     grid = _shared_grid(t, y, nyquist_factor, samples_per_peak)
     P = periodogram_batched(t, y, dy, grid)
     odds = torch.log1p(-P.clamp(max=1.0 - 2.0 ** -52)).mul_(-0.5 * (y.shape[-1] - 3))      # (a noiseless sinusoid's P rounds to one)

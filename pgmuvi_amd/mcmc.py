@@ -528,6 +528,17 @@ def effective_sample_size(x: np.ndarray) -> np.ndarray:
     return out.reshape(x.shape[2:])
 
 
+def _start_frequencies(t, y, dy, num, seed, chains):
+    """``num`` frequencies for each chain (C, num), drawn from the 95 % highest-density set of its light curve's periodogram; NaN
+    where there is none.  A chain's draws depend on its own light curve and number alone, not on the others' sampling spans."""
+    from .lombscargle import draw_frequencies
+    u = torch.as_tensor(np.stack([np.random.default_rng([seed, 104729, c]).random(num) for c in chains]), device=y.device)
+    first, last = t.amin(-1), t.amax(-1)
+    one_span = bool(((first == first[0]) & (last == last[0])).all())
+    rows = [slice(None)] if one_span else [slice(c, c + 1) for c in range(y.shape[0])]
+    return torch.cat([draw_frequencies(t[r], y[r], None if dy is None else dy[r], u[r], top_p=0.95)[0] for r in rows]).cpu().numpy()
+
+
 def run_mcmc(x, y, noise=None, num_mixtures=4, sampler="NUTS", num_samples=500, warmup_steps=100, num_chains=1, seed=0,
              initial_values=None, priors=None, dim_order=0, group=None, compute=None,
              group_by_chain=False, **sampler_kwargs):
@@ -556,11 +567,11 @@ def run_mcmc(x, y, noise=None, num_mixtures=4, sampler="NUTS", num_samples=500, 
     world = dist.get_world_size(group) if dist.is_available() and dist.is_initialized() else 1
     rank = dist.get_rank(group) if world > 1 else 0
     lo, hi = shard_bounds(C, rank, world)
+    if isinstance(initial_values, str) and initial_values != "periodogram":
+        raise ValueError(f"initial_values must be a dictionary of sites, 'periodogram' or None, got {initial_values!r}")
     if hi > lo:
         pot = SMPotential(xs[lo:hi].contiguous(), ys[lo:hi].contiguous(), None if nz is None else nz[lo:hi].contiguous(),
                           num_mixtures, dim_order, priors, compute)
-        if isinstance(initial_values, str) and initial_values != "periodogram":
-            raise ValueError(f"initial_values must be a dictionary of sites, 'periodogram' or None, got {initial_values!r}")
         if initial_values is not None and not isinstance(initial_values, str):      # {site: value of site.shape (all chains) or (C, *site.shape)}
             vals = {}
             for st in pot.sites:
@@ -574,11 +585,11 @@ def run_mcmc(x, y, noise=None, num_mixtures=4, sampler="NUTS", num_samples=500, 
             if initial_values is not None:   # 'periodogram': the mixture means start on draws from the frequency posterior
                 if pot.d != 1:
                     raise NotImplementedError("initial_values='periodogram' needs light curves with one input dimension")
-                from .lombscargle import draw_frequencies
-                u = np.stack([np.random.default_rng([seed, 104729, c]).random(pot.Q) for c in range(lo, hi)])
-                freqs, _, _ = draw_frequencies(pot.x[..., 0], pot.y, None if pot.noise is None else pot.noise.sqrt(),
-                                               torch.as_tensor(u, device=pot.y.device), top_p=0.95)
-                z0[:, pot.slices()["covar_module.mixture_means_prior"]] = np.log(freqs.cpu().numpy())
+                freqs = _start_frequencies(pot.x[..., 0], pot.y, None if pot.noise is None else pot.noise.sqrt(), pot.Q, seed, range(lo, hi))
+                if not np.isfinite(freqs).all():
+                    raise ValueError("initial_values='periodogram': no finite periodogram (a constant light curve?) for chains "
+                                     f"{[lo + int(c) for c in np.flatnonzero(~np.isfinite(freqs).all(1))]}")
+                z0[:, pot.slices()["covar_module.mixture_means_prior"]] = np.log(freqs)
         res = sample(pot, z0, num_samples, warmup_steps, sampler, seed, chain_ids=range(lo, hi), **sampler_kwargs)
         P = pot.P
         local = np.concatenate([res["samples"].reshape(hi - lo, -1), res["stats"]["accept_prob"], res["stats"]["n_leapfrog"].astype(float),

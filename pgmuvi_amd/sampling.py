@@ -55,7 +55,7 @@ def draw_indices(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=N
     if not torch.is_tensor(u) or u.dtype not in _TYPE:
         raise TypeError("draw_indices: u must be a floating-point tensor of random numbers")
     _hip.require_gpu(logits, "draw_indices")
-    dev = logits.device
+    dev, logits, u = logits.device, logits.resolve_neg(), u.resolve_neg()
     if u.device != dev:
         raise ValueError(f"draw_indices: u is on {u.device}, the logits on {dev}")
     single = logits.dim() == 1

@@ -220,3 +220,33 @@ def test_a_multi_start_fit(dev):
         for k, z in zip(("w", "mu", "v"), logs):
             theta[k] = theta[k] * torch.exp(0.5 * z)
     assert all(bool(torch.isfinite(x).all()) and bool((x > 0).all()) for x in theta.values())
+
+
+def test_a_limit_is_set_before_the_first_step(dev):
+    from pgmuvi_amd.trainers import _native_fit_handle
+    m, lik, x, y = _model(dev, 60)
+    fit = _native_fit_handle(m, lik, x, y, 4, 1e-3, "Adam", 1e-8)[0]
+    for bad in (-1.0, math.nan, math.inf):
+        with pytest.raises(RuntimeError):
+            fit.set_clip(bad)
+    fit.set_clip(0.5)
+    fit.set_clip(0.25)
+    fit.run(2)
+    with pytest.raises(RuntimeError):
+        fit.set_clip(1.0)
+
+
+def test_chains_without_a_periodogram_and_with_spans_of_their_own(dev):
+    t, y, e = _curves(dev, 3, 100)
+    t = t.clone()
+    t[1] *= 1.5                                                  # (its own span, so its own grid)
+    both = mcmc._start_frequencies(t, y, e, 4, 7, range(5, 8))
+    alone = [mcmc._start_frequencies(t[c:c + 1], y[c:c + 1], e[c:c + 1], 4, 7, range(5 + c, 6 + c)) for c in range(3)]
+    assert np.array_equal(both, np.concatenate(alone)) and np.isfinite(both).all()
+    y = y.clone()
+    y[2] = 0.0
+    dead = mcmc._start_frequencies(t, y, e, 4, 7, range(5, 8))
+    assert np.array_equal(dead[:2], both[:2]) and np.isnan(dead[2]).all()
+    kw = dict(noise=e ** 2, num_mixtures=2, num_samples=2, warmup_steps=2, max_tree_depth=2, seed=5, group_by_chain=True)
+    with pytest.raises(ValueError, match=r"chains \[2\]"):
+        mcmc.run_mcmc(t.unsqueeze(-1), y, initial_values="periodogram", **kw)

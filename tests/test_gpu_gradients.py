@@ -266,3 +266,18 @@ def test_more_than_32_bits_of_offset(dev):
     assert norm.tolist() == [3.0, float(torch.tensor(math.sqrt(160.0)).float())]
     G.clip_grads_([rows], 6.5 - 1e-6, members=False)             # (norm 13: factor one half, to 1e-7)
     assert rows[0, -1] == 1.5 and rows[1, 0] == 2.0 and rows[1, -2] == 6.0 and float(rows[1, 5:-2].abs().max()) == 0.0
+
+
+def test_negated_views(dev):
+    """The imaginary part of a conjugate is a view whose memory holds the opposite sign."""
+    z = torch.complex(torch.randn(300, dtype=torch.float64, device=dev), torch.randn(300, dtype=torch.float64, device=dev)).conj()
+    g, want = z.imag, z.imag.clone()
+    assert g.is_neg()
+    out = torch.empty_like(want)
+    n = G.clip_grads_([g], 1.0, out=[out])
+    scale = 1.0 / (float(want.norm()) + 1e-6)
+    assert torch.allclose(out, want * scale, rtol=1e-13, atol=0.0) and abs(float(n) / float(want.norm()) - 1) < 1e-13
+    with pytest.raises(ValueError, match="negated"):
+        G.clip_grads_([want], 1.0, out=[g])
+    G.clip_grads_([g], 1.0)
+    assert torch.allclose(g, want * scale, rtol=1e-13, atol=0.0)

@@ -256,3 +256,28 @@ def test_long_rows_with_settings_per_row(dev, V):
     _check(l, u, got, **per)
     wide = l.to(dev).t().contiguous().t()                        # a column per frequency: strided rows
     assert torch.equal(draw_indices(wide, u.to(dev), top_p=0.8), draw_indices(l.to(dev), u.to(dev), top_p=0.8))
+
+
+def test_negated_views(dev):
+    """The imaginary part of a conjugate is a view whose memory holds the opposite sign."""
+    z = torch.complex(torch.zeros(2, 500, dtype=torch.float64), torch.as_tensor(np.random.default_rng(1).normal(0, 3, (2, 500)))).to(dev).conj()
+    l, u = z.imag, torch.as_tensor(np.random.default_rng(2).random((2, 8)), device=dev)
+    assert l.is_neg() and torch.equal(draw_indices(l, u), draw_indices(l.clone(), u))
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=7), dict(top_k=700), dict(top_p=0.4, min_p=0.1), dict(min_p=0.05)])
+def test_many_draws_of_many_short_rows(dev, dtype, kw):
+    """A row's draws do not depend on how many there are, nor on the rows beside it."""
+    g = np.random.default_rng(11)
+    l = torch.as_tensor(g.normal(0, 3, (1030, 777))).to(dtype).to(dev)
+    l[5] = -math.inf
+    u = torch.as_tensor(g.random((1030, 130)), device=dev)
+    index, logp = draw_indices(l, u, return_logprob=True, **kw)
+    assert bool((index[5] == -1).all())
+    for s in (slice(0, 40), slice(90, 130)):
+        few, lp = draw_indices(l, u[:, s], return_logprob=True, **kw)
+        assert torch.equal(few, index[:, s]) and torch.equal(lp, logp[:, s])
+    for b in (0, 1029):
+        want, lp = oracle.draw_row(l[b].double().cpu().numpy(), u[b].cpu().numpy(), **kw)
+        assert torch.equal(index[b].cpu(), torch.as_tensor(want)) and np.allclose(logp[b].cpu().numpy(), lp, rtol=1e-12, atol=1e-12)

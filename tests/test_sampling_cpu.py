@@ -62,3 +62,15 @@ def test_oracle_on_small_distributions():
     assert oracle.draw_row([-math.inf, math.nan], [0.5])[0].tolist() == [-1]
     idx, lp = oracle.draw_row(l, [0.3], top_k=2)
     assert idx[0] == 1 and abs(lp[0] - math.log(4 / 7)) < 1e-15
+
+
+def test_light_curves_too_short_for_odds_are_refused():
+    from pgmuvi_amd.lombscargle import draw_frequencies
+    with pytest.raises(ValueError, match="at least four points"):
+        draw_frequencies(torch.zeros(1, 3), torch.zeros(1, 3), None, torch.zeros(1, 1))
+
+
+def test_a_start_that_does_not_exist_is_refused():
+    from pgmuvi_amd import mcmc
+    with pytest.raises(ValueError, match="initial_values"):
+        mcmc.run_mcmc(torch.zeros(5), torch.zeros(5), initial_values="peaks")
