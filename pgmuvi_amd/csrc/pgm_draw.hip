@@ -65,6 +65,7 @@ __device__ __forceinline__ double of_key(u64 k) { return __longlong_as_double((l
 struct Param { double v; const double* p; };                    // one number for every row, or one per row
 struct ParamI { int64_t v; const int64_t* p; };
 struct CutState { double value; int64_t idx; };
+constexpr int64_t DRAWN = -2;                                   // (a cut's idx: the row's draws have been made)
 constexpr int TABLE_BINS = 4096, TABLE_LIST = 1024;             // (those of the build All below)
 struct Table { u64 hi[TABLE_BINS], lo[TABLE_BINS]; double value[TABLE_LIST]; uint32_t count[TABLE_BINS], idx[TABLE_LIST]; int listed, pad; };
 struct DrawArgs {
@@ -75,6 +76,7 @@ struct DrawArgs {
   int64_t* index; double* logp;
   int mult, max_cells;                                          // loads per lane and cell over U, cells of a full row
   double *best, *sums, *lows; CutState* cut; Table* tables;     // rows whose passes are launches of their own: [row][max_cells] twice, [row][groups], [row], [row][2]
+  double* lots;                                                 // [row][64 mult max_cells], where many draws share them
 };
 
 // kept: values above the cut's, and equal ones up to its index
@@ -600,20 +602,20 @@ template <int THREADS, class F> __device__ __forceinline__ void pass_weights(con
     if ((threadIdx.x & 63) == 0) sums[c] = total;
   });
 }
-// running sums over S.cells
-template <class C> __device__ __forceinline__ void scan_cells(Shared<C>& S, int cells) {
+// running sums over the cells, in place
+template <class C> __device__ __forceinline__ void scan_cells(double* sums, double* red, int cells) {
   constexpr int PER = (C::CELLS + C::NT - 1) / C::NT;
   double v[PER], s = 0.0;
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < PER; ++k) { const int c = threadIdx.x * PER + k; s += c < cells ? S.cells[c] : 0.0; v[k] = s; }
-  const double base = block_scan<C::NT>(S.red, s) - s;
+  for (int k = 0; k < PER; ++k) { const int c = threadIdx.x * PER + k; s += c < cells ? sums[c] : 0.0; v[k] = s; }
+  const double base = block_scan<C::NT>(red, s) - s;
 #pragma unroll
-  for (int k = 0; k < PER; ++k) { const int c = threadIdx.x * PER + k; if (c < cells) S.cells[c] = base + v[k]; }
+  for (int k = 0; k < PER; ++k) { const int c = threadIdx.x * PER + k; if (c < cells) sums[c] = base + v[k]; }
   __syncthreads();
 }
 // first of n running sums above x (or equal to it)
-__device__ __forceinline__ int first_above(const double* run, int n, double x, bool or_equal) {
+template <class Run> __device__ __forceinline__ int first_above(Run run, int n, double x, bool or_equal) {
   int a = 0, b = n;
   while (a < b) { const int m = (a + b) >> 1; const double f = run[m]; if (f > x || (or_equal && f >= x)) b = m; else a = m + 1; }
   return a;
@@ -622,57 +624,93 @@ __device__ __forceinline__ double target_of(double u, double Z) {               
   const double x = u * Z;
   return x > 0.0 ? x : x == x ? 0.0 : Z;
 }
-// the draws [s0, s1) of a row from its running sums, one wavefront each
-template <class C, class F> __device__ __forceinline__ void draw(const DrawArgs& A, const Row<F>& R, const Shared<C>& S, int64_t row, int64_t s0, int64_t s1, const Cut& cut, double min_p) {
+__device__ __forceinline__ void put_draw(const DrawArgs& A, int64_t at, int64_t found, double logp) {
+  A.index[at] = found;
+  if (A.logp) A.logp[at] = logp;
+}
+// (Running sums of two threads are rounded differently, so that one may grow by a rounding over entries that weigh nothing.  A draw
+// that falls into such a gap takes the nearest kept entry behind it, or before it where there is none.)
+// The draws [s0, s1) of a row from the running sums of its cells, one wavefront each
+template <int THREADS, class F> __device__ __forceinline__ void draw(const DrawArgs& A, const Row<F>& R, const double* cells, int64_t row, int64_t s0, int64_t s1, const Cut& cut, double min_p) {
   const int lane = threadIdx.x & 63;
-  const double Z = S.cells[R.cells - 1], log_z = log(Z);
-  for (int64_t s = s0 + (threadIdx.x >> 6); s < s1; s += Shared<C>::NW) {
+  const double Z = cells[R.cells - 1], log_z = log(Z);
+  for (int64_t s = s0 + (threadIdx.x >> 6); s < s1; s += THREADS / 64) {
     double target = target_of(A.u[row * A.draws + s], Z);
-    int c = first_above(S.cells, R.cells, target, false);
-    if (c == R.cells) { c = first_above(S.cells, R.cells, Z, true); target = INF; }
-    double base = c ? S.cells[c - 1] : 0.0;
+    int c = first_above(cells, R.cells, target, false);
+    if (c == R.cells) { c = first_above(cells, R.cells, Z, true); target = INF; }
     // the cell's running weight: every lane sums PER neighbouring entries, one scan over the lanes, and the lane that reaches the
     // target looks through its own
     constexpr int PER = F::U * Row<F>::VEC;
-    int64_t found = -1, last = -1;
-    for (int j = 0; j < R.mult && found < 0; ++j) {
-      const int64_t i0 = c * R.width() + (int64_t)j * 64 * PER + lane * PER;
-      double w[PER], sum = 0.0;
-      int some = -1;
+    int64_t found = -1;
+    for (int step = 1, start = c; found < 0 && c >= 0;) {
+      int64_t last = -1;
+      double base = c ? cells[c - 1] : 0.0;
+      for (int j = 0; j < R.mult && found < 0; ++j) {
+        const int64_t i0 = c * R.width() + (int64_t)j * 64 * PER + lane * PER;
+        double w[PER], sum = 0.0;
+        int some = -1;
 #pragma unroll
-      for (int e = 0; e < PER; ++e) {
-        w[e] = 0.0;
-        if (i0 + e < R.n) {
-          const double l = R.value(i0 + e);
-          if (l > -INF && cut.keeps(l, i0 + e)) { const double x = R.weight(l); w[e] = x < min_p ? 0.0 : x; }
+        for (int e = 0; e < PER; ++e) {
+          w[e] = 0.0;
+          if (i0 + e < R.n) {
+            const double l = R.value(i0 + e);
+            if (l > -INF && cut.keeps(l, i0 + e)) { const double x = R.weight(l); w[e] = x < min_p ? 0.0 : x; }
+          }
+          sum += w[e];
+          some = w[e] > 0.0 ? e : some;
         }
-        sum += w[e];
-        some = w[e] > 0.0 ? e : some;
-      }
-      const double inc = wave_scan(sum);
-      const u64 hit = __ballot(sum > 0.0 && base + inc > target), any = __ballot(sum > 0.0);
-      if (any) { const int l = 63 - __clzll(any); last = i0 - lane * PER + l * PER + __shfl(some, l); }
-      if (hit) {
-        const int l = __ffsll(hit) - 1;
-        double run = base + (inc - sum);
-        int e = some;                                           // (its last kept one, should the sums differ by a rounding)
+        const double inc = wave_scan(sum);
+        const u64 hit = __ballot(sum > 0.0 && base + inc > target), any = __ballot(sum > 0.0);
+        if (any) { const int l = 63 - __clzll(any); last = i0 - lane * PER + l * PER + __shfl(some, l); }
+        if (hit) {
+          const int l = __ffsll(hit) - 1;
+          double run = base + (inc - sum);
+          int e = some;                                         // (its last kept one, should the sums differ by a rounding)
 #pragma unroll
-        for (int k = PER - 1; k >= 0; --k) {                    // run before entry k, from the back: the first that passes the target stays
-          double r = run;
+          for (int k = PER - 1; k >= 0; --k) {                  // run before entry k, from the back: the first that passes the target stays
+            double r = run;
 #pragma unroll
-          for (int m = 0; m <= k; ++m) r += w[m];
-          if (w[k] > 0.0 && r > target) e = k;
+            for (int m = 0; m <= k; ++m) r += w[m];
+            if (w[k] > 0.0 && r > target) e = k;
+          }
+          found = i0 - lane * PER + l * PER + __shfl(e, l);
         }
-        found = i0 - lane * PER + l * PER + __shfl(e, l);
+        base += __shfl(inc, 63);
       }
-      base += __shfl(inc, 63);
+      if (found < 0) found = last;                              // (the cell's own sum and this one differ by a rounding)
+      if (found < 0) {                                          // (nothing kept in this cell)
+        c += step;
+        if (c == R.cells) { step = -1; c = start - 1; }
+      }
     }
-    if (found < 0) found = last;                                // (the cell's own sum and this one differ by a rounding)
-    if (lane == 0) {
-      A.index[row * A.draws + s] = found;
-      if (A.logp) A.logp[row * A.draws + s] = R.z(R.value(found)) - log_z;
-    }
+    if (lane == 0) put_draw(A, row * A.draws + s, found, found < 0 ? -INF : R.z(R.value(found)) - log_z);
   }
+}
+template <class F> __device__ __forceinline__ double kept_weight(const Row<F>& R, const Cut& cut, double min_p, int64_t i) {
+  if (i >= R.n) return 0.0;
+  const double l = R.value(i);
+  if (!(l > -INF) || !cut.keeps(l, i)) return 0.0;
+  const double w = R.weight(l);
+  return w < min_p ? 0.0 : w;
+}
+// The entry of lot j (PER neighbouring entries; run: running sums of the lots) where the running sum passes `target`
+template <class F, class Run> __device__ __forceinline__ int64_t entry_of_lot(const Row<F>& R, Run run, int lots, int j, double target, const Cut& cut, double min_p) {
+  constexpr int PER = F::U * Row<F>::VEC;
+  double r = j ? run[j - 1] : 0.0;
+  int64_t found = -1;
+#pragma unroll 1
+  for (int k = j, step = 1; found < 0 && k >= 0;) {
+#pragma unroll 1
+    for (int e = 0; e < PER; ++e) {
+      const int64_t i = (int64_t)k * PER + e;
+      const double w = kept_weight(R, cut, min_p, i);
+      r += w;
+      if (w > 0.0) { found = i; if (r > target) break; }         // (else its last kept one: the sums differ by a rounding)
+    }
+    k += step;                                                  // (nothing kept in this lot)
+    if (k == lots) { step = -1; k = j - 1; }
+  }
+  return found;
 }
 __device__ __forceinline__ void draw_nothing(const DrawArgs& A, int64_t row, int64_t s0, int64_t s1, int threads) {
   for (int64_t s = s0 + threadIdx.x; s < s1; s += threads) {
@@ -713,8 +751,10 @@ template <class C, class F> __device__ __forceinline__ void draw_list(const Draw
   for (int64_t s = t; s < A.draws; s += C::NT) {
     int j = first_above(run, n, target_of(A.u[row * A.draws + s], Z), false);
     if (j == n) j = first_above(run, n, Z, true);
-    A.index[row * A.draws + s] = (int64_t)S.list_idx[j];
-    if (A.logp) A.logp[row * A.draws + s] = R.z(S.list_value[j]) - log_z;
+    const int start = j;
+    while (j < n && !(R.weight(S.list_value[j]) > 0.0)) ++j;     // (see draw)
+    if (j == n) for (j = start; j > 0 && !(R.weight(S.list_value[j]) > 0.0);) --j;
+    put_draw(A, row * A.draws + s, (int64_t)S.list_idx[j], R.z(S.list_value[j]) - log_z);
   }
 }
 // A lower bound of the top_k-th value: the top_k-th highest of the cells' best values, from bins over them (S.best); `lowest` if there
@@ -799,20 +839,13 @@ template <class C, class F> __device__ __forceinline__ void draw_tiny(const Draw
   static_assert(C::NT == 64 && C::CELLS * 64 <= 2 * Shared<C>::BINS, "running sums in the bins' place");
   double* run = reinterpret_cast<double*>(S.bins.hi);            // (hi and lo)
   const int lane = threadIdx.x;
-  auto weight = [&](int64_t i) {
-    if (i >= R.n) return 0.0;
-    const double l = R.value(i);
-    if (!(l > -INF) || !cut.keeps(l, i)) return 0.0;
-    const double w = R.weight(l);
-    return w < min_p ? 0.0 : w;
-  };
   const int lots = (int)((R.n + PER - 1) / PER), rounds = (lots + 63) / 64;
   double base = 0.0;
   __syncthreads();
   for (int c = 0; c < rounds; ++c) {
     double sum = 0.0;
 #pragma unroll
-    for (int e = 0; e < PER; ++e) sum += weight((int64_t)(c * 64 + lane) * PER + e);
+    for (int e = 0; e < PER; ++e) sum += kept_weight(R, cut, min_p, (int64_t)(c * 64 + lane) * PER + e);
     const double inc = wave_scan(sum);
     run[c * 64 + lane] = base + inc;
     base += __shfl(inc, 63);
@@ -823,21 +856,14 @@ template <class C, class F> __device__ __forceinline__ void draw_tiny(const Draw
     double target = target_of(A.u[row * A.draws + s], Z);
     int j = first_above(run, lots, target, false);
     if (j == lots) { j = first_above(run, lots, Z, true); target = INF; }
-    double r = j ? run[j - 1] : 0.0;
-    int64_t found = -1;
-    for (int e = 0; e < PER; ++e) {
-      const int64_t i = (int64_t)j * PER + e;
-      const double w = weight(i);
-      r += w;
-      if (w > 0.0) { found = i; if (r > target) break; }        // (else its last kept one: the sums differ by a rounding)
-    }
-    A.index[row * A.draws + s] = found;
-    if (A.logp) A.logp[row * A.draws + s] = R.z(R.value(found)) - log_z;
+    const int64_t found = entry_of_lot(R, run, lots, j, target, cut, min_p);
+    put_draw(A, row * A.draws + s, found, found < 0 ? -INF : R.z(R.value(found)) - log_z);
   }
 }
 
 // ---- kernels --------------------------------------------------------------------------------------------------------------------------
-// One workgroup per row: everything, or (draws_here 0: many draws per row) all but the draws, which k_draws makes from memory
+// One workgroup per row: everything, or (draws_here 0: many draws per row) all but the draws of rows whose kept entries are not in a
+// list, which k_draws makes from memory
 template <class C, class F> __global__ __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(4))) void k_row(DrawArgs A, int draws_here) {
   __shared__ Shared<C> S;
   const int64_t row = blockIdx.x;
@@ -858,7 +884,11 @@ template <class C, class F> __global__ __launch_bounds__(C::NT) __attribute__((a
       int listed;
       bool summed;
       cut = cut_of<C, F>(R, S, p, lowest ? block_min<C::NT>(S.red, low) : -INF, listed, summed);
-      if (listed && (TINY || draws_here)) { draw_list<C, F>(A, R, S, row, listed); return; }
+      if (listed) {
+        draw_list<C, F>(A, R, S, row, listed);
+        if (!TINY && !draws_here && threadIdx.x == 0) A.cut[row] = CutState{0.0, DRAWN};
+        return;
+      }
       if constexpr (TINY) { draw_tiny<C, F>(A, R, S, row, cut, p.min_p); return; }
       __syncthreads();                                          // (the cells take the bins' place)
       if (!summed) pass_weights<C::NT, F>(R, S.best, 0, R.cells, cut, p.min_p, S.cells);
@@ -871,8 +901,8 @@ template <class C, class F> __global__ __launch_bounds__(C::NT) __attribute__((a
   }
   if (TINY || draws_here) {
     if (!(R.best > -INF)) { draw_nothing(A, row, 0, A.draws, C::NT); return; }
-    scan_cells(S, R.cells);
-    draw<C, F>(A, R, S, row, 0, A.draws, cut, p.min_p);
+    scan_cells<C>(S.cells, S.red, R.cells);
+    draw<C::NT, F>(A, R, S.cells, row, 0, A.draws, cut, p.min_p);
     return;
   }
   __syncthreads();
@@ -1015,53 +1045,136 @@ template <class F> __global__ __launch_bounds__(256) void k_weights(DrawArgs A, 
   const int c0 = (int)((int64_t)R.cells * g / groups), c1 = (int)((int64_t)R.cells * (g + 1) / groups);
   pass_weights<256, F>(R, A.best + row * A.max_cells, c0, c1, cut, p.min_p, A.sums + row * A.max_cells);
 }
-// ... and the draws, `per` of a row in every workgroup
-template <class F> __global__ __launch_bounds__(Long::NT) void k_draws(DrawArgs A, int blocks, int per, int cuts) {
-  __shared__ Shared<Long> S;
-  const int64_t row = blockIdx.x / blocks;
-  const int64_t s0 = (int64_t)(blockIdx.x % blocks) * per, s1 = s0 + per < A.draws ? s0 + per : A.draws;
-  const Settings p = settings_of(A, row);
-  Row<F> R = row_of<F>(A, row, p.t);
+// The running sums of a row's cells from memory; false: nothing to draw from them
+struct Sums { double cells[MAX_CELLS], red[Long::NT / 64]; };
+template <class F> __device__ __forceinline__ bool load_sums(const DrawArgs& A, Sums& S, Row<F>& R, const Settings& p, int64_t row, int cuts, Cut& cut) {
   R.best = best_of_row<Long::NT>(A, row, R.cells, S.red);
-  if (!(R.best > -INF)) { draw_nothing(A, row, s0, s1, Long::NT); return; }
-  const Cut cut = cuts ? tighter(everything(R.best), Cut{A.cut[row].value, A.cut[row].idx}) : everything(R.best);
+  if (!(R.best > -INF)) return false;
+  cut = cuts ? tighter(everything(R.best), Cut{A.cut[row].value, A.cut[row].idx}) : everything(R.best);
   for (int c = threadIdx.x; c < R.cells; c += Long::NT) {
     const double w = A.sums[row * A.max_cells + c];
     S.cells[c] = p.plain ? w * cell_factor(R, A.best[row * A.max_cells + c]) : w;
   }
-  scan_cells(S, R.cells);
-  draw<Long, F>(A, R, S, row, s0, s1, cut, p.min_p);
+  scan_cells<Long>(S.cells, S.red, R.cells);
+  return true;
+}
+typedef __attribute__((address_space(1))) double* Lots;
+// ... the running sums of the cells' lots (PER neighbouring entries, a lane's share of draw), for rows with many draws
+__device__ __forceinline__ bool drawn(const DrawArgs& A, int64_t row, int cuts) { return cuts && A.cut[row].idx == DRAWN; }
+template <class F> __global__ __launch_bounds__(Long::NT) void k_lots(DrawArgs A, int shares, int cuts) {
+  __shared__ Sums S;
+  constexpr int PER = F::U * Row<F>::VEC;
+  const int64_t row = blockIdx.x / shares;
+  const int g = blockIdx.x % shares, lane = threadIdx.x & 63;
+  if (drawn(A, row, cuts)) return;
+  const Settings p = settings_of(A, row);
+  Row<F> R = row_of<F>(A, row, p.t);
+  Cut cut;
+  if (!load_sums(A, S, R, p, row, cuts, cut)) return;
+  const Lots lots = (Lots)A.lots + row * ((int64_t)A.max_cells * A.mult * 64);
+  const int c0 = (int)((int64_t)R.cells * g / shares), c1 = (int)((int64_t)R.cells * (g + 1) / shares);
+  for (int c = c0 + (int)(threadIdx.x >> 6); c < c1; c += Long::NT / 64) {
+    double base = c ? S.cells[c - 1] : 0.0;
+    const bool some = A.best[row * A.max_cells + c] >= cut.value;
+    for (int j = 0; j < R.mult; ++j) {
+      const int64_t lot = ((int64_t)c * R.mult + j) * 64 + lane;
+      double sum = 0.0;
+      if (some) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) sum += kept_weight(R, cut, p.min_p, lot * PER + e);
+      }
+      const double inc = wave_scan(sum);
+      lots[lot] = base + inc;
+      base += __shfl(inc, 63);
+    }
+  }
+}
+// ... and the draws, `per` of a row in every workgroup: a wavefront for each, or (LOTS) a lane
+template <class F, bool LOTS> __global__ __launch_bounds__(Long::NT) void k_draws(DrawArgs A, int blocks, int per, int cuts) {
+  __shared__ Sums S;
+  const int64_t row = blockIdx.x / blocks;
+  const int64_t s0 = (int64_t)(blockIdx.x % blocks) * per, s1 = s0 + per < A.draws ? s0 + per : A.draws;
+  if (drawn(A, row, cuts)) return;
+  const Settings p = settings_of(A, row);
+  Row<F> R = row_of<F>(A, row, p.t);
+  Cut cut;
+  if (!load_sums(A, S, R, p, row, cuts, cut)) { draw_nothing(A, row, s0, s1, Long::NT); return; }
+  if constexpr (!LOTS) {
+    draw<Long::NT, F>(A, R, S.cells, row, s0, s1, cut, p.min_p);
+  } else {
+    constexpr int PER = F::U * Row<F>::VEC;
+    const Lots run = (Lots)A.lots + row * ((int64_t)A.max_cells * A.mult * 64);
+    const int all = (int)((R.n + PER - 1) / PER), each_cell = 64 * R.mult;
+    const double Z = S.cells[R.cells - 1], log_z = log(Z);
+    for (int64_t s = s0 + threadIdx.x; s < s1; s += Long::NT) {
+      double target = target_of(A.u[row * A.draws + s], Z);
+      int c = first_above(S.cells, R.cells, target, false);
+      if (c == R.cells) { c = first_above(S.cells, R.cells, Z, true); target = INF; }
+      const int from = c * each_cell, n = all - from < each_cell ? all - from : each_cell;
+      int j = first_above(run + from, n, target, false);
+      if (j == n) { j = first_above(run + from, n, run[from + n - 1], true); target = INF; }
+      const int64_t found = entry_of_lot(R, run, all, from + j, target, cut, p.min_p);
+      put_draw(A, row * A.draws + s, found, found < 0 ? -INF : R.z(R.value(found)) - log_z);
+    }
+  }
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------------
-// How a call runs: cells of a row, workgroups per row (0: one workgroup does a whole row), which build of it, draws apart from the rest
-struct Plan { int mult, max_cells, groups, shares, build; bool draws_here; };
+// How a call runs: cells of a row, workgroups per row (0: one workgroup does a whole row), which build of it (0 Long, 1 Many, 2 Tiny),
+// draws made by the row's own workgroup, and from lots where not
+struct Plan { int mult, max_cells, groups, shares, build; bool draws_here, lots; };
 static_assert(Shared<All>::BINS == TABLE_BINS && All::LIST == TABLE_LIST, "tables in memory");
-Plan plan_of(int type, int64_t rows, int64_t cols, int64_t draws) {
+enum Cuts { NO_CUT = 0, CUT = 1, FEW = 2 };                     // truncated?  FEW: to no more entries than a list takes
+Plan plan_of(int type, int64_t rows, int64_t cols, int64_t draws, Cuts cuts) {
   Plan p;
   const int64_t group = type == 0 ? 2 * 128 : type == 1 ? 2 * 256 : 512;
   p.mult = (int)((cols + group * MAX_CELLS - 1) / (group * MAX_CELLS));
   p.max_cells = (int)((cols + group * p.mult - 1) / (group * p.mult));
-  p.build = p.max_cells <= Tiny::CELLS && rows >= 1024 ? 2 : rows > 512 ? 1 : 0;
-  p.groups = (p.build == 0 && p.max_cells >= 32 && rows <= 64) ? (int)std::min<int64_t>(p.max_cells / 8, std::max<int64_t>(1, 512 / rows)) : 0;
+  // One wavefront per row: many short rows (4096 x 1113 fp64, top_p, 8 draws: 54 us against 67 with four; 1000 of them: 29 against 22,
+  // hence the 1024), and the shortest while it can make the draws (300 x 161, top_p, 8 draws: 16 against 23; 256 draws: 25 against 32;
+  // 1000 draws: 54 against 30).  Four wavefronts where rows fill the chip (two such workgroups' phases overlap better than one of
+  // eight: 4096 x 51200 fp32, top_k 50, 208 us against 227); eight else
+  p.build = (p.max_cells <= Tiny::CELLS && rows >= 1024) || (p.max_cells <= 2 && draws <= 256) ? 2 : rows > 512 ? 1 : 0;
+  // A few long rows are cut into pieces, so that more of the chip works on them, at the price of one launch more, with a cut of four or
+  // seven (fp64, plain, one workgroup against pieces: 1 x 25600 19 and 13 us, 1 x 204800 93 and 14, 64 x 204800 97 and 41, 256 x 204800
+  // 111 and 124;  top_p: 1 x 25600 37 and 49, 1 x 51200 61 and 50, 64 x 51200 67 and 82, 64 x 102400 110 and 99, 128 x 204800 200 and
+  // 195;  top_k 20, which a row's own workgroup makes from a list: 1 x 204800 47 and 47, 64 x 204800 49 and 78)
+  const int64_t loads = (int64_t)p.max_cells * p.mult, least = cuts == NO_CUT ? 48 : cuts == CUT ? 160 + 2 * rows : 800 + 3 * rows;
+  p.groups = (p.build == 0 && loads >= least && rows <= 128) ? (int)std::min<int64_t>(p.max_cells / 8, std::max<int64_t>(1, 512 / rows)) : 0;
   p.shares = (int)std::max<int64_t>(1, std::min<int64_t>(p.max_cells / 16, 256 / rows));      // (of the launches with 16 wavefronts and tables to merge)
-  p.draws_here = p.groups == 0 && (p.build == 2 || draws <= 64);
+  // A wavefront takes 3 us for a draw, a launch more 4: four rounds of them in place (300 x 1113, 17 draws: 16 us against 24; 64: 35
+  // against 20).  One wavefront's rows have lanes make them
+  p.draws_here = p.groups == 0 && (p.build == 2 || draws <= (p.build == 1 ? 16 : 32));
+  // Lots: each cell's weights once for all draws of the row, then a lane per draw instead of a wavefront.  Worth it where a row has as
+  // many draws as cells and the chip has more draws than wavefronts (600 x 50000 fp32, 300 draws: 174 us against 388; 65 draws on
+  // those 98 cells: 158 without; 32 x 161, 168 draws: 24 both)
+  p.lots = !p.draws_here && draws >= p.max_cells && draws * rows >= 8192;
   return p;
 }
+int64_t lots_of(const Plan& p) { return p.lots ? (int64_t)p.max_cells * p.mult * 64 : 0; }
 int64_t scratch_of(const Plan& p, int64_t rows) {
   if (p.draws_here) return 0;
-  return rows * (2 * (int64_t)p.max_cells + p.groups + 2 + (p.groups ? 2 * (int64_t)(sizeof(Table) / sizeof(double)) : 0));
+  return rows * (2 * (int64_t)p.max_cells + p.groups + 2 + lots_of(p) + (p.groups ? 2 * (int64_t)(sizeof(Table) / sizeof(double)) : 0));
 }
 static_assert(sizeof(Table) % sizeof(double) == 0, "scratch in doubles");
+Cuts cuts_of(const DrawArgs& A) {
+  if (!A.temperature.p && A.temperature.v == 0.0) return FEW;
+  if (!A.top_p.p && A.top_p.v == 0.0) return FEW;
+  if (!A.top_k.p && A.top_k.v > 0 && A.top_k.v <= Long::LIST) return FEW;
+  return A.temperature.p || A.top_k.p || A.top_k.v > 0 || A.top_p.p || A.top_p.v < 1.0 ? CUT : NO_CUT;
+}
 
 template <class F> void launch(DrawArgs& A, const Plan& p, int64_t rows, hipStream_t st) {
   int cuts = 1;
   if (p.groups == 0) {
     const dim3 grid((unsigned)rows);
-    if (p.build == 2) hipLaunchKernelGGL((k_row<Tiny, F>), grid, dim3(Tiny::NT), 0, st, A, p.draws_here ? 1 : 0);
-    else if (p.build == 1) hipLaunchKernelGGL((k_row<Many, F>), grid, dim3(Many::NT), 0, st, A, p.draws_here ? 1 : 0);
-    else hipLaunchKernelGGL((k_row<Long, F>), grid, dim3(Long::NT), 0, st, A, p.draws_here ? 1 : 0);
-    if (p.draws_here) return;
+    // (where a list of few entries is likely, its draws are cheap: 300 x 1113 rows of 64 draws, top_k 20: 16 us, with launches for the
+    // draws of other rows 21)
+    const bool here = p.draws_here || (A.draws <= 64 && !A.top_k.p && A.top_k.v > 0 && A.top_k.v <= 64);
+    if (p.build == 2) hipLaunchKernelGGL((k_row<Tiny, F>), grid, dim3(Tiny::NT), 0, st, A, here ? 1 : 0);
+    else if (p.build == 1) hipLaunchKernelGGL((k_row<Many, F>), grid, dim3(Many::NT), 0, st, A, here ? 1 : 0);
+    else hipLaunchKernelGGL((k_row<Long, F>), grid, dim3(Long::NT), 0, st, A, here ? 1 : 0);
+    if (here) return;
   } else {
     const dim3 grid((unsigned)(rows * p.groups));
     const bool ks = A.temperature.p || A.temperature.v == 0.0 || A.top_k.p || A.top_k.v > 0 || A.top_p.p || A.top_p.v == 0.0;
@@ -1081,16 +1194,25 @@ template <class F> void launch(DrawArgs& A, const Plan& p, int64_t rows, hipStre
     }
     if (cuts || A.min_p.p || A.min_p.v > 0.0) hipLaunchKernelGGL(k_weights<F>, grid, dim3(256), 0, st, A, p.groups, cuts);
   }
-  // a wavefront makes one draw at a time: two each, more where that fills the chip anyway
-  const int per = (int)std::max<int64_t>(16, (A.draws * rows / 1024 + 15) / 16 * 16);
+  if (p.lots) {
+    const int shares = (int)std::max<int64_t>(1, std::min<int64_t>(p.max_cells / 8, 1024 / rows));
+    hipLaunchKernelGGL(k_lots<F>, dim3((unsigned)(rows * shares)), dim3(Long::NT), 0, st, A, shares, cuts);
+  }
+  // a wavefront makes one draw at a time (with lots: 64): two each, more where that fills the chip anyway
+  const int at_once = p.lots ? Long::NT : 16;
+  const int per = (int)std::max<int64_t>(at_once, (A.draws * rows / 1024 + at_once - 1) / at_once * at_once);
   const int blocks = (int)((A.draws + per - 1) / per);
-  hipLaunchKernelGGL(k_draws<F>, dim3((unsigned)(rows * blocks)), dim3(Long::NT), 0, st, A, blocks, per, cuts);
+  const dim3 grid((unsigned)(rows * blocks));
+  if (p.lots) hipLaunchKernelGGL((k_draws<F, true>), grid, dim3(Long::NT), 0, st, A, blocks, per, cuts);
+  else hipLaunchKernelGGL((k_draws<F, false>), grid, dim3(Long::NT), 0, st, A, blocks, per, cuts);
 }
 }  // namespace
 
 extern "C" int64_t pgm_draw_scratch_doubles(int type, int64_t rows, int64_t cols, int64_t draws) {
   if (type < 0 || type > 3 || rows < 1 || cols < 1 || cols >= MAX_COLS || draws < 1) return 0;
-  return scratch_of(plan_of(type, rows, cols, draws), rows);
+  int64_t most = 0;                                             // (whatever the truncation)
+  for (const Cuts cuts : {NO_CUT, CUT, FEW}) most = std::max(most, scratch_of(plan_of(type, rows, cols, draws, cuts), rows));
+  return most;
 }
 
 extern "C" int pgm_draw_indices(const void* logits, int type, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride,
@@ -1112,18 +1234,20 @@ extern "C" int pgm_draw_indices(const void* logits, int type, int64_t rows, int6
   if (!min_p_row && !(min_p >= 0.0 && min_p <= 1.0)) return -16;
   if (!index) return -18;
   if (draws > 0x7fffffff || rows * draws > ((int64_t)1 << 40)) return -9;
-  const Plan p = plan_of(type, rows, cols, draws);
+  DrawArgs A{logits, row_stride, col_stride, cols, lengths, u, draws, {temperature, temperature_row}, {top_p, top_p_row}, {min_p, min_p_row},
+             {top_k, top_k_row}, index, logp, 0, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+  const Plan p = plan_of(type, rows, cols, draws, cuts_of(A));
   const int64_t need = scratch_of(p, rows);
   if (need > 0 && !scratch) return -20;
   if (need > scratch_doubles) return -21;
-  DrawArgs A{logits, row_stride, col_stride, cols, lengths, u, draws, {temperature, temperature_row}, {top_p, top_p_row}, {min_p, min_p_row},
-             {top_k, top_k_row}, index, logp, p.mult, p.max_cells, nullptr, nullptr, nullptr, nullptr, nullptr};
+  A.mult = p.mult; A.max_cells = p.max_cells;
   if (need > 0) {
     A.best = scratch;
     A.sums = scratch + rows * p.max_cells;
     A.lows = scratch + 2 * rows * p.max_cells;
     A.cut = reinterpret_cast<CutState*>(A.lows + rows * p.groups);
     A.tables = reinterpret_cast<Table*>(A.cut + rows);
+    A.lots = scratch + need - rows * lots_of(p);
   }
   hipStream_t st = (hipStream_t)stream;
   if (type == 0) launch<F64>(A, p, rows, st);

@@ -281,3 +281,40 @@ def test_many_draws_of_many_short_rows(dev, dtype, kw):
     for b in (0, 1029):
         want, lp = oracle.draw_row(l[b].double().cpu().numpy(), u[b].cpu().numpy(), **kw)
         assert torch.equal(index[b].cpu(), torch.as_tensor(want)) and np.allclose(logp[b].cpu().numpy(), lp, rtol=1e-12, atol=1e-12)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, cols, lengths", [(30, 5000, None), (100, 9000, [9000, 0, 1, 4097, 777]), (2, 300_000, None), (1, 40_000, None)])
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=7), dict(top_k=3000), dict(top_p=0.4, min_p=0.1), dict(min_p=0.05)])
+def test_many_draws_of_long_rows(dev, dtype, rows, cols, lengths, kw):
+    l = _rows(rows, cols, dtype, 21).to(dev)
+    g = np.random.default_rng(12)
+    S = 3000 if rows < 30 else 300
+    u = torch.as_tensor(g.random((rows, S)), device=dev)
+    u[:, 0], u[:, 1], u[:, 2] = 0.0, 1.0 - 2.0 ** -53, 1.0
+    n = None if lengths is None else torch.as_tensor((lengths * rows)[:rows], device=dev)
+    index, logp = draw_indices(l, u, lengths=n, return_logprob=True, **kw)
+    few, lp = draw_indices(l, u[:, :60], lengths=n, return_logprob=True, **kw)
+    assert torch.equal(few[:, 3:], index[:, 3:60]) and torch.allclose(lp[:, 3:], logp[:, 3:60], rtol=1e-12, atol=1e-12)
+    for b in {0, 1 % rows, 2 % rows, 4 % rows, rows - 1}:
+        v = cols if n is None else int(n[b])
+        want, wl = oracle.draw_row(l[b, :v].double().cpu().numpy(), u[b, :2].cpu().numpy().tolist() + u[b, 3:].cpu().numpy().tolist(), **kw)
+        got, gl = index[b].cpu().numpy(), logp[b].cpu().numpy()
+        assert np.array_equal(np.delete(got, 2), want) and np.allclose(np.delete(gl, 2), wl, rtol=1e-12, atol=1e-12)
+        if v:
+            assert got[2] == oracle.kept_entries(l[b, :v].double().cpu().numpy(), **kw)[0].max()           # (u outside [0, 1): the last kept one)
+
+
+@pytest.mark.parametrize("rows", [1, 9])
+@pytest.mark.parametrize("kw", [dict(), dict(min_p=0.05), dict(temperature=0.0), dict(top_p=0.0), dict(top_k=3), dict(top_k=600), dict(top_p=0.5), dict(top_k=5000, top_p=0.8)])
+@pytest.mark.parametrize("cols", [13_000, 90_000, 210_000])
+def test_a_setting_per_row_is_the_same_as_one_for_all(dev, rows, kw, cols):
+    """One number and a tensor of it may take other launches: the same draws."""
+    l = _rows(rows, cols, torch.float64, 5).to(dev)
+    u = torch.as_tensor(np.random.default_rng(6).random((rows, 12)), device=dev)
+    index, logp = draw_indices(l, u, return_logprob=True, **kw)
+    each = {k: torch.full((rows,), v, dtype=torch.int64 if k == "top_k" else torch.float64, device=dev) for k, v in kw.items()}
+    i2, l2 = draw_indices(l, u, return_logprob=True, **each)
+    assert torch.equal(index, i2) and torch.allclose(logp, l2, rtol=1e-12, atol=1e-12)
+    want, wl = oracle.draw_row(l[-1].cpu().numpy(), u[-1].cpu().numpy(), **kw)
+    assert np.array_equal(index[-1].cpu().numpy(), want) and np.allclose(logp[-1].cpu().numpy(), wl, rtol=1e-12, atol=1e-12)
