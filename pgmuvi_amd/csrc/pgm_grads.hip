@@ -8,7 +8,13 @@
 // upload, and a captured graph holds them like any other kernel's arguments).  Large sets: k_norm_part (partial sums of
 // contiguous ranges, at most PARTS workgroups) and then k_scale, whose every workgroup adds the partial sums up again in the
 // same fixed order -- or k_norm_final, one workgroup, where only the norm is asked for.  Small sets and batches of members:
-// k_member, one workgroup per member, norm and scaling in one launch.  No atomics: every result is reproducible bit for bit.
+// k_member_kept (entries in registers between norm and scaling) or k_member, one workgroup per member, norm and scaling in one
+// launch.  No atomics: every result is reproducible bit for bit.
+//
+// What bounds it: memory, at a copy's rate of 4.9 TB/s on this card (reading alone goes faster).  The norm of 2.1 GB fp64: 358 us,
+// 6.0 TB/s.  Clipping 1.07 GB bf16 in place: k_norm_part 217 us (4.9 TB/s) + k_scale 407 (5.3 TB/s of reading and writing); the
+// second read is needed, the set does not fit the caches.  The norm of 64 MB in 61 fp32 tensors: 16 + 4 us on the GPU, 35 with the host's description of them.  4096 members of 64 KB fp64: 105 us, 5.1 TB/s, each read once.
+// Small sets are one launch (the five tensors of a fit, 14 numbers: 6 us on the GPU, 17 with the host).
 //
 // Arithmetic.  All sums are fp64 whatever the tensors' type.  An fp64 square overflows from 1e154 on and vanishes below
 // 1e-162: fp64 entries go to one of three accumulators by magnitude (above 2^480, below 2^-480, between), the outer two
@@ -27,7 +33,7 @@ namespace {
 
 constexpr int TABLE = 64;             // tensors per launch (kernel arguments stay below 4 KB)
 constexpr int STRIDED_TABLE = 24;     // tensors whose entries are not one contiguous run (136 bytes each)
-constexpr int PARTS = 2048;           // partial sums per pass of a large set: 8 workgroups per CU
+constexpr int PARTS = 2048;           // partial sums per pass of a large set: 8 workgroups per CU, all resident at once
 constexpr int NT = 256;
 constexpr int CHUNK = 16384;          // bytes of one tensor a workgroup takes at a time: four 16-byte loads per thread in flight
 
@@ -399,10 +405,13 @@ bool any_clash(std::vector<Span>& v) {
 
 struct Item { int type; int64_t n; const char* in; char* out; int64_t in_member, out_member; const int64_t* layout; int64_t bytes, chunks; };
 
-// One workgroup per member, in one launch: a small set of few tensors (one CU streams 64 KB in the time a second launch takes; more
-// tensors, one after the other, take longer than two launches), or members enough to fill the chip with whole workgroups
+// One workgroup per member, in one launch: few tensors (one after the other, more take longer than two launches) of no more bytes
+// than a CU streams in the time a second launch takes, or, with members for half the chip, than its registers hold.  GPU times in
+// fp64, one launch against two: 1 member, 5 tensors, 112 B 6.2 and 7.0 us, 16 KB 6.4 and 7.2, 64 KB 8.6 and 8.1 (a launch less for
+// the host), 256 KB 12.5 and 7.4; 16 tensors, 4 KB 10.6 and 7.5;  512 members, 5 tensors, 64 KB 12.2 and 24.6, 320 KB 42 and 39;
+// 20 tensors, 64 KB 48 and 29
 bool one_launch(int batch, int64_t count, int64_t bytes, bool strided) {
-  return !strided && ((count <= 8 && bytes <= 65536) || (count <= TABLE && batch >= 512));
+  return !strided && count <= 8 && bytes <= (batch < 128 ? 65536 : 98304);
 }
 
 int run_clip(int batch, int count, const uint64_t* in, const uint64_t* out, const int64_t* numel, const unsigned char* type,
