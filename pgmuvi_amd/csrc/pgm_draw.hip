@@ -12,6 +12,15 @@
 // steps: sums of integers do not depend on the order of the LDS atomics, and 80 bits are more than the fp64 sums they are compared
 // with).  Equal values are split by index the same way.  The running sums are fp64, cell by cell in a fixed order: the same call
 // gives the same draws.
+//
+// What bounds it (MI355X; a copy moves 4.9 TB/s, so that reading a row once is the floor of all but the smallest calls).
+//   4096 x 51200 fp32, top_k 50 and top_p 0.9, one draw: 206 us, 4.1 TB/s of the one pass that reads everything (171 us at the
+//     copy's rate); the list and the draw overlap with other rows' loads.  Not truncated: 280 us, the exponentials of 2.1e8 entries.
+//   512 x 25600 fp64, top_p 0.95, four draws: 91 us against 21 for the bytes.  A row is one workgroup, two of them share a CU, and
+//     the phases follow each other: highest values 12 us, bins 20 (exponential and two LDS atomics an entry), the cut's entries and
+//     the cells' weights 19, the sort 3, the draws and waits the rest.  min_p or nothing instead of top_p: 32 us.
+//   1 x 204800 fp64, min_p 0.02, 1000 draws: 13 us on the GPU, three launches of 3 to 6 us; their bytes take 0.3.
+//   Short calls (1 x 1113 fp64, 8 draws): 8 us, one launch whose phases wait for each other.
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -1198,8 +1207,9 @@ template <class F> void launch(DrawArgs& A, const Plan& p, int64_t rows, hipStre
     const int shares = (int)std::max<int64_t>(1, std::min<int64_t>(p.max_cells / 8, 1024 / rows));
     hipLaunchKernelGGL(k_lots<F>, dim3((unsigned)(rows * shares)), dim3(Long::NT), 0, st, A, shares, cuts);
   }
-  // a wavefront makes one draw at a time (with lots: 64): two each, more where that fills the chip anyway
-  const int at_once = p.lots ? Long::NT : 16;
+  // a wavefront makes one draw at a time (with lots: 64): one each while that leaves the chip room (1 x 204800, 1000 draws: 13 us
+  // against 16 with two; 100 x 20000, 40: 23 against 29), else two, or more where that fills it anyway
+  const int at_once = p.lots ? Long::NT : A.draws * rows <= 4096 ? 8 : 16;
   const int per = (int)std::max<int64_t>(at_once, (A.draws * rows / 1024 + at_once - 1) / at_once * at_once);
   const int blocks = (int)((A.draws + per - 1) / per);
   const dim3 grid((unsigned)(rows * blocks));

@@ -318,3 +318,21 @@ def test_a_setting_per_row_is_the_same_as_one_for_all(dev, rows, kw, cols):
     assert torch.equal(index, i2) and torch.allclose(logp, l2, rtol=1e-12, atol=1e-12)
     want, wl = oracle.draw_row(l[-1].cpu().numpy(), u[-1].cpu().numpy(), **kw)
     assert np.array_equal(index[-1].cpu().numpy(), want) and np.allclose(logp[-1].cpu().numpy(), wl, rtol=1e-12, atol=1e-12)
+
+
+@pytest.mark.parametrize("rows, cols, per", [(1030, 777, 40), (3, 777, 700), (3, 5000, 20), (3, 5000, 40), (2, 60_000, 700), (2, 60_000, 5000), (200, 5000, 60)])
+@pytest.mark.parametrize("kw", [dict(min_p=0.3), dict(top_k=30), dict(top_k=900, min_p=0.2)])
+def test_draws_at_the_borders_of_the_kept_entries(dev, rows, cols, per, kw):
+    """Random numbers within a few steps of every border between two kept entries, with entries that weigh nothing between them: one
+    of the two is drawn, whatever the roundings of the running sums."""
+    rng = np.random.default_rng(31)
+    l = rng.normal(-60.0, 1.0, cols)
+    l[rng.choice(cols, 60, replace=False)] = rng.uniform(-1.0, 0.0, 60)
+    idx, w, _ = oracle.kept_entries(l, **kw)
+    c = np.cumsum(w)
+    at = rng.integers(0, len(idx) - 1, rows * per)
+    u = c[at] / c[-1] * (1.0 + rng.integers(-6, 7, rows * per) * 2.0 ** -53)
+    got = draw_indices(torch.as_tensor(l, device=dev).expand(rows, cols), torch.as_tensor(u.reshape(rows, per), device=dev), **kw).cpu().numpy().ravel()
+    pos = np.searchsorted(idx, got)
+    assert (got >= 0).all() and np.array_equal(idx[np.minimum(pos, len(idx) - 1)], got)
+    assert ((pos == at) | (pos == at + 1)).all()
