@@ -114,8 +114,8 @@ def test_refusals_come_before_any_launch(code, kw):
 def test_scratch_covers_every_launch():
     need = _hip.load().pgm_grad_scratch_doubles
     assert need(0, 3, 8, 0) == 0 and need(1, -1, 8, 0) == 0 and need(1, 3, -8, 0) == 0
-    assert need(1, 5, 112, 0) == 0 and need(4096, 5, 1 << 20, 0) == 0            # (one launch: no partial sums)
-    for batch in (1, 7, 300):
+    assert need(1, 5, 112, 0) == 0 and need(4096, 5, 90_000, 0) == 0            # (one launch: no partial sums)
+    for batch in (1, 7, 300, 4096):
         for count in (1, 64, 65, 5000):
             assert need(batch, count, 1 << 24, 0) >= 3 * (2048 + batch * (count // 64 + 1))
             assert need(batch, count, 64, 1) >= 3 * (2048 + batch * (count // 24 + 1))
