@@ -19,7 +19,7 @@
 //   512 x 25600 fp64, top_p 0.95, four draws: 91 us against 21 for the bytes.  A row is one workgroup, two of them share a CU, and
 //     the phases follow each other: highest values 12 us, bins 20 (exponential and two LDS atomics an entry), the cut's entries and
 //     the cells' weights 19, the sort 3, the draws and waits the rest.  min_p or nothing instead of top_p: 32 us.
-//   1 x 204800 fp64, min_p 0.02, 1000 draws: 13 us on the GPU, three launches of 3 to 6 us; their bytes take 0.3.
+//   1 x 204800 fp64, min_p 0.02, 1000 draws: 16 us on the GPU, three launches of 3 to 8 us; their bytes take 0.3.
 //   Short calls (1 x 1113 fp64, 8 draws): 8 us, one launch whose phases wait for each other.
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
