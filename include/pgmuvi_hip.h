@@ -349,7 +349,7 @@ int pgm_lomb_scargle_fast_f64(const double* t, const double* y, const double* dy
  * Norm of a set of gradients and its clipping (no counterpart in the reference: what a user of pgmuvi/trainers.py:177-182 would
  * put between `loss.backward()` and `optimizer.step()`):
  *     n = (sum |g|^p)^(1/p) over all entries of all tensors,   c = min(1, max_norm / (n + 1e-6)),   out = c g,
- * for each of `batch` members by itself (batch 1: one model; otherwise every tensor has a leading axis of `batch` members).
+ * for each of `batch` (< 2^22) members by itself (batch 1: one model; otherwise every tensor has a leading axis of `batch` members).
  * The tensors are described by HOST arrays of `count` entries:
  *   in_host / out_host  device addresses (out_host NULL: the norm only; out_host[t] == in_host[t]: in place);
  *   numel_host          entries per member;       type_host   0 fp64, 1 fp32, 2 bf16, 3 fp16 (mixed sets are fine);
@@ -381,7 +381,7 @@ int pgm_grad_clip(int batch, int count, const uint64_t* in_host, const uint64_t*
  * lengths[rows] (device, may be NULL): entries of each row; what lies behind is not read.  A row without a weight: index -1, logp -inf.
  * temperature_row / top_k_row / top_p_row / min_p_row: NULL, or [rows] device values used instead of the scalars -- there a
  * temperature <= 0 or NaN means 0, a top_k <= 0 all, a top_p >= 1 or NaN all and <= 0 the best entry, a min_p <= 0 or NaN none.
- * u outside [0, 1) draws the first or the last kept entry.  1 <= cols < 2^24.  scratch: pgm_draw_scratch_doubles doubles of device
+ * u outside [0, 1) draws the first or the last kept entry.  1 <= rows < 2^23, 1 <= cols < 2^24.  scratch: pgm_draw_scratch_doubles doubles of device
  * memory owned by the caller, used by this call only (NULL where that is 0).  Sums are fp64 in a fixed order; nothing is kept
  * between calls; the call may be captured.
  */

@@ -35,6 +35,7 @@ typedef unsigned long long u64;
 constexpr int LOAD = 16, CB = 2;                                // bytes of a lane's load; cells a wavefront works on at a time
 constexpr int MAX_CELLS = 1024;                                 // of a row (longer rows: wider cells)
 constexpr int64_t MAX_COLS = 1 << 24;                           // 2^24 weights of at most one, in steps of 2^-40, fit 64 bits
+constexpr int64_t MAX_ROWS = 1 << 23;                           // 512 threads a row: less than 2^32 of a launch
 constexpr int64_t EVERY = INT64_MAX;
 constexpr double INF = __builtin_inf();
 
@@ -1219,7 +1220,7 @@ template <class F> void launch(DrawArgs& A, const Plan& p, int64_t rows, hipStre
 }  // namespace
 
 extern "C" int64_t pgm_draw_scratch_doubles(int type, int64_t rows, int64_t cols, int64_t draws) {
-  if (type < 0 || type > 3 || rows < 1 || cols < 1 || cols >= MAX_COLS || draws < 1) return 0;
+  if (type < 0 || type > 3 || rows < 1 || rows >= MAX_ROWS || cols < 1 || cols >= MAX_COLS || draws < 1) return 0;
   int64_t most = 0;                                             // (whatever the truncation)
   for (const Cuts cuts : {NO_CUT, CUT, FEW}) most = std::max(most, scratch_of(plan_of(type, rows, cols, draws, cuts), rows));
   return most;
@@ -1232,7 +1233,7 @@ extern "C" int pgm_draw_indices(const void* logits, int type, int64_t rows, int6
                                 int64_t* index, double* logp, double* scratch, int64_t scratch_doubles, void* stream) {
   if (!logits) return -1;
   if (type < 0 || type > 3) return -2;
-  if (rows < 1 || rows > 0x7fffffff) return -3;
+  if (rows < 1 || rows >= MAX_ROWS) return -3;
   if (cols < 1 || cols >= MAX_COLS) return -4;
   if (row_stride < 0) return -5;
   if (col_stride < 0) return -6;

@@ -35,6 +35,7 @@ constexpr int TABLE = 64;             // tensors per launch (kernel arguments st
 constexpr int STRIDED_TABLE = 24;     // tensors whose entries are not one contiguous run (136 bytes each)
 constexpr int PARTS = 2048;           // partial sums per pass of a large set: 8 workgroups per CU, all resident at once
 constexpr int NT = 256;
+constexpr int MAX_MEMBERS = 1 << 22;  // 1024 threads each: less than 2^32 of a launch
 constexpr int CHUNK = 16384;          // bytes of one tensor a workgroup takes at a time: four 16-byte loads per thread in flight
 
 enum { T_F64 = 0, T_F32 = 1, T_BF16 = 2, T_F16 = 3 };
@@ -520,7 +521,6 @@ int run_clip(int batch, int count, const uint64_t* in, const uint64_t* out, cons
     l.groups = (int)std::max<int64_t>(1, std::min<int64_t>(l.chunks, (int64_t)share));
     l.slot0 = slots;
     slots += l.groups;
-    if ((int64_t)l.groups * batch > 0x7fffffff) return -1;
   }
   if (slots * batch * 3 > scratch_doubles) return -14;
   Acc* part = reinterpret_cast<Acc*>(scratch);
@@ -566,7 +566,7 @@ extern "C" int64_t pgm_grad_scratch_doubles(int batch, int count, int64_t bytes,
 extern "C" int pgm_grad_clip(int batch, int count, const uint64_t* in_host, const uint64_t* out_host, const int64_t* numel_host,
                              const unsigned char* type_host, const int64_t* member_host, const int64_t* layout_host, int p,
                              double max_norm, void* norm, int norm_f64, double* scratch, int64_t scratch_doubles, void* stream) {
-  if (batch < 1) return -1;
+  if (batch < 1 || batch >= MAX_MEMBERS) return -1;
   if (count < 0) return -2;
   if (count > 0 && !in_host) return -3;
   if (count > 0 && !numel_host) return -5;

@@ -130,6 +130,8 @@ def _run(tensors, outs, max_norm, norm_type, members, what):
         if any(t.dim() == 0 for t in tensors) or len({t.shape[0] for t in tensors}) != 1:
             raise ValueError(f"{what}: with members=True every tensor needs the same leading size, got {[tuple(t.shape) for t in tensors]}")
         batch = tensors[0].shape[0]
+        if batch >= 1 << 22:
+            raise ValueError(f"{what}: at most {(1 << 22) - 1} members, got {batch}")
     dev = tensors[0].device
     if batch == 0:
         return torch.empty(0, dtype=torch.float64 if any(t.dtype is torch.float64 for t in tensors) else torch.float32, device=dev)

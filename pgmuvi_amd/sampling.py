@@ -85,6 +85,8 @@ def draw_indices(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=N
         if return_logprob:
             logp.fill_(float("-inf"))
     elif B and S:
+        if B >= 1 << 23:
+            raise ValueError(f"draw_indices: at most {(1 << 23) - 1} rows, got {B}")
         if V >= 1 << 24:
             raise ValueError(f"draw_indices: rows of at most {(1 << 24) - 1} entries, got {V}")
         (t, tp, _t), (k, kp, _k), (p, pp, _p), (m, mp, _m) = settings

@@ -303,3 +303,15 @@ def test_members_of_many_tensors(dev, batch, count, n):
     b = batch // 2
     one = G.total_norm([t[b] for t in g])
     assert abs(float(one) / float(norm[b]) - 1) <= tol
+
+
+def test_the_most_members(dev):
+    n = (1 << 22) - 1
+    g = torch.stack([torch.arange(n, dtype=torch.float64, device=dev), torch.full((n,), 3.0, dtype=torch.float64, device=dev)], 1)
+    want = g.norm(dim=1)
+    assert float((G.total_norm([g], members=True) / want - 1).abs().max()) < 8 * 2.0 ** -53
+    rows = [g[:, :1], g[:, 1:]]                                  # (interleaved, and over more than one launch's tensors)
+    assert float((G.clip_grads_(rows + [torch.zeros(n, 1, device=dev) for _ in range(7)], 1.0, members=True) / want - 1).abs().max()) < 8 * 2.0 ** -53
+    assert float(g.norm(dim=1).max()) <= 1.0 + 2.0 ** -50
+    with pytest.raises(ValueError, match="members"):
+        G.total_norm([torch.zeros(1, 1, device=dev).expand(n + 1, 1)], members=True)

@@ -336,3 +336,12 @@ def test_draws_at_the_borders_of_the_kept_entries(dev, rows, cols, per, kw):
     pos = np.searchsorted(idx, got)
     assert (got >= 0).all() and np.array_equal(idx[np.minimum(pos, len(idx) - 1)], got)
     assert ((pos == at) | (pos == at + 1)).all()
+
+
+def test_the_most_rows(dev):
+    n = (1 << 23) - 1
+    u = torch.rand(n, dtype=torch.float64, device=dev)
+    l = torch.zeros(2, dtype=torch.float64, device=dev)
+    assert torch.equal(draw_indices(l.expand(n, 2), u), (u >= 0.5).to(torch.int64))
+    with pytest.raises(ValueError, match="rows"):
+        draw_indices(l.expand(n + 1, 2), torch.zeros(1, dtype=torch.float64, device=dev).expand(n + 1))

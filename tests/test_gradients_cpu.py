@@ -85,6 +85,7 @@ A = 1 << 20
 
 @pytest.mark.parametrize("code, kw", [
     (-1, dict(src=[A], dst=None, numel=[8], types=[0], batch=0)),
+    (-1, dict(src=[A], dst=None, numel=[8], types=[0], batch=1 << 22, member=[[8, 8]])),
     (-3, dict(src=[0], dst=None, numel=[8], types=[0])),
     (-4, dict(src=[A], dst=[0], numel=[8], types=[0])),
     (-5, dict(src=[A], dst=None, numel=[-8], types=[0])),

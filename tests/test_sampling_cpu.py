@@ -42,7 +42,7 @@ def _call(**kw):
 
 
 @pytest.mark.parametrize("code, kw", [
-    (-1, dict(logits=None)), (-2, dict(type=4)), (-2, dict(type=-1)), (-3, dict(rows=0)), (-3, dict(rows=1 << 31)), (-4, dict(cols=0)), (-4, dict(cols=1 << 24)),
+    (-1, dict(logits=None)), (-2, dict(type=4)), (-2, dict(type=-1)), (-3, dict(rows=0)), (-3, dict(rows=1 << 31)), (-3, dict(rows=1 << 23)), (-4, dict(cols=0)), (-4, dict(cols=1 << 24)),
     (-5, dict(row_stride=-1)), (-6, dict(col_stride=-1)), (-8, dict(u=None)), (-9, dict(draws=0)), (-10, dict(t=-1.0)), (-10, dict(t=math.nan)), (-10, dict(t=math.inf)),
     (-12, dict(k=-1)), (-14, dict(p=1.5)), (-14, dict(p=math.nan)), (-16, dict(m=-0.5)), (-16, dict(m=2.0)), (-18, dict(index=None)),
     (-20, dict(cols=200_000, scratch=None)), (-21, dict(cols=200_000, doubles=3)), (-21, dict(draws=1000, doubles=3))])
