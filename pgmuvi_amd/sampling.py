@@ -7,7 +7,8 @@ drawn from it differ in proportion to what the data say: top-p keeps the highest
 top-k the best grid points, and a temperature above one spreads the starts of several chains
 (:func:`pgmuvi_amd.mcmc.run_mcmc`, ``initial_values="periodogram"``).
 
-There is no CPU path: tensors on the GPU or an error.  Nothing synchronises the host.
+There is no CPU path: tensors on the GPU or an error.  Nothing synchronises the host, but a setting given as a 0-dim tensor on the
+device (it is read as a number).
 """
 from __future__ import annotations
 

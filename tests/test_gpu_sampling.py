@@ -345,3 +345,30 @@ def test_the_most_rows(dev):
     assert torch.equal(draw_indices(l.expand(n, 2), u), (u >= 0.5).to(torch.int64))
     with pytest.raises(ValueError, match="rows"):
         draw_indices(l.expand(n + 1, 2), torch.zeros(1, dtype=torch.float64, device=dev).expand(n + 1))
+
+
+@pytest.mark.parametrize("rows, cols, S", [(40, 9000, 300), (2, 80_000, 20), (2, 80_000, 5000), (1100, 900, 100)])
+def test_graphs_of_several_launches_replayed(dev, rows, cols, S):
+    """Two captured calls that share a memory pool, replayed in turn with new inputs and eager calls on another stream between."""
+    l, u = _rows(rows, cols, torch.float64, 3).to(dev), torch.rand(rows, S, dtype=torch.float64, device=dev)
+    kws = (dict(top_p=0.8), dict(top_k=700, min_p=0.01))
+    for kw in kws:
+        draw_indices(l, u, **kw)
+    graphs, outs = [], []
+    for kw in kws:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=graphs[0].pool() if graphs else None):
+            outs.append(draw_indices(l, u, return_logprob=True, **kw))
+        graphs.append(g)
+    side = torch.cuda.Stream()
+    for k in range(3):
+        l.copy_(_rows(rows, cols, torch.float64, 60 + k))
+        u.copy_(torch.rand(rows, S, dtype=torch.float64, device=dev))
+        for g, out, kw in zip(graphs, outs, kws):
+            g.replay()
+            got = [x.clone() for x in out]
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                eager = draw_indices(l, u, return_logprob=True, **kw)
+            torch.cuda.current_stream().wait_stream(side)
+            assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1])
