@@ -768,7 +768,8 @@ template <class C, class F> __device__ __forceinline__ void draw_list(const Draw
   }
 }
 // A lower bound of the top_k-th value: the top_k-th highest of the cells' best values, from bins over them (S.best); `lowest` if there
-// are no more cells than that (bounded: false).  Only cells that reach it are looked at again
+// are no more cells than that, or none with anything in them, and the bins are empty then (bounded: false: cut_of counts the row's
+// entries in them).  Only cells that reach the bound are looked at again
 template <class C, class F> __device__ __forceinline__ double bound_of_top_k(const Row<F>& R, Shared<C>& S, int64_t top_k, double lowest, bool& bounded) {
   bounded = false;
   clear_bins<false>(S);
@@ -779,7 +780,7 @@ template <class C, class F> __device__ __forceinline__ double bound_of_top_k(con
   const int shift = shift_of<C>(top - low);
   for (int c = threadIdx.x; c < R.cells; c += C::NT) if (S.best[c] > -INF) atomicAdd(&S.bins.count[(top - key_of(S.best[c])) >> shift], 1u);
   find_bin<false>(S, 0, 0, 0, (u64)top_k, 0.0, 0.0);
-  if (S.found[6] < (u64)top_k) return lowest;
+  if (S.found[6] < (u64)top_k) { clear_bins<false>(S); return lowest; }
   const u64 drop = ((S.found[0] + 1) << shift) - 1;             // (to the lowest pattern of the bin)
   bounded = true;
   return of_key(drop < top - low ? top - drop : low);

@@ -372,3 +372,34 @@ def test_graphs_of_several_launches_replayed(dev, rows, cols, S):
                 eager = draw_indices(l, u, return_logprob=True, **kw)
             torch.cuda.current_stream().wait_stream(side)
             assert torch.equal(got[0], eager[0]) and torch.equal(got[1], eager[1])
+
+
+def _mostly_masked(B, V, dtype, seed, values):
+    """Rows of -inf but for 40 neighbouring entries near the beginning and 40 near the end: fewer cells with an entry than any top_k below."""
+    rng = np.random.default_rng(seed)
+    l = np.full((B, V), -math.inf)
+    for b in range(B):
+        for at in (rng.integers(0, 60), V - 100 + rng.integers(0, 60)):
+            l[b, at:at + 40] = values(rng, 40)
+    return torch.as_tensor(l).to(dtype)
+
+
+@pytest.mark.parametrize("settings", [dict(top_k=5), dict(top_k=30, top_p=0.7), dict(top_k=79, min_p=0.2), dict(top_k=250)], ids=str)
+@pytest.mark.parametrize("B, V", [(3, 9001), (520, 80_000), (1030, 2000), (1, 300_000), (2, 60_000)])
+def test_fewer_cells_with_an_entry_than_top_k(dev, B, V, settings):
+    """... at the lowest end of float64 (the difference to the type's lowest value is below 1e300), where the row's entries are counted in
+    the bins that counted the cells, and in the usual range of every type."""
+    u = torch.as_tensor(np.random.default_rng(V).random((B, 9)))
+    some = sorted({0, B // 2, B - 1})
+    low, step = np.finfo(np.float64).min, 2.0 ** 971             # (the distance of two float64 there)
+    cases = [(torch.float64, lambda rng, n: low + step * rng.integers(0, 1 << 20, n), dict(temperature=2e296)),
+             (torch.float64, lambda rng, n: low + step * rng.integers(0, 3, n), dict(temperature=2e293))]
+    cases += [(dtype, lambda rng, n: rng.normal(0, 3, n), {}) for dtype in TYPES]
+    for dtype, values, kw in cases:
+        l = _mostly_masked(B, V, dtype, B, values)
+        kw = dict(settings, **kw)
+        idx, logp = draw_indices(l.to(dev), u.to(dev), return_logprob=True, **kw)
+        assert int(idx.min()) >= 0
+        _check(l[some], u[some], (idx[some], logp[some]), **kw)
+        each = {k: torch.full((B,), v, dtype=torch.int64 if k == "top_k" else torch.float64, device=dev) for k, v in kw.items()}
+        assert torch.equal(draw_indices(l.to(dev), u.to(dev), **each), idx)
