@@ -2764,12 +2764,14 @@ __device__ __forceinline__ void fit_post_body(const FitDev& F, const FitLoads& L
     g = gth * dth;
   }
   if (L.clip >= 0.0 && t < 64) {
-    // the gradient's norm (P <= 52 entries: wavefront 0 holds them all), scaled by the largest entry so that no square overflows
+    // the gradient's norm (P <= 52 entries: wavefront 0 holds them all), scaled by the largest entry so that no square overflows.  Zero,
+    // an infinity or a NaN as the largest entry is the norm itself (inf / inf would make a NaN of it: a factor of zero is due there)
     double top = fabs(g);
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) { const double v = __shfl_xor(top, s); top = (v > top || v != v) ? v : top; }
-    const double q = top > 0.0 ? g / top : 0.0;
-    const double norm = top > 0.0 ? top * sqrt(wave_sum_dpp(q * q)) : top;
+    const bool scaled = top > 0.0 && top <= 1.7976931348623157e308;
+    const double q = scaled ? g / top : 0.0;
+    const double norm = scaled ? top * sqrt(wave_sum_dpp(q * q)) : top;
     const double c = L.clip / (norm + 1e-6);
     if (!(c >= 1.0)) g *= c;
   }

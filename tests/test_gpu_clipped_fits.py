@@ -250,3 +250,26 @@ def test_chains_without_a_periodogram_and_with_spans_of_their_own(dev):
     kw = dict(noise=e ** 2, num_mixtures=2, num_samples=2, warmup_steps=2, max_tree_depth=2, seed=5, group_by_chain=True)
     with pytest.raises(ValueError, match=r"chains \[2\]"):
         mcmc.run_mcmc(t.unsqueeze(-1), y, initial_values="periodogram", **kw)
+
+
+@pytest.mark.parametrize("n", [60, 300, 1300])
+@pytest.mark.parametrize("optim", ["SGD", "Adam"])
+def test_an_infinite_gradient_gives_every_loop_the_same_step(dev, n, optim):
+    """A prior so narrow that its derivative overflows while its logarithm does not ((1e-10 / 2^-535)^2 / 2 = 6e301, and the
+    variance 2^-1070 is exact): the norm is infinite, the factor zero, and only the infinite entry's parameter becomes NaN."""
+    ends = []
+    for loop, kw in ((train, dict(progress=False)), (train_native, {}), (train_device, {})):
+        m, lik, x, y = _model(dev, n)
+        m.initialize(**{"mean_module.constant": torch.tensor(1e-10, dtype=D, device=dev)})
+        scale = torch.tensor(2.0 ** -535, dtype=D, device=dev)
+        m.mean_module.register_prior("narrow", g.priors.NormalPrior(torch.zeros_like(scale), scale), "constant")
+        start = {k: p.detach().clone() for k, p in m.named_parameters()}
+        r = loop(model=m, likelihood=lik, train_x=x, train_y=y, maxiter=1, lr=0.01, optim=optim, max_grad_norm=0.1, **kw)
+        assert np.isfinite(_losses(r)).all()
+        for k, p in m.named_parameters():
+            if k == "mean_module.raw_constant":
+                assert bool(torch.isnan(p).all()), loop
+            else:
+                assert torch.equal(p.detach(), start[k]), (loop, k)
+        ends.append(_losses(r))
+    assert np.allclose(ends[0], ends[1], rtol=1e-9, atol=0) and np.allclose(ends[0], ends[2], rtol=1e-9, atol=0)
