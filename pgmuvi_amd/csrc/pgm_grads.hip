@@ -405,6 +405,30 @@ bool any_clash(std::vector<Span>& v) {
 }
 
 struct Item { int type; int64_t n; const char* in; char* out; int64_t in_member, out_member; const int64_t* layout; int64_t bytes, chunks; };
+// An array a call touches: runs of `run` bytes at every combination of up to five steps (the member axis and a layout's four
+// dimensions; bytes, largest step first).
+struct Axis { uint64_t size, step; };
+struct Box { Axis a[5]; int n; uint64_t run; };
+
+uint64_t reach_of(const Box& b, int from) {
+  uint64_t r = b.run;
+  for (int d = from; d < b.n; ++d) r += (b.a[d].size - 1) * b.a[d].step;
+  return r;
+}
+// entries at the same address?  (No for sure where every step clears all the smaller ones)
+bool meets_itself(const Box& b) {
+  for (int d = 0; d < b.n; ++d) if (b.a[d].step < reach_of(b, d + 1)) return true;
+  return false;
+}
+Box box_of(const Item& it, int batch, bool write) {
+  const int s = type_bytes(it.type), o = write ? 8 : 4;
+  Box b{{}, 0, (uint64_t)(it.layout ? s : it.bytes)};
+  auto axis = [&](int64_t size, int64_t step) { if (size > 1) b.a[b.n++] = Axis{(uint64_t)size, (uint64_t)step * s}; };
+  axis(batch, write ? it.out_member : it.in_member);
+  if (it.layout) for (int d = 0; d < 4; ++d) axis(it.layout[d], it.layout[o + d]);
+  std::sort(b.a, b.a + b.n, [](const Axis& x, const Axis& y) { return x.step > y.step; });
+  return b;
+}
 
 // One workgroup per member, in one launch: few tensors (one after the other, more take longer than two launches) of no more bytes
 // than a CU streams in the time a second launch takes, or, with members for half the chip, than its registers hold.  GPU times in
@@ -456,8 +480,7 @@ int run_clip(int batch, int count, const uint64_t* in, const uint64_t* out, cons
       if (it.layout) for (int d = 0; d < 4; ++d) same = same && L[4 + d] == L[8 + d];
       if (!same) span(in[t], it.in_member, 4, false);
       span(out[t], it.out_member, 8, true);
-      if (batch > 1 && !it.layout && it.out_member < it.n) return -12;          // (members written over each other)
-      if (batch > 1 && it.layout && it.out_member == 0) return -12;
+      if (meets_itself(box_of(it, batch, true))) return -12;     // (entries, or members, written over each other)
     }
   }
   if (out && any_clash(spans)) return -12;

@@ -120,3 +120,18 @@ def test_scratch_covers_every_launch():
         for count in (1, 64, 65, 5000):
             assert need(batch, count, 1 << 24, 0) >= 3 * (2048 + batch * (count // 64 + 1))
             assert need(batch, count, 64, 1) >= 3 * (2048 + batch * (count // 24 + 1))
+
+
+# ---- what may share memory (layouts are never one launch, so that a call without scratch ends with -13 where it is not refused) -------
+SHARED, DISTINCT = -12, -13
+
+
+@pytest.mark.parametrize("kw", [
+    dict(src=[A], dst=[A], numel=[4], types=[0], layout=[[1, 1, 1, 4, 0, 0, 0, 1, 0, 0, 0, 1]], batch=3, member=[[2, 2]]),     # members two apart, of four entries
+    dict(src=[A], dst=[A], numel=[4], types=[0], layout=[[1, 1, 2, 2, 0, 0, 1, 8, 0, 0, 1, 8]], batch=9, member=[[1, 1]]),     # ... reaching each other's second column
+    dict(src=[A], dst=[A], numel=[6], types=[0], layout=[[1, 1, 2, 3, 0, 0, 3, 1, 0, 0, 0, 1]]),                               # an expanded output
+    dict(src=[A], dst=[A], numel=[6], types=[0], layout=[[1, 1, 2, 3, 0, 0, 2, 1, 0, 0, 2, 1]]),                               # rows that overlap by one
+    dict(src=[A], dst=[A], numel=[4], types=[0], layout=[[1, 1, 1, 4, 0, 0, 0, 2, 0, 0, 0, 2]], batch=3, member=[[8, 0]]),     # one output for all members
+])
+def test_outputs_written_over_themselves_are_refused(kw):
+    assert _clip(scratch=None, **kw) == SHARED
