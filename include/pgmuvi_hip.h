@@ -361,7 +361,8 @@ int pgm_lomb_scargle_fast_f64(const double* t, const double* y, const double* dy
  * that is 0; bytes: of one member's gradients together, strided: is there a layout_host).
  * Sums are fp64; fp64 tensors' squares are held in three ranges, so that the norm neither overflows nor vanishes where the
  * result does not.  A NaN norm makes every output NaN, an infinite one zero (NaN where the gradient is infinite).  Memory that
- * is written must not be shared with another tensor of the call (-12; interleaved columns of one buffer are fine).
+ * is written must not be shared with another tensor of the call, nor by two entries of one (-12).  Columns, rows and blocks of one
+ * buffer are fine; arrays that mesh without meeting in other ways (steps that no common period divides into disjoint parts) are refused.
  * Nothing is kept between calls; the call may be captured.  -98: out of host memory.
  * norm and scratch lie outside the tensors.
  */

@@ -385,28 +385,8 @@ __global__ __launch_bounds__(NT) void k_scale_strided(StridedTable T, int groups
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
-// May two of the arrays a clipping call touches share memory where one of them is written?  Every array is `batch` runs of
-// `run` bytes `step` bytes apart (step 0: one run), or -- loose -- something inside [lo, hi).
-struct Span { uint64_t lo, hi, run, step; bool write, loose; };
-
-bool clash(const Span& a, const Span& b) {                       // a.lo <= b.lo < a.hi
-  if (!a.write && !b.write) return false;
-  if (a.loose || b.loose || a.step != b.step || a.step == 0) return true;
-  // interleaved rows of one buffer (columns of a (batch, k) gradient array): disjoint within the common step
-  const uint64_t d = (b.lo - a.lo) % a.step;
-  return !(a.run <= d && d + b.run <= a.step);
-}
-bool any_clash(std::vector<Span>& v) {
-  std::sort(v.begin(), v.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
-  for (size_t i = 0; i < v.size(); ++i)
-    for (size_t j = i + 1; j < v.size() && v[j].lo < v[i].hi; ++j)
-      if (clash(v[i], v[j])) return true;
-  return false;
-}
-
-struct Item { int type; int64_t n; const char* in; char* out; int64_t in_member, out_member; const int64_t* layout; int64_t bytes, chunks; };
-// An array a call touches: runs of `run` bytes at every combination of up to five steps (the member axis and a layout's four
-// dimensions; bytes, largest step first).
+// May two of the arrays a clipping call touches share memory where one of them is written?  An array is runs of `run` bytes at every
+// combination of up to five steps (the member axis and a layout's four dimensions; bytes, largest step first): [lo, lo + reach) holds it.
 struct Axis { uint64_t size, step; };
 struct Box { Axis a[5]; int n; uint64_t run; };
 
@@ -420,6 +400,21 @@ bool meets_itself(const Box& b) {
   for (int d = 0; d < b.n; ++d) if (b.a[d].step < reach_of(b, d + 1)) return true;
   return false;
 }
+// Disjoint for sure?  `a` from its axis i on, at zero, and `b` from its axis j on, `at` bytes behind (or, negative, in front).  Over the
+// largest step both are laid out in, each lies within one period of it or may reach into the next one: the rests are compared within
+// the period they share, and one further.  (Columns of a matrix, blocks of a grid, members' rows in one buffer.)
+bool apart(const Box& a, int i, const Box& b, int j, int64_t at) {
+  const int64_t ra = (int64_t)reach_of(a, i), rb = (int64_t)reach_of(b, j);
+  if (at >= ra || -at >= rb) return true;
+  const uint64_t sa = i < a.n ? a.a[i].step : 0, sb = j < b.n ? b.a[j].step : 0;
+  const int64_t step = (int64_t)(sa > sb ? sa : sb);
+  if (step == 0) return false;                                  // (two runs that meet)
+  const int i2 = sa == (uint64_t)step ? i + 1 : i, j2 = sb == (uint64_t)step ? j + 1 : j;
+  if ((int64_t)reach_of(a, i2) > step || (int64_t)reach_of(b, j2) > step) return false;       // (interleaved otherwise: not decided here)
+  const int64_t d = ((at % step) + step) % step;
+  return apart(a, i2, b, j2, d) && apart(a, i2, b, j2, d - step);
+}
+struct Item { int type; int64_t n; const char* in; char* out; int64_t in_member, out_member; const int64_t* layout; int64_t bytes, chunks; };
 Box box_of(const Item& it, int batch, bool write) {
   const int s = type_bytes(it.type), o = write ? 8 : 4;
   Box b{{}, 0, (uint64_t)(it.layout ? s : it.bytes)};
@@ -428,6 +423,15 @@ Box box_of(const Item& it, int batch, bool write) {
   if (it.layout) for (int d = 0; d < 4; ++d) axis(it.layout[d], it.layout[o + d]);
   std::sort(b.a, b.a + b.n, [](const Axis& x, const Axis& y) { return x.step > y.step; });
   return b;
+}
+struct Span { uint64_t lo, hi; const Item* it; bool write; };
+bool any_clash(std::vector<Span>& v, int batch) {
+  std::sort(v.begin(), v.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+  for (size_t i = 0; i < v.size(); ++i)
+    for (size_t j = i + 1; j < v.size() && v[j].lo < v[i].hi; ++j)
+      if ((v[i].write || v[j].write) &&
+          !apart(box_of(*v[i].it, batch, v[i].write), 0, box_of(*v[j].it, batch, v[j].write), 0, (int64_t)(v[j].lo - v[i].lo))) return true;
+  return false;
 }
 
 // One workgroup per member, in one launch: few tensors (one after the other, more take longer than two launches) of no more bytes
@@ -443,7 +447,6 @@ int run_clip(int batch, int count, const uint64_t* in, const uint64_t* out, cons
              const int64_t* member, const int64_t* layout, int p, double max_norm, void* norm, int norm_f64, double* scratch,
              int64_t scratch_doubles, hipStream_t st) {
   std::vector<Item> flat, loose;
-  std::vector<Span> spans;
   int64_t per_member = 0, flat_chunks = 0, loose_chunks = 0;
   for (int t = 0; t < count; ++t) {
     if (numel[t] < 0) return -5;
@@ -469,21 +472,21 @@ int run_clip(int batch, int count, const uint64_t* in, const uint64_t* out, cons
       flat.push_back(it); flat_chunks += it.chunks;
     }
     per_member += it.bytes;
-    if (out) {
-      auto span = [&](uint64_t at, int64_t step, int o, bool write) {
-        int64_t last = it.layout ? 0 : it.n - 1;
-        if (it.layout) for (int d = 0; d < 4; ++d) last += (L[d] - 1) * L[o + d];
-        const uint64_t run = (uint64_t)(last + 1) * s;
-        spans.push_back(Span{at, at + (uint64_t)(batch - 1) * step * s + run, run, batch > 1 ? (uint64_t)step * s : 0, write, it.layout != nullptr});
-      };
-      bool same = in[t] == out[t] && it.in_member == it.out_member;
-      if (it.layout) for (int d = 0; d < 4; ++d) same = same && L[4 + d] == L[8 + d];
-      if (!same) span(in[t], it.in_member, 4, false);
-      span(out[t], it.out_member, 8, true);
-      if (meets_itself(box_of(it, batch, true))) return -12;     // (entries, or members, written over each other)
-    }
   }
-  if (out && any_clash(spans)) return -12;
+  if (out) {
+    std::vector<Span> spans;
+    spans.reserve(2 * (flat.size() + loose.size()));
+    for (const std::vector<Item>* items : {&flat, &loose})
+      for (const Item& it : *items) {
+        const Box to = box_of(it, batch, true);
+        if (meets_itself(to)) return -12;                        // (entries, or members, written over each other)
+        bool same = it.in == it.out && (batch == 1 || it.in_member == it.out_member);
+        if (it.layout) for (int d = 0; d < 4; ++d) same = same && (it.layout[d] == 1 || it.layout[4 + d] == it.layout[8 + d]);
+        if (!same) spans.push_back(Span{(uint64_t)it.in, (uint64_t)it.in + reach_of(box_of(it, batch, false), 0), &it, false});
+        spans.push_back(Span{(uint64_t)it.out, (uint64_t)it.out + reach_of(to, 0), &it, true});
+      }
+    if (any_clash(spans, batch)) return -12;
+  }
   if (flat_chunks > (1 << 30) || loose_chunks > (1 << 30)) return -5;
   const int scale = out ? 1 : 0;
 

@@ -148,7 +148,8 @@ def _run(tensors, outs, max_norm, norm_type, members, what):
         rc = lib.pgm_grad_clip(members, count, _address(src), _address(dst), _address(numel), bytes(types), _address(member), _address(layout), p,
                                max_norm, norm.data_ptr(), f64, None if scratch is None else scratch.data_ptr(), n, _hip.stream_of(dev.index))
     if rc == -12:
-        raise ValueError(f"{what}: tensors that share memory cannot be clipped together (the same gradient given twice?)")
+        raise ValueError(f"{what}: tensors that share memory, or mesh in ways other than columns, rows and blocks of one buffer, cannot be clipped "
+                         "together (the same gradient given twice?)")
     _hip._check(rc, "pgm_grad_clip")
     return norm
 

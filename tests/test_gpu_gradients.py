@@ -315,3 +315,27 @@ def test_the_most_members(dev):
     assert float(g.norm(dim=1).max()) <= 1.0 + 2.0 ** -50
     with pytest.raises(ValueError, match="members"):
         G.total_norm([torch.zeros(1, 1, device=dev).expand(n + 1, 1)], members=True)
+
+
+@pytest.mark.parametrize("dtype", list(HALF_STEP))
+def test_columns_and_blocks_of_one_buffer(dev, dtype):
+    """Views that lie between each other's rows but share no entry are clipped as torch clips them, in place and into such views."""
+    cuts = [lambda m: [m[:, :4], m[:, 4:]], lambda m: [m[:, 9:], m[:, 2:9]], lambda m: [m[::2], m[1::2]], lambda m: [m[:30, :5], m[30:, :5], m[:30, 5:], m[30:, 5:]],
+            lambda m: [m[7, :3], m[:, 3:], m[:7, :3]], lambda m: list(m.t().split(3)), lambda m: [m.view(5, 10, 13)[:, 2:5, ::2], m.view(5, 10, 13)[:, 5:, 1:]]]
+    for k, cut in enumerate(cuts):
+        buf = _make([(50, 13)], dtype, 40 + k, dev=dev)[0]
+        ref = buf.clone()
+        before = [_cpu(t) for t in cut(ref)]
+        outs = torch.full_like(buf, 7.0)
+        norm = G.clip_grads_(cut(buf), 0.2, out=cut(outs))
+        _check_clip(None, cut(outs), before, norm, 0.2)
+        assert torch.equal(buf, ref)
+        got = G.clip_grads_(cut(buf), 0.2)
+        assert torch.equal(got, norm)
+        _check_clip(None, cut(buf), before, got, 0.2)
+        mark = torch.zeros(50, 13, dtype=torch.int64, device=dev)
+        for t in cut(mark):
+            t.add_(1)
+        assert int(mark.max()) == 1 and torch.equal(buf[mark == 0], ref[mark == 0])          # (what belongs to nobody stays)
+        with pytest.raises(ValueError, match="share memory"):
+            G.clip_grads_(cut(buf) + [buf[:, 3:5]], 0.2)

@@ -135,3 +135,70 @@ SHARED, DISTINCT = -12, -13
 ])
 def test_outputs_written_over_themselves_are_refused(kw):
     assert _clip(scratch=None, **kw) == SHARED
+
+
+def _addresses(base, size, stride, batch, member):
+    n = [batch] + list(size)
+    st = [member] + list(stride)
+    at = np.zeros(1, dtype=np.int64) + base
+    for k, s in zip(n, st):
+        at = (at[:, None] + np.arange(k) * s).ravel()
+    return at
+
+
+def _strided_call(boxes, batch):
+    """In-place clip of (first entry, sizes, strides, member stride) of one fp64 buffer; an output given twice or overlapping -> SHARED."""
+    layout = [list(size) + list(stride) + list(stride) for _, size, stride, _ in boxes]
+    src = [A + 8 * b for b, _, _, _ in boxes]
+    numel = [int(np.prod(size)) for _, size, _, _ in boxes]
+    return _clip(src=src, dst=src, numel=numel, types=[0] * len(boxes), layout=layout, batch=batch, member=[[m, m] for _, _, _, m in boxes], scratch=None)
+
+
+def test_no_two_entries_at_one_address_are_let_through():
+    """Random layouts against the addresses themselves.  (The check may refuse entries that mesh without meeting, never the reverse.)"""
+    rng = np.random.default_rng(0)
+    let = met = 0
+    for _ in range(20_000):
+        batch = int(rng.choice([1, 1, 2, 3]))
+        boxes = []
+        for _ in range(int(rng.integers(1, 4))):
+            size = [int(v) for v in rng.integers(1, 4, 4) * (rng.random(4) < 0.5) + 1]
+            stride = [int(v) for v in rng.choice([0, 1, 2, 3, 4, 6, 8, 12, 24, 48, 49], 4, p=[0.02] + [0.098] * 10)]
+            boxes.append((int(rng.integers(0, 200)), size, stride, int(rng.choice([1, 5, 24, 96, 200, 400]))))
+        at = np.concatenate([_addresses(b, s, st, batch, m) for b, s, st, m in boxes])
+        meets = len(np.unique(at)) < len(at)
+        rc = _strided_call(boxes, batch)
+        assert rc in (SHARED, DISTINCT)
+        assert rc == SHARED or not meets, (batch, boxes)
+        let += rc == DISTINCT
+        met += meets
+    assert let > 2000 and met > 2000                             # (the test reaches both)
+
+
+def test_columns_rows_and_blocks_of_one_buffer_are_let_through():
+    rng = np.random.default_rng(1)
+    for _ in range(500):
+        # a grid cut along every axis, all blocks of it (sizes of one and whole axes among them), the members' axis first or last
+        dims = [int(v) for v in rng.integers(1, 7, 3)]
+        batch = int(rng.choice([1, 1, 4]))
+        inner = int(np.prod(dims))
+        if batch > 1 and rng.random() < 0.5:
+            stride, member = [dims[1] * dims[2] * batch, dims[2] * batch, batch], 1                # [..., member]
+        else:
+            stride, member = [dims[1] * dims[2], dims[2], 1], inner                                # [member, ...]
+        cuts = [sorted({0, n, *(int(v) for v in rng.integers(0, n + 1, 2))}) for n in dims]
+        boxes = []
+        for a, b in zip(cuts[0], cuts[0][1:]):
+            for c, d in zip(cuts[1], cuts[1][1:]):
+                for e, f in zip(cuts[2], cuts[2][1:]):
+                    boxes.append((a * stride[0] + c * stride[1] + e * stride[2], [1, b - a, d - c, f - e], [0] + stride, member))
+        order = rng.permutation(len(boxes))
+        assert _strided_call([boxes[k] for k in order], batch) == DISTINCT, (dims, cuts, batch)
+        twice = boxes + [boxes[int(rng.integers(0, len(boxes)))]]
+        assert _strided_call(twice, batch) == SHARED
+    even, odd = (0, [1, 1, 5, 8], [0, 0, 16, 1], 0), (8, [1, 1, 5, 8], [0, 0, 16, 1], 0)
+    assert _strided_call([even, odd], 1) == DISTINCT             # every other row each
+    # columns of two types in one buffer of bytes (the size of an entry differs, the row does not)
+    layout = [[1, 1, 6, 4, 0, 0, 6, 1, 0, 0, 6, 1], [1, 1, 6, 4, 0, 0, 12, 1, 0, 0, 12, 1]]
+    assert _clip(src=[A, A + 32], dst=[A, A + 32], numel=[24, 24], types=[0, 1], layout=layout, scratch=None) == DISTINCT
+    assert _clip(src=[A, A + 28], dst=[A, A + 28], numel=[24, 24], types=[0, 1], layout=layout, scratch=None) == SHARED
