@@ -356,11 +356,12 @@ int pgm_lomb_scargle_fast_f64(const double* t, const double* y, const double* dy
  *   member_host         [count][2] distance between members of in / out, in entries (may be NULL for batch 1);
  *   layout_host         NULL, or [count][12]: four sizes, four strides of in, four of out (entries, outermost first) of a tensor
  *                       whose entries per member are not one contiguous run; first size 0 = they are.
- * p: 1, 2 or 0 (largest magnitude).  max_norm >= 0 (infinity: nothing is clipped).  norm: [batch] fp64 (norm_f64 != 0) or fp32,
+ * p: 1, 2 or 0 (largest magnitude).  max_norm >= 0 (infinity: no limit, out = g whatever the norm).  norm: [batch] fp64 (norm_f64 != 0) or fp32,
  * device.  scratch: pgm_grad_scratch_doubles doubles of device memory owned by the caller, used by this call only (NULL where
  * that is 0; bytes: of one member's gradients together, strided: is there a layout_host).
  * Sums are fp64; fp64 tensors' squares are held in three ranges, so that the norm neither overflows nor vanishes where the
- * result does not.  A NaN norm makes every output NaN, an infinite one zero (NaN where the gradient is infinite).  Memory that
+ * result does not.  Under a finite max_norm a NaN norm makes every output NaN, an infinite one zero (NaN where the gradient is
+ * infinite); the factor is a double, with fewer bits below 2^-1022.  Memory that
  * is written must not be shared with another tensor of the call, nor by two entries of one (-12).  Columns, rows and blocks of one
  * buffer are fine; arrays that mesh without meeting in other ways (steps that no common period divides into disjoint parts) are refused.
  * Nothing is kept between calls; the call may be captured.  -98: out of host memory.

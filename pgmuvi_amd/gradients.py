@@ -166,7 +166,8 @@ def clip_grads_(grads, max_norm: float, norm_type: float = 2.0, out=None, member
     """Scales gradients to a norm of at most ``max_norm``, in place or into ``out`` (tensors of the same shapes and types),
     and returns the norm they had (see :func:`total_norm`).  ``members``: one norm and one factor for every index of the
     leading axis.  The factor is ``min(1, max_norm / (norm + 1e-6))``; a NaN norm makes the gradients NaN, an infinite one
-    zero.  ``error_if_nonfinite``: raise instead, with the gradients untouched (waits for the norm)."""
+    zero (NaN where the gradient is infinite).  An infinite ``max_norm`` is no limit: the gradients stay as they are, whatever
+    their norm.  ``error_if_nonfinite``: raise where the norm is not finite, with the gradients untouched (waits for the norm)."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grads_: max_norm must not be negative, got {max_norm}")

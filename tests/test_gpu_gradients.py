@@ -339,3 +339,24 @@ def test_columns_and_blocks_of_one_buffer(dev, dtype):
         assert int(mark.max()) == 1 and torch.equal(buf[mark == 0], ref[mark == 0])          # (what belongs to nobody stays)
         with pytest.raises(ValueError, match="share memory"):
             G.clip_grads_(cut(buf) + [buf[:, 3:5]], 0.2)
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, 3.0])
+@pytest.mark.parametrize("n", [9, 50_000])
+def test_no_limit_leaves_the_gradients_as_they_are(dev, n, value):
+    """... whatever their norm, in place and out of place, for one model, per member and for strided tensors."""
+    for members in (False, True):
+        grads = _make([(4, n), (4, 3)], torch.float64, 2, dev=dev)
+        grads[0][1, n // 3] = value
+        grads.append(grads[1].t().contiguous().t())
+        ref = [g.clone() for g in grads]
+        outs = [torch.zeros_like(g) for g in grads]
+        norm = G.clip_grads_(grads, math.inf, out=outs, members=members)
+        assert torch.equal(torch.isnan(norm), torch.isnan(G.total_norm(grads, members=members)))
+        G.clip_grads_(grads, math.inf, members=members)
+        for a, b, o in zip(grads, ref, outs):
+            for got in (a, o):
+                assert torch.equal(torch.isnan(got), torch.isnan(b)) and torch.equal(torch.nan_to_num(got), torch.nan_to_num(b))
+        if not math.isfinite(value):
+            with pytest.raises(RuntimeError, match="not finite"):
+                G.clip_grads_(grads, math.inf, members=members, error_if_nonfinite=True)
