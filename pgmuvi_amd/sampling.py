@@ -29,7 +29,7 @@ def _setting(value, off, lo, hi, name, rows, dev, dtype):
         _hip.require_gpu(value, "draw_indices")
         if dtype is torch.int64 and value.dtype.is_floating_point:
             raise TypeError(f"draw_indices: {name} takes whole numbers")
-        t = value.detach().to(device=dev, dtype=dtype).contiguous()
+        t = value.detach().to(device=dev, dtype=dtype).resolve_neg().contiguous()
         return off, t.data_ptr(), t
     number = int(value) if dtype is torch.int64 else float(value)
     if not lo <= number <= hi or (dtype is torch.int64 and number != value):

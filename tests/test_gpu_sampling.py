@@ -403,3 +403,15 @@ def test_fewer_cells_with_an_entry_than_top_k(dev, B, V, settings):
         _check(l[some], u[some], (idx[some], logp[some]), **kw)
         each = {k: torch.full((B,), v, dtype=torch.int64 if k == "top_k" else torch.float64, device=dev) for k, v in kw.items()}
         assert torch.equal(draw_indices(l.to(dev), u.to(dev), **each), idx)
+
+
+def test_settings_that_are_negated_views(dev):
+    """(One row's view is contiguous as it is, so that nothing on the way copies it.)"""
+    for rows in (1, 3):
+        l = _rows(rows, 600, torch.float64, 8).to(dev)
+        u = torch.as_tensor(np.random.default_rng(2).random((rows, 40)), device=dev)
+        for name, v in (("temperature", [0.5, 2.0, 1.0]), ("top_p", [0.5, 0.9, 0.3]), ("min_p", [0.1, 0.02, 0.5])):
+            v = torch.tensor(v[:rows], dtype=torch.float64, device=dev)
+            view = torch.complex(torch.zeros_like(v), -v).conj().imag
+            assert view.is_neg() and torch.equal(view, v)
+            assert torch.equal(draw_indices(l, u, **{name: view}), draw_indices(l, u, **{name: v}))
