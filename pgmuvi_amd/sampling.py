@@ -7,8 +7,9 @@ drawn from it differ in proportion to what the data say: top-p keeps the highest
 top-k the best grid points, and a temperature above one spreads the starts of several chains
 (:func:`pgmuvi_amd.mcmc.run_mcmc`, ``initial_values="periodogram"``).
 
-There is no CPU path: tensors on the GPU or an error.  Nothing synchronises the host, but a setting given as a 0-dim tensor on the
-device (it is read as a number).
+There is no CPU path: tensors on the GPU or an error.  Nothing synchronises the host but a setting given as a 0-dim tensor on the
+device (it is read as a number) and ``lengths`` given on the host (they are copied): a call that is captured gives numbers or (B,)
+tensors on the device.  Neither the indices nor the log-probabilities carry a gradient.
 """
 from __future__ import annotations
 
@@ -46,11 +47,12 @@ def draw_indices(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=N
     (value descending, index ascending): ``top_k`` keeps the first k entries, ``top_p`` the shortest beginning of those that
     holds at least that share of their weight, ``min_p`` the entries of that with a weight of at least ``min_p`` times the
     best one's.  The index is the first kept one, in index order, whose running weight exceeds ``u`` times the kept weight.
-    ``temperature`` 0 takes the best entry.  Each of the four is a number (``None``: off) or a (B,) tensor.  ``lengths`` (B,):
-    entries of each row; the rest is not read.  Entries of -inf or NaN are never drawn.
+    ``temperature`` 0 takes the best entry.  Each of the four is a number (``None``: off) or a (B,) tensor.  ``lengths`` (B,)
+    whole numbers, on the device or the host: entries of each row; the rest is not read.  Entries of -inf or NaN are never drawn.
 
     Returns int64 indices of the shape of ``u`` (-1 where a row has nothing to draw), with ``return_logprob`` also the
-    float64 log-probabilities of the draws under the truncated distribution (-inf there)."""
+    float64 log-probabilities of the draws under the truncated distribution (-inf there), outside any autograd graph: a loss on
+    them differentiates its own expression of the logits at the indices."""
     if not torch.is_tensor(logits) or logits.dtype not in _TYPE or logits.layout is not torch.strided:
         raise TypeError("draw_indices: logits must be a dense float64, float32, bfloat16 or float16 tensor")
     if not torch.is_tensor(u) or u.dtype not in _TYPE:
