@@ -539,6 +539,27 @@ def _start_frequencies(t, y, dy, num, seed, chains):
     return torch.cat([draw_frequencies(t[r], y[r], None if dy is None else dy[r], u[r], top_p=0.95)[0] for r in rows]).cpu().numpy()
 
 
+def _checked_starts(pot, seed, chains, total, world, group):
+    """:func:`_start_frequencies` of a rank's chains.  A chain without any is an error on every rank of the job, its own or not: the
+    others would wait for this one's draws."""
+    from .batch import gather_logliks
+    failure = None
+    try:
+        freqs = _start_frequencies(pot.x[..., 0], pot.y, None if pot.noise is None else pot.noise.sqrt(), pot.Q, seed, chains)
+    except Exception as e:                       # (a light curve whose points share one time has no grid of frequencies)
+        failure, freqs = e, np.full((len(chains), pot.Q), np.nan)
+    some = torch.as_tensor(np.isfinite(freqs).all(1), dtype=torch.float64, device=pot.device)
+    if world > 1:
+        some = gather_logliks(some, total, group)
+    if failure is not None:
+        raise failure
+    if not bool(some.all()):
+        first = 0 if world > 1 else chains[0]
+        raise ValueError("initial_values='periodogram': no finite periodogram (a constant light curve?) for chains "
+                         f"{[first + int(c) for c in np.flatnonzero(some.cpu().numpy() == 0.0)]}")
+    return freqs
+
+
 def run_mcmc(x, y, noise=None, num_mixtures=4, sampler="NUTS", num_samples=500, warmup_steps=100, num_chains=1, seed=0,
              initial_values=None, priors=None, dim_order=0, group=None, compute=None,
              group_by_chain=False, **sampler_kwargs):
@@ -548,7 +569,8 @@ def run_mcmc(x, y, noise=None, num_mixtures=4, sampler="NUTS", num_samples=500, 
     ``y`` (N,) -> ``num_chains`` chains on that light curve; ``y`` (C,N) -> one chain per row (config 5: each chain its own
     light curve).  With ``torch.distributed`` initialised the chains are block-partitioned over the ranks
     (``batch.shard_bounds``), each rank advances its chains with batched evaluations on its own GPU, and one
-    ``all_gather`` of the draws closes the run (the only collective).  ``initial_values``: a dictionary of sites, None (pyro's
+    ``all_gather`` of the draws closes the run (the only collective, but for one of a flag per chain before starts from the
+    periodogram).  ``initial_values``: a dictionary of sites, None (pyro's
     uniform start) or ``"periodogram"`` -- the same, but every chain's mixture means start on frequencies drawn from the 95 %
     highest-density set of its Lomb-Scargle periodogram, so that the chains start on the light curve's own peaks and not all on
     the same one (one input dimension; GPU).  Returns pyro-style ``{site name: draws}`` with
@@ -585,10 +607,7 @@ def run_mcmc(x, y, noise=None, num_mixtures=4, sampler="NUTS", num_samples=500, 
             if initial_values is not None:   # 'periodogram': the mixture means start on draws from the frequency posterior
                 if pot.d != 1:
                     raise NotImplementedError("initial_values='periodogram' needs light curves with one input dimension")
-                freqs = _start_frequencies(pot.x[..., 0], pot.y, None if pot.noise is None else pot.noise.sqrt(), pot.Q, seed, range(lo, hi))
-                if not np.isfinite(freqs).all():
-                    raise ValueError("initial_values='periodogram': no finite periodogram (a constant light curve?) for chains "
-                                     f"{[lo + int(c) for c in np.flatnonzero(~np.isfinite(freqs).all(1))]}")
+                freqs = _checked_starts(pot, seed, range(lo, hi), C, world, group)
                 z0[:, pot.slices()["covar_module.mixture_means_prior"]] = np.log(freqs)
         res = sample(pot, z0, num_samples, warmup_steps, sampler, seed, chain_ids=range(lo, hi), **sampler_kwargs)
         P = pot.P

@@ -198,3 +198,43 @@ def test_effective_sample_size_on_known_chains():
             z[c, t] = 0.9 * z[c, t - 1] + rng.standard_normal()
     ar = float(mcmc.effective_sample_size(z[:, :, None])[0])
     assert 120 < ar < 350, ar                                     # 4000 * 0.0526 = 210
+
+
+def _dead_chain_worker(rank, world, rendezvous, q, how):
+    import _oracle_backend as ob
+    dist.init_process_group("gloo", init_method="file://" + rendezvous, rank=rank, world_size=world)
+    x, y, nz = _lightcurves(3, 32)
+
+    def starts(t, y, dy, num, seed, chains):      # (the periodogram is the GPU's: chain 2, on the last rank, has none)
+        if how == "raises" and 2 in chains:
+            raise ZeroDivisionError("float division by zero")
+        return np.array([[np.nan if c == 2 else 0.01] * num for c in chains])
+
+    mcmc._start_frequencies = starts
+    try:
+        mcmc.run_mcmc(x, y, nz, num_mixtures=1, num_samples=2, warmup_steps=2, seed=1, compute=ob.mll_value_grad, max_tree_depth=2,
+                      initial_values="periodogram")
+        q.put((rank, "no error"))
+    except Exception as e:
+        q.put((rank, f"{type(e).__name__}: {e}"))
+    dist.barrier()                                 # (every rank is here: nobody waits in a collective of the run)
+    dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("how", ["nan", "raises"])
+def test_a_chain_without_a_start_is_an_error_on_every_rank(tmp_path, how):
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_dead_chain_worker, args=(r, 2, str(tmp_path / "rendezvous"), q, how)) for r in range(2)]
+    for p in procs:
+        p.start()
+    try:
+        got = dict(q.get(timeout=90) for _ in range(2))
+    finally:
+        for p in procs:
+            p.join(20)
+            if p.is_alive():
+                p.kill()
+    assert "chains [2]" in got[0] and got[0].startswith("ValueError")
+    assert got[1].startswith("ZeroDivisionError") if how == "raises" else got[1] == got[0]
+    assert all(p.exitcode == 0 for p in procs)
