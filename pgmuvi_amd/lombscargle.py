@@ -210,7 +210,7 @@ def _shared_grid(t, y, nyquist_factor, samples_per_peak):
 
 
 def draw_frequencies(t: torch.Tensor, y: torch.Tensor, dy: Optional[torch.Tensor], u: torch.Tensor, temperature=1.0, top_k=None,
-                     top_p=None, min_p=None, nyquist_factor=5, samples_per_peak=5):
+                     top_p=None, min_p=None, nyquist_factor=5, samples_per_peak=5, distinct=False):
     """Frequencies drawn from the periodograms of light curves (B, N) that share one sampling span, one for each of the uniform
     random numbers ``u`` (B, S): starts for several fits or chains that differ in proportion to what the data say, where
     :func:`seed_frequencies` always returns the highest peaks.
@@ -218,15 +218,29 @@ def draw_frequencies(t: torch.Tensor, y: torch.Tensor, dy: Optional[torch.Tensor
     The log odds of a grid frequency are ``-log FAP_single = -(n - 3) / 2 log(1 - P)`` (:meth:`LombScargle.false_alarm_probability`,
     'single': the likelihood ratio of a sinusoid of that frequency, its amplitude and the noise level fitted).  ``top_p`` keeps the
     smallest set of frequencies with that share of the posterior, ``min_p`` those within a likelihood ratio of the best,
-    ``top_k`` the k best, ``temperature`` > 1 flattens it (:func:`pgmuvi_amd.sampling.draw_indices`).  Returns (freqs (B, S),
-    their log-probabilities (B, S), grid), all on the device; NaN where a light curve has no finite periodogram."""
+    ``top_k`` the k best, ``temperature`` > 1 flattens it (:func:`pgmuvi_amd.sampling.draw_indices`).  The odds of a clear period leave
+    one frequency, or a few beside it, in any such set.  ``distinct``: a light curve's frequencies are drawn one after the other,
+    each from what is left more than a peak's width (``samples_per_peak`` grid points, 1 / span) from the earlier ones, the set anew
+    each time -- from the whole periodogram again where nothing is left.  Returns (freqs (B, S), their log-probabilities (B, S) in the
+    distribution each was drawn from, grid), all on the device; NaN where a light curve has no finite periodogram."""
     from .sampling import draw_indices
     if y.shape[-1] < 4:
         raise ValueError(f"draw_frequencies: light curves of at least four points, got {y.shape[-1]}")      # (the odds' power: (n - 3) / 2)
+    if distinct and u.dim() != 2:
+        raise ValueError(f"draw_frequencies: u must be (B, S) for distinct frequencies, got {tuple(u.shape)}")
     grid = _shared_grid(t, y, nyquist_factor, samples_per_peak)
     P = periodogram_batched(t, y, dy, grid)
     odds = torch.log1p(-P.clamp(max=1.0 - 2.0 ** -52)).mul_(-0.5 * (y.shape[-1] - 3))      # (a noiseless sinusoid's P rounds to one)
-    index, logp = draw_indices(odds, u, temperature, top_k, top_p, min_p, return_logprob=True)
+    if not distinct:
+        index, logp = draw_indices(odds, u, temperature, top_k, top_p, min_p, return_logprob=True)
+    else:
+        place, left, draws = torch.arange(grid.numel(), device=grid.device), odds, []
+        for s in range(u.shape[1]):
+            if s:
+                left = left.masked_fill((place - draws[-1][0]).abs() <= samples_per_peak, float("-inf"))
+                left = torch.where((left > float("-inf")).any(1, keepdim=True), left, odds)
+            draws.append(draw_indices(left, u[:, s:s + 1], temperature, top_k, top_p, min_p, return_logprob=True))
+        index, logp = (torch.cat(c, 1) for c in zip(*draws)) if draws else draw_indices(odds, u, return_logprob=True)
     freqs = torch.where(index >= 0, grid[index.clamp(min=0)], torch.full((), float("nan"), dtype=grid.dtype, device=grid.device))
     return freqs, logp, grid
 

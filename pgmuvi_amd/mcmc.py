@@ -529,14 +529,14 @@ def effective_sample_size(x: np.ndarray) -> np.ndarray:
 
 
 def _start_frequencies(t, y, dy, num, seed, chains):
-    """``num`` frequencies for each chain (C, num), drawn from the 95 % highest-density set of its light curve's periodogram; NaN
-    where there is none.  A chain's draws depend on its own light curve and number alone, not on the others' sampling spans."""
+    """``num`` frequencies for each chain (C, num), drawn one after the other from the 95 % highest-density set of its light curve's
+    periodogram, each away from the peaks of the earlier ones; NaN where there is none.  A chain's draws depend on its own light curve and number alone, not on the others' sampling spans."""
     from .lombscargle import draw_frequencies
     u = torch.as_tensor(np.stack([np.random.default_rng([seed, 104729, c]).random(num) for c in chains]), device=y.device)
     first, last = t.amin(-1), t.amax(-1)
     one_span = bool(((first == first[0]) & (last == last[0])).all())
     rows = [slice(None)] if one_span else [slice(c, c + 1) for c in range(y.shape[0])]
-    return torch.cat([draw_frequencies(t[r], y[r], None if dy is None else dy[r], u[r], top_p=0.95)[0] for r in rows]).cpu().numpy()
+    return torch.cat([draw_frequencies(t[r], y[r], None if dy is None else dy[r], u[r], top_p=0.95, distinct=True)[0] for r in rows]).cpu().numpy()
 
 
 def _checked_starts(pot, seed, chains, total, world, group):
@@ -571,9 +571,10 @@ def run_mcmc(x, y, noise=None, num_mixtures=4, sampler="NUTS", num_samples=500, 
     (``batch.shard_bounds``), each rank advances its chains with batched evaluations on its own GPU, and one
     ``all_gather`` of the draws closes the run (the only collective, but for one of a flag per chain before starts from the
     periodogram).  ``initial_values``: a dictionary of sites, None (pyro's
-    uniform start) or ``"periodogram"`` -- the same, but every chain's mixture means start on frequencies drawn from the 95 %
-    highest-density set of its Lomb-Scargle periodogram, so that the chains start on the light curve's own peaks and not all on
-    the same one (one input dimension; GPU).  Returns pyro-style ``{site name: draws}`` with
+    uniform start) or ``"periodogram"`` -- the same, but a chain's mixture means start on that many different peaks of its light
+    curve's Lomb-Scargle periodogram (one input dimension; GPU): each is drawn from the 95 % highest-density set of what the earlier
+    ones leave (:func:`pgmuvi_amd.lombscargle.draw_frequencies`, ``distinct``).  Chains differ where the data leave a choice; a clear
+    period is the first start of all of them.  Returns pyro-style ``{site name: draws}`` with
     chains flattened unless ``group_by_chain``, plus ``"_diagnostics"``.
     """
     import torch.distributed as dist

@@ -4,7 +4,7 @@ numbers the caller gives.
 The reference seeds a fit from the highest peaks of a periodogram (``pgmuvi/lightcurve.py:5516-5541``), so every start is the
 same one.  A periodogram is also a posterior over the frequency (:func:`pgmuvi_amd.lombscargle.draw_frequencies`), and starts
 drawn from it differ in proportion to what the data say: top-p keeps the highest-density set, min-p a likelihood ratio,
-top-k the best grid points, and a temperature above one spreads the starts of several chains
+top-k the best grid points, and a temperature above one flattens it.  The sampler's chains start on such draws
 (:func:`pgmuvi_amd.mcmc.run_mcmc`, ``initial_values="periodogram"``).
 
 There is no CPU path: tensors on the GPU or an error.  Nothing synchronises the host but a setting given as a 0-dim tensor on the

@@ -273,3 +273,65 @@ def test_an_infinite_gradient_gives_every_loop_the_same_step(dev, n, optim):
                 assert torch.equal(p.detach(), start[k]), (loop, k)
         ends.append(_losses(r))
     assert np.allclose(ends[0], ends[1], rtol=1e-9, atol=0) and np.allclose(ends[0], ends[2], rtol=1e-9, atol=0)
+
+
+def _apart(f, baseline):
+    """Smallest distance of two frequencies of each row, in peak widths (1 / baseline)."""
+    f = np.sort(np.asarray(f), axis=-1)
+    return np.diff(f, axis=-1).min(-1) * baseline
+
+
+@pytest.mark.parametrize("n", [89, 300, 1000])
+def test_distinct_frequencies_are_drawn_from_what_the_earlier_ones_leave(dev, n):
+    """The light curves have a clear period: 0.95 of the odds lie in one or two grid points."""
+    B, S = 3, 6
+    t, y, e = _curves(dev, B, n)
+    t = (t - t.amin(1, keepdim=True)) / (t.amax(1, keepdim=True) - t.amin(1, keepdim=True)) * 3450.0     # (one span)
+    u = torch.as_tensor(np.random.default_rng(n).random((B, S)), device=dev)
+    plain, _, grid = L.draw_frequencies(t, y, e, u, top_p=0.95)
+    assert (_apart(plain.cpu(), 3450.0) < 1.0).all()             # (with repetition: the same peak again)
+    odds = (-0.5 * (n - 3) * torch.log1p(-L.periodogram_batched(t, y, e, grid).clamp(max=1 - 2.0 ** -52))).cpu().numpy()
+    for kw in (dict(top_p=0.95), dict(temperature=5.0, min_p=1e-3), dict(temperature=0.0)):
+        f, lp, _ = L.draw_frequencies(t, y, e, u, distinct=True, **kw)
+        assert (_apart(f.cpu(), 3450.0) > 1.0).all()
+        for b in range(B):
+            left = odds[b].copy()
+            for s in range(S):
+                idx, want = oracle.draw_row(left, u[b, s:s + 1].cpu().numpy(), **kw)
+                assert float(f[b, s]) == float(grid[int(idx[0])]), (b, s)
+                assert abs(float(lp[b, s]) - want[0]) <= 1e-9 * max(1.0, abs(want[0]))       # (odds of hundreds, log1p on two machines)
+                left[max(0, idx[0] - 5):idx[0] + 6] = -math.inf
+    assert L.draw_frequencies(t, y, e, u[:, :0], distinct=True)[0].shape == (B, 0)
+    dead, lp, _ = L.draw_frequencies(t, torch.zeros_like(y), e, u, distinct=True)
+    assert bool(torch.isnan(dead).all()) and bool((lp == -math.inf).all())
+
+
+def test_more_distinct_frequencies_than_there_are_begin_again(dev):
+    t, y, e = _curves(dev, 2, 8)
+    t = (t - t.amin(1, keepdim=True)) / (t.amax(1, keepdim=True) - t.amin(1, keepdim=True)) * 100.0
+    u = torch.as_tensor(np.random.default_rng(1).random((2, 60)), device=dev)
+    f, lp, grid = L.draw_frequencies(t, y, e, u, distinct=True)
+    assert grid.numel() < 60 * 6 and bool(torch.isfinite(f).all()) and bool((lp <= 0).all())
+    first = grid.numel() // 11                                   # (a draw takes at most eleven grid points away)
+    assert (_apart(f[:, :first].cpu(), 100.0) > 1.0).all()
+
+
+@pytest.mark.parametrize("n", [89, 300, 1000])
+def test_the_mixtures_of_a_chain_start_on_different_peaks(dev, n):
+    t, y, e = _curves(dev, 3, n)
+    span = (t.amax(1) - t.amin(1)).cpu().numpy()
+    chains, Q = 8, 4
+    for b in range(3):
+        f = mcmc._start_frequencies(t[b].expand(chains, n), y[b].expand(chains, n), e[b].expand(chains, n), Q, 5, range(chains))
+        assert f.shape == (chains, Q) and (_apart(f, span[b]) > 1.0).all()
+
+
+def test_chains_differ_where_the_data_leave_a_choice(dev):
+    """Noise alone: 0.95 of the odds of the first draw are spread over 260 of 750 grid points, the largest share is 0.36."""
+    n, chains, Q = 60, 8, 4
+    rng = np.random.default_rng(4)
+    t = torch.as_tensor(np.sort(rng.uniform(0, 1000.0, n)), device=dev).expand(chains, n)
+    y = torch.as_tensor(rng.normal(size=n), device=dev).expand(chains, n)
+    f = mcmc._start_frequencies(t, y, None, Q, 5, range(chains))
+    assert len(np.unique(f[:, 0])) >= 3 and len(np.unique(np.sort(f, axis=1), axis=0)) >= 6
+    assert (_apart(f, float(t.max() - t.min())) > 1.0).all()

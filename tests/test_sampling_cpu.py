@@ -74,3 +74,9 @@ def test_a_start_that_does_not_exist_is_refused():
     from pgmuvi_amd import mcmc
     with pytest.raises(ValueError, match="initial_values"):
         mcmc.run_mcmc(torch.zeros(5), torch.zeros(5), initial_values="peaks")
+
+
+def test_distinct_frequencies_need_numbers_per_light_curve():
+    from pgmuvi_amd.lombscargle import draw_frequencies
+    with pytest.raises(ValueError, match=r"\(B, S\)"):
+        draw_frequencies(torch.zeros(2, 9), torch.zeros(2, 9), None, torch.zeros(2), distinct=True)
