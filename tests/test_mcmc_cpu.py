@@ -238,3 +238,43 @@ def test_a_chain_without_a_start_is_an_error_on_every_rank(tmp_path, how):
     assert "chains [2]" in got[0] and got[0].startswith("ValueError")
     assert got[1].startswith("ZeroDivisionError") if how == "raises" else got[1] == got[0]
     assert all(p.exitcode == 0 for p in procs)
+
+
+@pytest.mark.parametrize("one_curve", [True, False])
+def test_drawn_frequencies_are_where_the_sampler_starts(monkeypatch, one_curve):
+    """What ``_start_frequencies`` returns (the periodogram is the GPU's: numbers of this test's own) arrives in the sampler's initial
+    state as the mixture means of its chain, and nothing else of the usual start changes."""
+    import _oracle_backend as ob
+    C, Q, n = 3, 2, 20
+    x, y, nz = _lightcurves(C, n)
+    args = (x[0], y[0], nz[0]) if one_curve else (x, y, nz)
+    freqs = 0.01 * (1.0 + np.arange(C * Q).reshape(C, Q))
+    seen, asked = [], []
+
+    class Stop(Exception):
+        pass
+
+    def sample(pot, z0, *a, **kw):
+        seen.append((pot, np.array(z0)))
+        raise Stop
+
+    def starts(t, yy, dy, num, seed, chains):
+        asked.append((t.clone(), yy.clone(), dy.clone(), num, seed, list(chains)))
+        return freqs
+
+    monkeypatch.setattr(mcmc, "sample", sample)
+    monkeypatch.setattr(mcmc, "_start_frequencies", starts)
+    for init in ("periodogram", None):
+        with pytest.raises(Stop):
+            mcmc.run_mcmc(*args, num_mixtures=Q, num_chains=C, seed=11, initial_values=init, compute=ob.mll_value_grad)
+    (pot, drawn), (_, usual) = seen
+    means = pot.slices()["covar_module.mixture_means_prior"]
+    assert np.allclose(pot.constrain(drawn)["covar_module.mixture_means_prior"].reshape(C, Q), freqs, rtol=1e-15, atol=0)
+    rest = np.ones(pot.P, dtype=bool)
+    rest[means] = False
+    assert np.array_equal(drawn[:, rest], usual[:, rest]) and not np.any(drawn[:, means] == usual[:, means])
+    (t, yy, dy, num, seed, chains), = asked                      # (asked once: the light curves, their errors, one number per mixture)
+    want = (torch.stack([v] * C) if one_curve else v for v in (args[0], args[1], args[2]))
+    for got, v in zip((t, yy, dy ** 2), want):
+        assert torch.allclose(got, v.reshape(C, n), rtol=1e-15, atol=0)
+    assert (num, seed, chains) == (Q, 11, [0, 1, 2])
