@@ -16,10 +16,14 @@
 // What bounds it (MI355X; a copy moves 4.9 TB/s, so that reading a row once is the floor of all but the smallest calls).
 //   4096 x 51200 fp32, top_k 50 and top_p 0.9, one draw: 206 us, 4.1 TB/s of the one pass that reads everything (171 us at the
 //     copy's rate); the list and the draw overlap with other rows' loads.  Not truncated: 280 us, the exponentials of 2.1e8 entries.
-//   512 x 25600 fp64, top_p 0.95, four draws: 91 us against 21 for the bytes.  A row is one workgroup, two of them share a CU, and
-//     the phases follow each other: highest values 12 us, bins 20 (exponential and two LDS atomics an entry), the cut's entries and
-//     the cells' weights 19, the sort 3, the draws and waits the rest.  min_p or nothing instead of top_p: 32 us.
-//   1 x 204800 fp64, min_p 0.02, 1000 draws: 16 us on the GPU, three launches of 3 to 8 us; their bytes take 0.3.
+//   512 x 25600 fp64, top_p 0.95, four draws: 91 us against 21 for the bytes.  A row is one workgroup and all of them are on the chip at
+//     once, two to a CU, so that the call takes as long as its slowest row.  Stamped (which adds 5 us), a row takes 46 us where a few
+//     peaks hold the 0.95 and 95 where noise does, 67 in the mean: highest values 13 us, waiting for each other and clearing the bins 4,
+//     bins 23 (exponential and three LDS atomics an entry: count and two words) and 5 of waiting, the bin 3, the cut's entries and the
+//     cells' weights 9 and 2 of waiting, the sort 1, joining the list to the cells 3, scan and draws 4.  min_p or nothing instead of
+//     top_p: 32 us.
+//   1 x 204800 fp64, min_p 0.02, 1000 draws: 15 us on the GPU (calls back to back in a graph), three launches one after the other; their
+//     bytes take 0.3.
 //   Short calls (1 x 1113 fp64, 8 draws): 8 us, one launch whose phases wait for each other.
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
@@ -160,7 +164,9 @@ template <class F> struct Row {
   __device__ __forceinline__ int64_t width() const { return (int64_t)mult * (U * UNIT); }
   __device__ __forceinline__ double value(int64_t i) const { return (double)F::widen(x[i * stride]); }
   __device__ __forceinline__ double z(double l) const { return l == best ? 0.0 : (l - best) / t; }
-  // (where the best value is infinite only infinite ones are kept: their difference, a NaN, is clamped to zero here)
+  // (the product with 1 / T, one instruction against the ten or so of z's quotient: one rounding more, 2^-53 |z| relative to the weight.
+  // The log-probabilities are z's.  Where the best value is infinite only infinite ones are kept: their difference, a NaN, is clamped
+  // to zero here)
   __device__ __forceinline__ double weight(double l) const { return exp_neg(__builtin_fmin((l - best) * per_t, 0.0)); }
   // this lane's entries of the group of U loads number g: load q's entry e is number first(g) + q UNIT + e; behind the end -inf
   __device__ __forceinline__ int64_t first(int64_t g) const { return g * (U * UNIT) + (threadIdx.x & 63) * VEC; }
@@ -1209,8 +1215,8 @@ template <class F> void launch(DrawArgs& A, const Plan& p, int64_t rows, hipStre
     const int shares = (int)std::max<int64_t>(1, std::min<int64_t>(p.max_cells / 8, 1024 / rows));
     hipLaunchKernelGGL(k_lots<F>, dim3((unsigned)(rows * shares)), dim3(Long::NT), 0, st, A, shares, cuts);
   }
-  // a wavefront makes one draw at a time (with lots: 64): one each while that leaves the chip room (1 x 204800, 1000 draws: 13 us
-  // against 16 with two; 100 x 20000, 40: 23 against 29), else two, or more where that fills it anyway
+  // a wavefront makes one draw at a time (with lots: 64): one each while that leaves the chip room (calls back to back in a graph,
+  // 1 x 204800, 1000 draws: 15 us against 18 with two; 100 x 20000, 40: 17 against 21), else two, or more where that fills it anyway
   const int at_once = p.lots ? Long::NT : A.draws * rows <= 4096 ? 8 : 16;
   const int per = (int)std::max<int64_t>(at_once, (A.draws * rows / 1024 + at_once - 1) / at_once * at_once);
   const int blocks = (int)((A.draws + per - 1) / per);

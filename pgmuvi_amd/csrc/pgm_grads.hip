@@ -12,8 +12,10 @@
 // launch.  No atomics: every result is reproducible bit for bit.
 //
 // What bounds it: memory, at a copy's rate of 4.9 TB/s on this card (reading alone goes faster).  The norm of 2.1 GB fp64: 358 us,
-// 6.0 TB/s.  Clipping 1.07 GB bf16 in place: k_norm_part 217 us (4.9 TB/s) + k_scale 407 (5.3 TB/s of reading and writing); the
-// second read is needed, the set does not fit the caches.  The norm of 64 MB in 61 fp32 tensors: 16 + 4 us on the GPU, 35 with the host's description of them.  4096 members of 64 KB fp64: 105 us, 5.1 TB/s, each read once.
+// 6.0 TB/s.  Clipping 1.07 GB bf16 into other tensors: k_norm_part 221 us (4.9 TB/s) + k_scale 419 (5.1 TB/s of reading and writing);
+// in place 617 together, and 227 where nothing exceeds the limit.  The second read is needed, the set does not fit the caches.  The
+// norm of 64 MB in 61 fp32 tensors: 16 + 4 us on the GPU, 35 with the host's description of them.  4096 members of 64 KB fp64: 105 us,
+// 5.1 TB/s, each read once.
 // Small sets are one launch (the five tensors of a fit, 14 numbers: 6 us on the GPU, 17 with the host).
 //
 // Arithmetic.  All sums are fp64 whatever the tensors' type.  An fp64 square overflows from 1e154 on and vanishes below
