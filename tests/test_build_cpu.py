@@ -67,3 +67,12 @@ def test_a_changed_header_or_source_compiles_again(tree):
     assert tree() >= 1
     os.utime(tree.dir / "include" / "pgmuvi_hip.h", (later + 5, later + 5))
     assert tree() == tree.sources
+
+
+def test_a_copy_elsewhere_is_built_by_the_same_commands(tree, tmp_path):
+    tree()
+    copy = tmp_path / "elsewhere" / "deeper"
+    shutil.copytree(tree.dir / "pkg", copy / "pkg", ignore=shutil.ignore_patterns("build", "*.so"))
+    shutil.copytree(tree.dir / "include", copy / "include")
+    subprocess.run(["make", "-C", str(copy / "pkg" / "csrc"), f"HIPCC={tree.dir / 'cc'}"], check=True, env=dict(os.environ, COUNT=os.devnull), capture_output=True)
+    assert (copy / "pkg" / "libpgmuvi_hip.so").read_text() == (tree.dir / "pkg" / "libpgmuvi_hip.so").read_text()
