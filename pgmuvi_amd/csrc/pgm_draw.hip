@@ -721,7 +721,8 @@ template <class F, class Run> __device__ __forceinline__ int64_t entry_of_lot(co
       const int64_t i = (int64_t)k * PER + e;
       const double w = kept_weight(R, cut, min_p, i);
       r += w;
-      if (w > 0.0) { found = i; if (r > target) break; }         // (else its last kept one: the sums differ by a rounding)
+      // (else its last kept one: the sums differ by a rounding.  So too on the way back, where the lots behind weigh nothing)
+      if (w > 0.0) { found = i; if (step > 0 && r > target) break; }
     }
     k += step;                                                  // (nothing kept in this lot)
     if (k == lots) { step = -1; k = j - 1; }

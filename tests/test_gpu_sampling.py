@@ -415,3 +415,22 @@ def test_settings_that_are_negated_views(dev):
             view = torch.complex(torch.zeros_like(v), -v).conj().imag
             assert view.is_neg() and torch.equal(view, v)
             assert torch.equal(draw_indices(l, u, **{name: view}), draw_indices(l, u, **{name: v}))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, cols, S", [(1, 500, 12), (3, 77, 12), (1030, 900, 12), (9, 30_000, 1200), (2, 90_000, 5000)])
+def test_the_last_kept_entry_at_the_end_of_the_weight(dev, rows, cols, S, dtype):
+    """u within twelve steps of one, and entries that weigh nothing behind the last kept one: that one is drawn, whatever the roundings
+    of the running sums behind it (the one in front of it ends a whole weight, more than 2^-18 of all, earlier)."""
+    u = torch.as_tensor(1.0 - 2.0 ** -53 * (1 + np.arange(S) % 12)[None] * np.ones((rows, 1)), device=dev)
+    rng = np.random.default_rng(cols)
+    flat = torch.full((rows, cols), -7.5, dtype=dtype)
+    few = torch.full((rows, cols), -math.inf, dtype=dtype)
+    few[:, :cols // 3] = torch.as_tensor(np.log(rng.uniform(0.5, 1.0, (rows, cols // 3)))).to(dtype)
+    for l, settings in ((flat, [dict(top_p=0.9), dict(top_p=0.23, temperature=0.3), dict(top_k=cols // 2 + 1), dict(top_k=17)]),
+                        (few, [dict(), dict(min_p=0.7), dict(temperature=1e5), dict(top_p=0.999), dict(top_k=cols // 5)])):
+        for kw in settings:
+            got = draw_indices(l.to(dev), u, **kw)
+            for b in (0, rows - 1):
+                idx, w, _ = oracle.kept_entries(l[b].double().numpy(), **kw)
+                assert (got[b] == int(idx[-1])).all(), (kw, b, int(idx[-1]), got[b][:12].tolist())
