@@ -45,19 +45,22 @@ constexpr double INF = __builtin_inf();
 
 // ---- types of the log-weights.  `wide`: what maxima are formed in; U: loads of a lane that make up a cell (the wavefront's reduction
 // for a cell costs ~35 instructions: over two loads of two fp64 or four fp32 entries each, over one of eight 16-bit ones)
+// (larger: a is never a signalling NaN, b may be one, which the hardware's maximum would return quiet instead of the other operand --
+// compiled with b made quiet in the form of two operands, but not in that of three, hence the canonical b of fp32 and bf16, whose
+// bits are loaded as they are: a quiet NaN loses)
 struct F64 {
   typedef double raw, wide;
   static constexpr int U = 2;
   static constexpr raw absent() { return -__builtin_inf(); }
   static __device__ __forceinline__ wide widen(raw x) { return x; }
-  static __device__ __forceinline__ wide larger(wide a, wide b) { return __builtin_fmax(a, b); }        // (a NaN loses)
+  static __device__ __forceinline__ wide larger(wide a, wide b) { return __builtin_fmax(a, b); }
 };
 struct F32 {
   typedef float raw, wide;
   static constexpr int U = 2;
   static constexpr raw absent() { return -__builtin_inff(); }
   static __device__ __forceinline__ wide widen(raw x) { return x; }
-  static __device__ __forceinline__ wide larger(wide a, wide b) { return __builtin_fmaxf(a, b); }
+  static __device__ __forceinline__ wide larger(wide a, wide b) { return __builtin_fmaxf(a, __builtin_canonicalizef(b)); }
 };
 template <int F16BIT> struct Half {                              // bf16 (0) and fp16 (1)
   typedef uint16_t raw; typedef float wide;
@@ -67,7 +70,7 @@ template <int F16BIT> struct Half {                              // bf16 (0) and
     if constexpr (F16BIT) { __half_raw r; r.x = b; return __half2float(__half(r)); }
     else return __uint_as_float((uint32_t)b << 16);
   }
-  static __device__ __forceinline__ wide larger(wide a, wide b) { return __builtin_fmaxf(a, b); }
+  static __device__ __forceinline__ wide larger(wide a, wide b) { return __builtin_fmaxf(a, F16BIT ? b : __builtin_canonicalizef(b)); }
 };
 // a bound not above v, in the type comparisons are cheap in
 __device__ __forceinline__ void bound_below(double v, double& w) { w = v; }

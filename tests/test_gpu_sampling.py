@@ -434,3 +434,24 @@ def test_the_last_kept_entry_at_the_end_of_the_weight(dev, rows, cols, S, dtype)
             for b in (0, rows - 1):
                 idx, w, _ = oracle.kept_entries(l[b].double().numpy(), **kw)
                 assert (got[b] == int(idx[-1])).all(), (kw, b, int(idx[-1]), got[b][:12].tolist())
+
+
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=4), dict(top_k=300), dict(top_p=0.7), dict(min_p=0.2), dict(temperature=0.0)], ids=str)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_signalling_nans_are_never_drawn_and_hide_nothing(dev, dtype, settings):
+    """Every NaN bit pattern is a masked entry: the hardware's maximum returns a NaN of a signalling one instead of its other operand."""
+    bits, patterns = {torch.float64: (torch.int64, (0x7FF0000000000001, -0x000FFFFFFFFFFFFF)), torch.float32: (torch.int32, (0x7F800001, -0x007FFFFF)),
+                      torch.bfloat16: (torch.int16, (0x7F81, -0x007F)), torch.float16: (torch.int16, (0x7C01, -0x03FF))}[dtype]
+    for B, V in ((1, 5), (3, 700), (2, 9000), (520, 20_001), (1030, 900), (1, 300_000)):
+        rng = np.random.default_rng(V)
+        l = _rows(B, V, dtype, V)
+        for share, pattern in ((0.05, patterns[0]), (0.3, patterns[1])):
+            l.view(bits)[torch.as_tensor(rng.random((B, V)) < share)] = pattern
+        l[0, 3] = 2.0                                            # (not all of a short row)
+        u = torch.as_tensor(rng.random((B, 6)))
+        d = torch.empty(B, V, dtype=dtype, device=dev)
+        d.view(bits).copy_(l.view(bits))
+        idx, logp = draw_indices(d, u.to(dev), return_logprob=True, **settings)
+        assert torch.equal(d.view(bits).cpu(), l.view(bits)) and int(idx[0].min()) >= 0
+        some = sorted({0, B // 2, B - 1})
+        _check(l[some], u[some], (idx[some], logp[some]), **settings)
